@@ -266,6 +266,72 @@ int kq_bf16_to_f32_transposed(const uint16_t* src, int64_t rows, int64_t cols, i
 int kq_reconstruct_rotated(const float* wq, const float* su, const float* sv, int64_t k, int64_t n, float* out,
                            void* stream);
 
+/* Element types and activations of the expert-layer operators. */
+#define KQ_BF16 0
+#define KQ_FP16 1
+#define KQ_FP32 2
+#define KQ_ACT_NONE 0
+#define KQ_ACT_RELU 1
+#define KQ_ACT_SILU 2
+#define KQ_ACT_GELU 3          /* z Phi(z), the error-function form */
+
+/*
+ * Products of rows sorted by expert with the experts' matrices (no
+ * counterpart in the reference, which leaves the expert layer to its serving
+ * stack).  Rows offsets[e] .. offsets[e+1] of x [rows x k] belong to expert
+ * e; offsets (int64 [experts+1], non-decreasing, on the device) may be NULL
+ * for one expert.  They are read by the kernels alone, so a captured call
+ * follows new offsets at replay; values outside 0 .. rows are clamped.
+ * W_e [k x n] is any pair of strides of which one is 1 (elements), so both
+ * the EXL [in, out] and the HF [out, in] orientation are taken as stored.
+ * x, W, bias, residual and y have one type (KQ_BF16 or KQ_FP16), products
+ * are summed in fp32 and rounded once.  Bases and strides that are not
+ * multiples of 16 bytes cost one more pass over that operand, into the
+ * workspace.
+ *
+ *     kq_expert_linear:         y = act(x W + b) + residual
+ *       gated (n = 2 n_out):    y = act(x Wg + bg) * (x Wu + bu) + residual
+ *                               (Wg the first n_out columns of W)
+ *     kq_expert_linear_grad_z:  dz from dy [rows x n_out] and the recomputed
+ *                               z; y receives dz [rows x n]
+ *     kq_expert_weight_grad:    dW_e = x_e^T dz_e, in W's strides (every
+ *                               expert is written, zeros where it has no rows)
+ *     kq_expert_bias_grad:      db_e = the column sums of dz_e
+ *
+ * The gradient in x is kq_expert_linear on dz with W's strides exchanged.
+ * Rows of no expert are left as they were, or zeroed with zero_rest.
+ * bias and residual may be NULL.  At most 1024 experts.
+ */
+typedef struct {
+    const void* x;
+    const void* w;
+    const int64_t* offsets;
+    const void* bias;          /* [experts][n], n contiguous */
+    const void* residual;      /* [rows][n_out] */
+    void* y;
+    int64_t rows, k, n, experts;
+    int64_t ldx;
+    int64_t w_stride_e, w_stride_k, w_stride_n;
+    int64_t bias_stride_e, ld_residual, ldy;
+    int32_t dtype, activation, gated, zero_rest;
+} kq_expert_product;
+
+size_t kq_expert_linear_workspace_bytes(const kq_expert_product* p);
+int kq_expert_linear(const kq_expert_product* p, void* workspace, size_t workspace_bytes, void* stream);
+int kq_expert_linear_grad_z(const kq_expert_product* p, const void* dy, int64_t ld_dy, void* workspace,
+                            size_t workspace_bytes, void* stream);
+size_t kq_expert_weight_grad_workspace_bytes(const kq_expert_product* p, const void* dz, int64_t ld_dz);
+int kq_expert_weight_grad(const kq_expert_product* p, const void* dz, int64_t ld_dz, void* dw, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n, int64_t experts,
+                        int dtype, void* db, int64_t db_stride_e, void* stream);
+
+/*
+ * Writes 1 to *out (device int32) if an internal wait of an expert-layer
+ * kernel ran out on this device since the last call, else 0, and clears it.
+ */
+int kq_wait_errors(int32_t* out, void* stream);
+
 /*
  * Roofline probe (no reference counterpart): launches blocks x threads
  * threads that each issue iters*128 independent __hfma2 instructions.  Time

@@ -41,6 +41,13 @@ EXPORTED = (
     "kq_ldlq_step_encode",
     "kq_ldlq_chain_step",
     "kq_reconstruct_rotated",
+    "kq_expert_linear_workspace_bytes",
+    "kq_expert_linear",
+    "kq_expert_linear_grad_z",
+    "kq_expert_weight_grad_workspace_bytes",
+    "kq_expert_weight_grad",
+    "kq_expert_bias_grad",
+    "kq_wait_errors",
 )
 
 KQ_CHAIN_MAX_ITEMS = 64
@@ -53,6 +60,19 @@ class ChainItem(ctypes.Structure):
                 ("size_n", ctypes.c_int64), ("r0", ctypes.c_int64), ("end", ctypes.c_int64),
                 ("tile_col0", ctypes.c_int64), ("n_tiles", ctypes.c_int64), ("labels", ctypes.c_void_p),
                 ("K", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+
+class ExpertProduct(ctypes.Structure):
+    """kq_expert_product of include/kq_b200.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("y", ctypes.c_void_p), ("rows", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("n", ctypes.c_int64), ("experts", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("w_stride_e", ctypes.c_int64), ("w_stride_k", ctypes.c_int64), ("w_stride_n", ctypes.c_int64),
+                ("bias_stride_e", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ldy", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("gated", ctypes.c_int32),
+                ("zero_rest", ctypes.c_int32)]
+
 
 _lib = None
 _lock = threading.Lock()
@@ -96,6 +116,16 @@ def load() -> ctypes.CDLL:
         L.kq_hessian_workspace_bytes.argtypes = [I64, I64, I]
         L.kq_hessian_workspace_bytes.restype = SZ
         L.kq_accumulate_hessian.argtypes = [P, P, I64, I64, I64, P, I64, I, P, SZ, P, P]
+        EP = ctypes.POINTER(ExpertProduct)
+        L.kq_expert_linear_workspace_bytes.argtypes = [EP]
+        L.kq_expert_linear_workspace_bytes.restype = SZ
+        L.kq_expert_linear.argtypes = [EP, P, SZ, P]
+        L.kq_expert_linear_grad_z.argtypes = [EP, P, I64, P, SZ, P]
+        L.kq_expert_weight_grad_workspace_bytes.argtypes = [EP, P, I64]
+        L.kq_expert_weight_grad_workspace_bytes.restype = SZ
+        L.kq_expert_weight_grad.argtypes = [EP, P, I64, P, P, SZ, P]
+        L.kq_expert_bias_grad.argtypes = [P, I64, P, I64, I64, I64, I, P, I64, P]
+        L.kq_wait_errors.argtypes = [P, P]
         for name in EXPORTED:
             f = getattr(L, name)
             if name not in ("kq_last_error", "kq_viterbi_workspace_bytes", "kq_hessian_workspace_bytes") and f.restype is ctypes.c_int:
@@ -463,3 +493,54 @@ def reconstruct_rotated(wq: torch.Tensor, su: torch.Tensor, sv: torch.Tensor) ->
                                              _stream(wq.device)), "kq_reconstruct_rotated")
     stats.launches += 1
     return out
+
+
+def scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Workspace of one call, from torch's allocator: ordered with the call's stream, and inside a captured graph
+    the graph's own, so that graphs replayed side by side share none."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def expert_linear(p: ExpertProduct, device: torch.device) -> None:
+    with torch.cuda.device(device):
+        n = load().kq_expert_linear_workspace_bytes(p)
+        ws = scratch(n, device)
+        _check(load().kq_expert_linear(p, None if ws is None else ws.data_ptr(), n, _stream(device)), "kq_expert_linear")
+    stats.launches += 1
+
+
+def expert_linear_grad_z(p: ExpertProduct, dy: torch.Tensor, device: torch.device) -> None:
+    with torch.cuda.device(device):
+        n = load().kq_expert_linear_workspace_bytes(p)
+        ws = scratch(n, device)
+        _check(load().kq_expert_linear_grad_z(p, dy.data_ptr(), dy.stride(0), None if ws is None else ws.data_ptr(), n,
+                                              _stream(device)), "kq_expert_linear_grad_z")
+    stats.launches += 1
+
+
+def expert_weight_grad(p: ExpertProduct, dz: torch.Tensor, dw: torch.Tensor, device: torch.device) -> None:
+    with torch.cuda.device(device):
+        n = load().kq_expert_weight_grad_workspace_bytes(p, dz.data_ptr(), dz.stride(0))
+        ws = scratch(n, device)
+        _check(load().kq_expert_weight_grad(p, dz.data_ptr(), dz.stride(0), dw.data_ptr(),
+                                            None if ws is None else ws.data_ptr(), n, _stream(device)),
+               "kq_expert_weight_grad")
+    stats.launches += 1
+
+
+def expert_bias_grad(dz: torch.Tensor, offsets: torch.Tensor | None, db: torch.Tensor, dtype: int) -> None:
+    device = dz.device
+    with torch.cuda.device(device):
+        _check(load().kq_expert_bias_grad(dz.data_ptr(), dz.stride(0), None if offsets is None else offsets.data_ptr(),
+                                          dz.shape[0], dz.shape[1], db.shape[0], dtype, db.data_ptr(), db.stride(0),
+                                          _stream(device)), "kq_expert_bias_grad")
+    stats.launches += 1
+
+
+def check_wait_errors(device: torch.device) -> None:
+    """Raise if a bounded wait inside an expert-layer kernel ran out since the last call (one device sync)."""
+    out = torch.empty((), dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        _check(load().kq_wait_errors(out.data_ptr(), _stream(device)), "kq_wait_errors")
+    if int(out.item()):
+        raise KQError("an internal wait of an expert-layer kernel timed out; results since the last check are invalid")

@@ -1,0 +1,163 @@
+"""The expert layer around the encode: products with the experts' matrices, and their gradients.
+
+Rows are sorted by expert: rows ``offsets[e] .. offsets[e + 1]`` of ``x`` belong to expert e (``offsets``: int64
+[experts + 1], non-decreasing, on the GPU).  The kernels read the offsets, the host never does, so no call waits for
+the GPU and a call captured into a graph follows new offsets at replay.  Rows before ``offsets[0]`` and from
+``offsets[-1]`` on belong to no expert: a fresh output holds zeros there, an ``out`` given by the caller keeps what
+it had.
+
+Matrices are [in, out] (EXL orientation), as the encoder takes and reconstructs them; a transposed view of the HF
+orientation ([out, in]) is taken as it is.  Operands are bf16 or fp16, sums are fp32, each result is rounded once.
+Bases, strides and widths that are not multiples of 16 bytes are accepted and cost one more pass over that operand.
+
+The results carry no autograd history; :func:`expert_linear_grad` computes the gradients.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _operand(t: torch.Tensor, name: str, dims: int, dtype: torch.dtype, device: torch.device) -> None:
+    if not t.is_cuda:
+        raise _native.KQError(f"{name} must be a CUDA tensor (kquant_b200 has no CPU path)")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.ndim != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {t.ndim}")
+
+
+def _rows_operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, device: torch.device) -> None:
+    _operand(t, name, 2, dtype, device)
+    if t.shape != (rows, width):
+        raise ValueError(f"{name} must be [{rows}, {width}], got {list(t.shape)}")
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} needs unit stride along its last dimension")
+
+
+def _check_offsets(offsets: torch.Tensor | None, experts: int, device: torch.device) -> None:
+    if offsets is None:
+        if experts != 1:
+            raise ValueError("several experts need offsets")
+        return
+    _operand(offsets, "offsets", 1, torch.int64, device)
+    if offsets.numel() != experts + 1 or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be {experts + 1} contiguous values for {experts} experts")
+
+
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _product(x, w, offsets, bias, activation, gated) -> _native.ExpertProduct:
+    """The checked operands that every product of these shares."""
+    if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor):
+        raise TypeError("x and w must be tensors")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
+    dev = x.device
+    _operand(x, "x", 2, x.dtype, dev)
+    _operand(w, "w", 3, x.dtype, dev)
+    E, k, n = w.shape
+    if min(E, k, n) < 1:
+        raise ValueError(f"w must not be empty, got {list(w.shape)}")
+    _rows_operand(x, "x", x.shape[0], k, x.dtype, dev)
+    if w.stride(1) != 1 and w.stride(2) != 1 and k > 1 and n > 1:
+        raise ValueError("w needs unit stride along its in or its out dimension")
+    _check_offsets(offsets, E, dev)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {[a for a in _ACTIVATIONS]}, got {activation!r}")
+    if gated and n % 2:
+        raise ValueError("a gated product needs an even out dimension (gate, then up)")
+    if bias is not None:
+        _operand(bias, "bias", 2, x.dtype, dev)
+        if bias.shape != (E, n) or (n > 1 and bias.stride(1) != 1):
+            raise ValueError(f"bias must be [{E}, {n}] with unit stride along its last dimension, got {list(bias.shape)}")
+    p = _native.ExpertProduct()
+    p.x, p.w, p.offsets, p.bias = x.data_ptr(), w.data_ptr(), _ptr(offsets), _ptr(bias)
+    p.rows, p.k, p.n, p.experts = x.shape[0], k, n, E
+    p.ldx = x.stride(0)
+    p.w_stride_e, p.w_stride_k, p.w_stride_n = w.stride()
+    p.bias_stride_e = 0 if bias is None else bias.stride(0)
+    p.dtype, p.activation, p.gated = _DTYPES[x.dtype], _ACTIVATIONS[activation], int(bool(gated))
+    return p
+
+
+def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *, bias: torch.Tensor | None = None,
+                  activation: str | None = None, gated: bool = False, residual: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[r] = act(x[r] w[e] + bias[e]) + residual[r] for the rows r of each expert e.
+
+    x [rows, k], w [experts, k, n], bias [experts, n], residual and y [rows, n].  ``gated``: w holds the gate's
+    columns and then the up projection's, y = act(gate) * up + residual has n / 2 columns.  ``activation``: None,
+    "relu", "silu" or "gelu" (the error-function form).  ``out`` may be the residual itself.
+    """
+    p = _product(x, w, offsets, bias, activation, gated)
+    n_out = p.n // 2 if gated else p.n
+    if residual is not None:
+        _rows_operand(residual, "residual", p.rows, n_out, x.dtype, x.device)
+        p.residual, p.ld_residual = residual.data_ptr(), residual.stride(0)
+    if out is None:
+        out = torch.empty((p.rows, n_out), dtype=x.dtype, device=x.device)
+        p.zero_rest = 1
+    else:
+        _rows_operand(out, "out", p.rows, n_out, x.dtype, x.device)
+    if p.rows:
+        p.y, p.ldy = out.data_ptr(), out.stride(0)
+        _native.expert_linear(p, x.device)
+    return out
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
+           gated: bool = False, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x w + bias) + residual with one matrix w [k, n] and bias [n]; see :func:`expert_linear`."""
+    if isinstance(w, torch.Tensor) and w.ndim != 2:
+        raise ValueError(f"w must have 2 dimensions, got {w.ndim}")
+    if bias is not None and bias.ndim != 1:
+        raise ValueError(f"bias must have 1 dimension, got {bias.ndim}")
+    return expert_linear(x, w[None], None, bias=None if bias is None else bias[None], activation=activation, gated=gated,
+                         residual=residual, out=out)
+
+
+def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *,
+                       bias: torch.Tensor | None = None, activation: str | None = None, gated: bool = False,
+                       need_dx: bool = True, need_dw: bool = True):
+    """Gradients (dx, dw, dbias) of :func:`expert_linear` for dy, the gradient of its result.
+
+    The pre-activation z = x w + bias is recomputed where the activation needs it; dz (one rounding to the operands'
+    type) then feeds dx = dz w^T, dw[e] = x_e^T dz_e and dbias[e] = sum dz_e.  dw has w's layout; an expert without
+    rows gets zeros.  dbias is None without a bias, dx and dw where they are not asked for.  The residual's gradient
+    is dy itself.
+    """
+    p = _product(x, w, offsets, bias, activation, gated)
+    dev, dt = x.device, x.dtype
+    _rows_operand(dy, "dy", p.rows, p.n // 2 if gated else p.n, dt, dev)
+    E, k, n = w.shape
+    dz = dy
+    if p.rows and (gated or activation is not None):
+        dz = torch.empty((p.rows, -(-n // 8) * 8), dtype=dt, device=dev)[:, :n]
+        p.y, p.ldy = dz.data_ptr(), dz.stride(0)
+        _native.expert_linear_grad_z(p, dy, dev)
+    elif gated:
+        dz = dy.new_empty((0, n))
+    dx = dw = db = None
+    if need_dx:
+        dx = expert_linear(dz, w.transpose(1, 2), offsets)
+    if need_dw:
+        n_major = not (w.stride(2) != 1 and w.stride(1) == 1)
+        dw = torch.empty((E, k, n), dtype=dt, device=dev) if n_major else \
+            torch.empty((E, n, k), dtype=dt, device=dev).transpose(1, 2)
+        p.w_stride_e, p.w_stride_k, p.w_stride_n = k * n, n if n_major else 1, 1 if n_major else k
+        p.gated, p.activation = 0, 0
+        _native.expert_weight_grad(p, dz, dw, dev)
+    if bias is not None:
+        db = torch.empty((E, n), dtype=dt, device=dev)
+        _native.expert_bias_grad(dz, offsets, db, p.dtype)
+    return dx, dw, db

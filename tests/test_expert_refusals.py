@@ -1,0 +1,88 @@
+"""What the expert-layer operators refuse, checked on the host before any launch."""
+import ctypes
+
+import pytest
+import torch
+
+from kquant_b200 import _native, experts
+
+
+class FakeCuda(torch.Tensor):
+    """A CPU tensor that says it is on a GPU: the argument checks run, no kernel is reached."""
+    is_cuda = True
+
+
+def fake(*shape, dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype).as_subclass(FakeCuda)
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(x=torch.zeros(4, 8, dtype=torch.bfloat16)), _native.KQError, "CUDA"),
+    (dict(x=fake(4, 8, dtype=torch.float32)), TypeError, "bfloat16 or torch.float16"),
+    (dict(w=fake(2, 8, 6, dtype=torch.float16)), TypeError, "w must be"),
+    (dict(w=fake(8, 6)), ValueError, "3 dimensions"),
+    (dict(w=fake(2, 9, 6)), ValueError, "x must be"),
+    (dict(w=fake(2, 8, 0)), ValueError, "empty"),
+    (dict(w=fake(2, 16, 12)[:, ::2, ::2]), ValueError, "unit stride"),
+    (dict(x=fake(4, 16)[:, ::2]), ValueError, "unit stride"),
+    (dict(offsets=None), ValueError, "offsets"),
+    (dict(offsets=torch.zeros(2, dtype=torch.int64).as_subclass(FakeCuda)), ValueError, "3 contiguous"),
+    (dict(offsets=torch.zeros(3, dtype=torch.int32).as_subclass(FakeCuda)), TypeError, "int64"),
+    (dict(offsets=torch.zeros(3, dtype=torch.int64)), _native.KQError, "CUDA"),
+    (dict(activation="tanh"), ValueError, "activation"),
+    (dict(w=fake(2, 8, 7), gated=True), ValueError, "even"),
+    (dict(bias=fake(2, 5)), ValueError, "bias"),
+    (dict(bias=fake(6)), ValueError, "2 dimensions"),
+    (dict(residual=fake(4, 5)), ValueError, "residual"),
+    (dict(residual=fake(4, 6), gated=True), ValueError, "residual"),
+    (dict(out=fake(3, 6)), ValueError, "out"),
+    (dict(out=fake(4, 6, dtype=torch.float32)), TypeError, "out"),
+])
+def test_expert_linear_refuses(change, error, match):
+    args = dict(x=fake(4, 8), w=fake(2, 8, 6), offsets=torch.zeros(3, dtype=torch.int64).as_subclass(FakeCuda))
+    args.update(change)
+    with pytest.raises(error, match=match):
+        experts.expert_linear(**args)
+
+
+def test_linear_and_gradient_refuse():
+    with pytest.raises(ValueError, match="2 dimensions"):
+        experts.linear(fake(4, 8), fake(1, 8, 6))
+    with pytest.raises(ValueError, match="1 dimension"):
+        experts.linear(fake(4, 8), fake(8, 6), bias=fake(1, 6))
+    with pytest.raises(ValueError, match="dy"):
+        experts.expert_linear_grad(fake(4, 5), fake(4, 8), fake(1, 8, 6), None)
+
+
+def _product(**kw):
+    p = _native.ExpertProduct(x=64, w=64, y=64, rows=4, k=8, n=6, experts=1, ldx=8, w_stride_e=48, w_stride_k=6, w_stride_n=1,
+                              ldy=6)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(rows=-1), -1), (dict(k=0), -1), (dict(n=0), -1), (dict(experts=0), -1), (dict(experts=1025, offsets=64), -1),
+    (dict(experts=2), -1), (dict(dtype=2), -1), (dict(activation=4), -1), (dict(gated=1, n=7), -1), (dict(w_stride_n=2), -1),
+    (dict(x=None), -1), (dict(y=None), -1), (dict(ldy=5), -1), (dict(rows=1 << 31), -1), (dict(w=65), -4),
+    (dict(), -2),        # 6 columns are not a multiple of 16 bytes: a workspace is needed
+])
+def test_c_entry_refuses(change, status):
+    """Status codes of the C entry points; the pointers are never followed."""
+    L, p = _native.load(), _product(**change)
+    assert L.kq_expert_linear(ctypes.byref(p), None, 0, None) == status
+    assert L.kq_last_error()
+
+
+def test_c_entries_refuse_null():
+    L = _native.load()
+    assert L.kq_expert_linear(None, None, 0, None) == -1
+    assert L.kq_expert_linear_grad_z(None, None, 0, None, 0, None) == -1
+    assert L.kq_expert_weight_grad(None, None, 0, None, None, 0, None) == -1
+    assert L.kq_expert_weight_grad(ctypes.byref(_product()), None, 0, 64, None, 0, None) == -1
+    assert L.kq_expert_bias_grad(None, 0, None, 4, 8, 1, 0, None, 0, None) == -1
+    assert L.kq_wait_errors(None, None) == -1
+    assert L.kq_expert_linear_workspace_bytes(None) == 0
+    # Nothing to do: no pointer is needed.
+    assert L.kq_expert_linear(ctypes.byref(_product(rows=0, x=None, y=None)), None, 0, None) == 0
