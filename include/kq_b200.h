@@ -327,6 +327,26 @@ int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t* offsets, i
                         int dtype, void* db, int64_t db_stride_e, void* stream);
 
 /*
+ * Calibration Hessians of all experts at once (kquant/capture.py:713-730,
+ * _accumulate_hessian, for every expert of a layer):
+ *     H_e (+)= sum_t w_t x[i_t] x[i_t]^T     den_e = sum_t w_t
+ * over slots t = offsets[e] .. offsets[e+1] of `rows` slots (offsets as for
+ * kq_expert_linear).  x [tokens x dim] (row stride ldx; KQ_BF16, KQ_FP16 or
+ * KQ_FP32); index [rows] (int64) picks the row of each slot, NULL: slot t is
+ * row t; a slot whose index is outside 0 .. tokens counts for nothing.  w
+ * [rows] fp32, NULL: all ones.  H [experts][dim][dim] fp32 (strides h_stride,
+ * ldh), added to when `add`, else overwritten; den [experts] fp64,
+ * overwritten.  fp32 accuracy (exact 16-bit operand terms, rounded fp32
+ * sums); every H_e is exactly symmetric when it starts so.  The workspace
+ * (128-byte aligned) holds the gathered operand rows.
+ */
+size_t kq_expert_hessian_workspace_bytes(int64_t rows, int64_t dim, int64_t experts, int dtype, int weighted);
+int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int64_t dim, int64_t ldx, int dtype,
+                                  const int64_t* index, const float* w, const int64_t* offsets, int64_t rows,
+                                  int64_t experts, float* H, int64_t h_stride, int64_t ldh, int add, double* den,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Writes 1 to *out (device int32) if an internal wait of an expert-layer
  * kernel ran out on this device since the last call, else 0, and clears it.
  */

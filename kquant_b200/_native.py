@@ -48,6 +48,8 @@ EXPORTED = (
     "kq_expert_weight_grad",
     "kq_expert_bias_grad",
     "kq_wait_errors",
+    "kq_expert_hessian_workspace_bytes",
+    "kq_accumulate_expert_hessians",
 )
 
 KQ_CHAIN_MAX_ITEMS = 64
@@ -126,6 +128,9 @@ def load() -> ctypes.CDLL:
         L.kq_expert_weight_grad.argtypes = [EP, P, I64, P, P, SZ, P]
         L.kq_expert_bias_grad.argtypes = [P, I64, P, I64, I64, I64, I, P, I64, P]
         L.kq_wait_errors.argtypes = [P, P]
+        L.kq_expert_hessian_workspace_bytes.argtypes = [I64, I64, I64, I, I]
+        L.kq_expert_hessian_workspace_bytes.restype = SZ
+        L.kq_accumulate_expert_hessians.argtypes = [P, I64, I64, I64, I, P, P, P, I64, I64, P, I64, I64, I, P, P, SZ, P]
         for name in EXPORTED:
             f = getattr(L, name)
             if name not in ("kq_last_error", "kq_viterbi_workspace_bytes", "kq_hessian_workspace_bytes") and f.restype is ctypes.c_int:
@@ -535,6 +540,20 @@ def expert_bias_grad(dz: torch.Tensor, offsets: torch.Tensor | None, db: torch.T
                                           dz.shape[0], dz.shape[1], db.shape[0], dtype, db.data_ptr(), db.stride(0),
                                           _stream(device)), "kq_expert_bias_grad")
     stats.launches += 1
+
+
+def accumulate_expert_hessians(x: torch.Tensor, dtype: int, index: torch.Tensor | None, w: torch.Tensor | None,
+                               offsets: torch.Tensor, rows: int, H: torch.Tensor, add: bool, den: torch.Tensor) -> None:
+    device, E = H.device, H.shape[0]
+    with torch.cuda.device(device):
+        n = load().kq_expert_hessian_workspace_bytes(rows, x.shape[1], E, dtype, int(w is not None))
+        ws = scratch(n, device)
+        _check(load().kq_accumulate_expert_hessians(
+            x.data_ptr(), x.shape[0], x.shape[1], x.stride(0), dtype, None if index is None else index.data_ptr(),
+            None if w is None else w.data_ptr(), offsets.data_ptr(), rows, E, H.data_ptr(), H.stride(0), H.stride(1),
+            int(add), den.data_ptr(), None if ws is None else ws.data_ptr(), n, _stream(device)),
+            "kq_accumulate_expert_hessians")
+    stats.launches += 2
 
 
 def check_wait_errors(device: torch.device) -> None:

@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _native
+from . import _native, experts
 
 _SPLIT = {"3xtf32": 3, "tf32": 1}
 
@@ -41,6 +41,54 @@ def accumulate_hessian(rows: torch.Tensor, weights: torch.Tensor, *, device: tor
         ws = _native.accumulate_hessian(x, w, acc, _SPLIT[precision], ws)
     _native.check_trace_errors()
     return acc, float(den.item())
+
+
+_ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, index: torch.Tensor | None = None,
+                               weights: torch.Tensor | None = None,
+                               out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The Hessians of all experts of a layer in one call: H[e] = sum_t w_t x_t x_t^T over the slots
+    ``offsets[e] .. offsets[e + 1]``.
+
+    ``rows`` [tokens, d] bf16, fp16 or fp32 on the GPU.  ``index`` (int64) names the row of each slot, as routing
+    gives it (a row may serve several experts, and an index outside the rows counts for nothing); without it slot t
+    is row t.  ``weights`` fp32, one per slot.  Returns (H [experts, d, d] fp32, denominators [experts] fp64, the
+    sums of the weights), both on the GPU: nothing waits for the device.  With ``out`` the sums are added to it,
+    which is how samples stream in; the denominators are this call's alone.  fp32 accuracy for every type.
+    """
+    if not isinstance(rows, torch.Tensor) or rows.dtype not in _ROW_DTYPES:
+        raise TypeError("rows must be a torch.bfloat16, torch.float16 or torch.float32 tensor")
+    dev = rows.device
+    experts._operand(rows, "rows", 2, rows.dtype, dev)
+    experts._operand(offsets, "offsets", 1, torch.int64, dev)
+    if offsets.numel() < 2 or not offsets.is_contiguous():
+        raise ValueError("offsets must be experts + 1 contiguous values")
+    E, (tokens, d) = offsets.numel() - 1, rows.shape
+    if d < 1 or (d > 1 and rows.stride(1) != 1):
+        raise ValueError("rows needs at least one column and unit stride along its last dimension")
+    slots = tokens
+    if index is not None:
+        experts._operand(index, "index", 1, torch.int64, dev)
+        slots = index.numel()
+    if weights is not None:
+        experts._operand(weights, "weights", 1, torch.float32, dev)
+        if weights.numel() != slots:
+            raise ValueError(f"weights must have {slots} values, got {weights.numel()}")
+    for name, t in (("index", index), ("weights", weights)):
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if out is not None:
+        experts._operand(out, "out", 3, torch.float32, dev)
+        if out.shape != (E, d, d) or (d > 1 and out.stride(2) != 1):
+            raise ValueError(f"out must be [{E}, {d}, {d}] with unit stride along its last dimension")
+    if tokens > 1 and rows.stride(0) < d:
+        rows = rows.contiguous()
+    H = out if out is not None else torch.empty((E, d, d), dtype=torch.float32, device=dev)
+    den = torch.empty(E, dtype=torch.float64, device=dev)
+    _native.accumulate_expert_hessians(rows, _ROW_DTYPES[rows.dtype], index, weights, offsets, slots, H, out is not None, den)
+    return H, den
 
 
 # the reference's private name, for callers that import it directly

@@ -1,0 +1,475 @@
+// Calibration Hessians of all experts at once, fp32:
+//
+//     H_e (+)= sum_t w_t x_i(t) x_i(t)^T,   den_e = sum_t w_t
+//
+// over the rows t of expert e (kquant/capture.py:713-730 for one matrix; the
+// reference calls it expert by expert).  x [tokens x d] is bf16, fp16 or
+// fp32, i an optional index of its rows.
+//
+// The products run on the 16-bit tensor pipe with exact operands: a value is
+// split into 16-bit terms that add up to it, and the products of terms below
+// 2^-24 of the whole are left out.
+//
+//     x 16-bit, no weights:  x x^T                            1 product
+//     x bf16, weights:       x * (w x in 3 bf16 terms)        3 products
+//     x fp16, weights:       (2 bf16 terms) * (3 terms)       5 products
+//     x fp32:                (3 terms) * (3 terms)            6 products
+//
+// Six bf16 products cost what three TF32 products do and carry 24 bits instead
+// of 22.  The operand kernel gathers the rows, applies the weights, splits, and
+// pads every expert to whole 32-row stages with zeros; it writes rows as they
+// are stored, since an MN-major tcgen05 operand needs no transpose.
+//
+// One persistent CTA per SM walks the 128 x 256 output tiles on or above the
+// diagonal.  A stage holds 32 rows of every term, so each is fetched once for
+// all products.  The tensor-core accumulator truncates: it holds only a few
+// stages (up to 128 rows), which the drain warps add into fp32 registers with
+// rounding.  Elements above the diagonal are written twice, so H is exactly
+// symmetric.  With few rows the kernel is bound by writing H.
+#include "kq_expert.cuh"
+
+namespace kq {
+namespace {
+
+constexpr int BM = 128, BN = 256, BK = 32;
+constexpr int CHUNK = BK * 128;                 // 32 rows x 64 columns of 16 bits
+constexpr int A_BYTES = BM / 64 * CHUNK, B_BYTES = BN / 64 * CHUNK;
+constexpr int THREADS = 320;
+constexpr int GROUP_BYTES = (kMaxExperts + 4) * 4;
+
+constexpr int stage_bytes(int na, int nb) { return na * A_BYTES + nb * B_BYTES; }
+constexpr int stages_for(int na, int nb) {
+    const int fit = (227 * 1024 - 1024 - GROUP_BYTES - 512) / stage_bytes(na, nb);
+    return fit > 8 ? 8 : fit;
+}
+constexpr int products(int na, int nb) { return na == 1 ? nb : na == 2 ? 5 : 6; }
+// Stages per drain: 128 rows of one product, 64 of three, 32 of more.
+constexpr int seg_stages(int na, int nb) { return products(na, nb) == 1 ? 4 : products(na, nb) == 3 ? 2 : 1; }
+
+struct Maps { CUtensorMap a[3], b[3]; };
+
+struct Params {
+    const int64_t* offsets;
+    float* H;
+    int* err;
+    int64_t h_stride, ldh;
+    int rows, experts, d, tiles;   // tiles per expert
+    uint32_t idesc;
+    bool add, vec;
+};
+
+// Tile l of an expert: column block ni holds the row blocks 0 .. 2 ni + 1.
+__device__ __forceinline__ void tri_tile(int l, int& m0, int& n0) {
+    int ni = (int)((sqrtf(4.f * l + 1.f) - 1.f) * 0.5f);
+    while (ni * (ni + 1) > l) --ni;
+    while ((ni + 1) * (ni + 2) <= l) ++ni;
+    m0 = (l - ni * (ni + 1)) * BM;
+    n0 = ni * BN;
+}
+
+// The products of a stage, small terms first: (a term, b term) in order.
+template <int NA, int NB>
+__device__ __forceinline__ void product_terms(int i, int& a, int& b) {
+    if constexpr (NA == 1) { a = 0; b = NB - 1 - i; }
+    else if constexpr (NA == 2) { a = (0x05 >> i) & 1; b = (0x0049 >> (i * 2)) & 3; }
+    else { a = (0x0052 >> (i * 2)) & 3; b = (0x0118 >> (i * 2)) & 3; }
+}
+
+template <int NA, int NB>
+__global__ void __launch_bounds__(THREADS, 1)
+hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
+    constexpr int STAGES = stages_for(NA, NB), STAGE = stage_bytes(NA, NB), SEG = seg_stages(NA, NB);
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], seg_full[2], seg_empty[2];
+    __shared__ uint32_t tmem_slot;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    int* cum = reinterpret_cast<int*>(smem + STAGES * STAGE);
+    int* lo = reinterpret_cast<int*>(smem);     // needed by the scan alone, before the first stage is loaded
+    int* cnt = lo + kMaxExperts;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&seg_full[b], 1);
+            mbar_init(&seg_empty[b], 8);
+        }
+        mbar_init_fence();
+    }
+    if (warp == 8) tmem_alloc(&tmem_slot, 2 * BN);
+    scan_groups(p.offsets, p.experts, p.rows, BK, lo, cnt, cum);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int64_t all = (int64_t)p.tiles * p.experts;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int64_t i = blockIdx.x; i < all && ok; i += gridDim.x) {
+                const int e = (int)(i / p.tiles);
+                int m0, n0;
+                tri_tile((int)(i - (int64_t)e * p.tiles), m0, n0);
+                for (int ks = cum[e]; ks < cum[e + 1]; ++ks, ++it) {
+                    const int s = it % STAGES;
+                    if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
+                    mbar_expect_tx(&full_bar[s], STAGE);
+                    uint8_t* dst = smem + s * STAGE;
+#pragma unroll
+                    for (int t = 0; t < NA; ++t)
+#pragma unroll
+                        for (int c = 0; c < BM / 64; ++c, dst += CHUNK)
+                            tma_load_2d(dst, &maps.a[t], m0 + 64 * c, ks * BK, &full_bar[s]);
+#pragma unroll
+                    for (int t = 0; t < NB; ++t)
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c, dst += CHUNK)
+                            tma_load_2d(dst, &maps.b[t], n0 + 64 * c, ks * BK, &full_bar[s]);
+                }
+            }
+            if (!ok) report_wait_error(p.err);
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            uint32_t it = 0, seg = 0;
+            bool ok = true;
+            for (int64_t i = blockIdx.x; i < all && ok; i += gridDim.x) {
+                const int e = (int)(i / p.tiles), ks_end = cum[e + 1];
+                for (int ks0 = cum[e]; ks0 < ks_end && ok; ks0 += SEG, ++seg) {
+                    const int b = seg & 1;
+                    if (!(ok = mbar_wait(&seg_empty[b], ((seg >> 1) & 1) ^ 1))) break;
+                    tc_fence_after();
+                    const int stop = min(ks_end, ks0 + SEG);
+                    for (int ks = ks0; ks < stop; ++ks, ++it) {
+                        const int s = it % STAGES;
+                        if (!(ok = mbar_wait(&full_bar[s], (it / STAGES) & 1))) break;
+                        tc_fence_after();
+                        const uint32_t base = smem_addr(smem + s * STAGE);
+#pragma unroll
+                        for (int i2 = 0; i2 < products(NA, NB); ++i2) {
+                            int ta, tb;
+                            product_terms<NA, NB>(i2, ta, tb);
+                            const uint64_t ad = smem_desc(base + ta * A_BYTES, CHUNK);
+                            const uint64_t bd = smem_desc(base + NA * A_BYTES + tb * B_BYTES, CHUNK);
+#pragma unroll
+                            for (int kk = 0; kk < BK / 16; ++kk)
+                                mma_f16(tmem + b * BN, ad + 128 * kk, bd + 128 * kk, p.idesc,
+                                        (ks != ks0 || i2 != 0 || kk != 0) ? 1u : 0u);
+                        }
+                        mma_commit(&empty_bar[s]);
+                    }
+                    if (ok) mma_commit(&seg_full[b]);
+                }
+            }
+            if (!ok) report_wait_error(p.err);
+        }
+    } else {
+        const int q = warp & 3, h = warp >> 2;
+        uint32_t seg = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; it < all && ok; it += gridDim.x) {
+            const int e = (int)(it / p.tiles), ks_end = cum[e + 1];
+            int m0, n0;
+            tri_tile((int)(it - (int64_t)e * p.tiles), m0, n0);
+            float r[BN / 2];
+#pragma unroll
+            for (int i = 0; i < BN / 2; ++i) r[i] = 0.f;
+            for (int ks0 = cum[e]; ks0 < ks_end; ks0 += SEG, ++seg) {
+                const int b = seg & 1;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[b], (seg >> 1) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + h * (BN / 2));
+#pragma unroll
+                for (int c0 = 0; c0 < BN / 2; c0 += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(base + (uint32_t)c0, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) r[c0 + i] += __uint_as_float(v[i]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&seg_empty[b]);
+            }
+            if (!ok || (p.add && cum[e] == ks_end)) continue;
+            const int i = m0 + q * 32 + lane, j0 = n0 + h * (BN / 2);
+            if (i < p.d) {
+                float* H = p.H + e * p.h_stride;
+                float* drow = H + (int64_t)i * p.ldh;
+#pragma unroll
+                for (int c = 0; c < BN / 2; c += 4) {
+                    const int j = j0 + c;
+                    if (p.vec && j + 3 < p.d && j >= i) {
+                        float4* dp = reinterpret_cast<float4*>(drow + j);
+                        const float4 v = make_float4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+                        if (p.add) atomicAdd(dp, v);
+                        else __stcs(dp, v);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (j + x < p.d && j + x >= i) {
+                                if (p.add) atomicAdd(drow + j + x, r[c + x]);
+                                else drow[j + x] = r[c + x];
+                            }
+                        }
+                    }
+                }
+                // (col, row) above the diagonal: lanes hold consecutive rows, one 128-byte access a column.
+#pragma unroll
+                for (int c = 0; c < BN / 2; ++c) {
+                    const int j = j0 + c;
+                    if (j > i && j < p.d) {
+                        float* dp = H + (int64_t)j * p.ldh + i;
+                        if (p.add) atomicAdd(dp, r[c]);
+                        else __stcs(dp, r[c]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0) report_wait_error(p.err);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) tmem_free(tmem, 2 * BN);
+}
+
+// Operand rows.  Block (t, c): slots 32 t .. of the padded rows, columns
+// 1024 c ..; the blocks behind the last row tile sum the weights of one
+// expert each, in an order that depends on nothing.
+struct OperandParams {
+    const void* x;
+    const int64_t* index;
+    const float* w;
+    const int64_t* offsets;
+    uint16_t* terms;           // a terms, then b terms, each [slots][ld]
+    double* den;
+    int64_t ldx, tokens, term_stride;
+    int rows, experts, d, ld, row_tiles;
+    bool vec;
+};
+
+__device__ __forceinline__ void split_bf16(float v, int n, uint16_t (&t)[3]) {
+    float rest = v;
+    const bool finite = fabsf(v) <= 3.3895313892515355e38f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (i < n) {
+            const __nv_bfloat16 b = __float2bfloat16_rn(rest);
+            t[i] = __bfloat16_as_ushort(b);
+            rest = finite ? rest - __bfloat162float(b) : 0.f;
+        }
+    }
+}
+
+// NA = NB = 0: the 16-bit values themselves.
+template <typename T, int NA, int NB>
+__global__ void __launch_bounds__(256) operand_kernel(const OperandParams p) {
+    __shared__ int lo[kMaxExperts], cnt[kMaxExperts], cum[kMaxExperts + 1];
+    __shared__ double part[256];
+    if ((int)blockIdx.x >= p.row_tiles) {
+        if (blockIdx.y) return;
+        const int e = blockIdx.x - p.row_tiles;
+        int first, n;
+        group_of(p.offsets, e, p.rows, first, n);
+        double s = 0.0;
+        for (int r = threadIdx.x; r < n; r += 256) {
+            const int64_t src = p.index ? p.index[first + r] : first + r;
+            if (src >= 0 && src < p.tokens) s += p.w ? (double)p.w[first + r] : 1.0;
+        }
+        part[threadIdx.x] = s;
+        for (int d = 128; d; d >>= 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
+        }
+        if (threadIdx.x == 0) p.den[e] = part[0];
+        return;
+    }
+    scan_groups(p.offsets, p.experts, p.rows, BK, lo, cnt, cum);
+    const int t = blockIdx.x;
+    if (t >= cum[p.experts]) return;
+    const int e = expert_of(cum, p.experts, t), first = (t - cum[e]) * BK;
+    for (int i = threadIdx.x; i < BK * 128; i += 256) {        // 8 columns of one row at a time
+        const int r = i >> 7, c = blockIdx.y * 1024 + (i & 127) * 8;
+        if (c >= p.ld) continue;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        float w = 0.f;
+        if (first + r < cnt[e]) {
+            const int row = lo[e] + first + r;
+            const int64_t src = p.index ? p.index[row] : row;
+            if (src >= 0 && src < p.tokens) {
+                w = p.w ? p.w[row] : 1.f;
+                const T* xr = static_cast<const T*>(p.x) + src * p.ldx + c;
+                const int nv = p.d - c;
+                if constexpr (sizeof(T) == 4) {
+                    if (p.vec && nv >= 8) {
+                        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(xr);
+                        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(xr + 4);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) if (k < nv) v[k] = xr[k];
+                    }
+                } else {
+                    load8(xr, p.vec && nv >= 8, nv, v);
+                }
+            }
+        }
+        uint16_t* dst = p.terms + ((int64_t)t * BK + r) * p.ld + c;
+        if constexpr (NA == 0) {
+            T o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = from_f<T>(v[k]);
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+        } else {
+            uint16_t a[8][3], b[8][3];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                split_bf16(v[k], NA, a[k]);
+                split_bf16(v[k] * w, NB, b[k]);
+            }
+#pragma unroll
+            for (int q = 0; q < NA + NB; ++q) {
+                uint16_t o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = q < NA ? a[k][q < NA ? q : 0] : b[k][q < NA ? 0 : q - NA];
+                *reinterpret_cast<uint4*>(dst + q * p.term_stride) = *reinterpret_cast<const uint4*>(o);
+            }
+        }
+    }
+}
+
+int64_t pad8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+
+int64_t slots(int64_t rows, int64_t experts) { return ((rows + BK - 1) / BK + (experts < rows ? experts : rows)) * BK; }
+
+void terms_of(int dtype, bool weighted, int& na, int& nb) {
+    if (dtype == KQ_FP32) { na = 3; nb = 3; }
+    else if (!weighted) { na = 0; nb = 0; }
+    else if (dtype == KQ_BF16) { na = 1; nb = 3; }
+    else { na = 2; nb = 3; }
+}
+
+// fp32 rows without weights share one set of terms for both sides.
+int term_count(int dtype, bool weighted) {
+    int na, nb;
+    terms_of(dtype, weighted, na, nb);
+    return na == 0 ? 1 : na + nb;
+}
+
+template <int NA, int NB>
+int launch_hessian(const Maps& m, const Params& p, int grid, cudaStream_t s) {
+    constexpr int smem = stages_for(NA, NB) * stage_bytes(NA, NB) + GROUP_BYTES + 1024;
+    cudaError_t e = cudaFuncSetAttribute(hessian_kernel<NA, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+    hessian_kernel<NA, NB><<<grid, THREADS, smem, s>>>(m, p);
+    return check_launch("hessian_kernel");
+}
+
+bool bad_sizes(int64_t rows, int64_t tokens, int64_t d, int64_t experts, int dtype) {
+    return rows < 0 || tokens < 0 || d <= 0 || experts <= 0 || experts > kMaxExperts || rows > 0x3FFFFFFF || d > (1 << 20) ||
+           (dtype != KQ_BF16 && dtype != KQ_FP16 && dtype != KQ_FP32);
+}
+
+}  // namespace
+}  // namespace kq
+
+extern "C" size_t kq_expert_hessian_workspace_bytes(int64_t rows, int64_t dim, int64_t experts, int dtype, int weighted) {
+    using namespace kq;
+    if (bad_sizes(rows, 0, dim, experts, dtype) || rows == 0) return 0;
+    return (size_t)term_count(dtype, weighted != 0) * (size_t)slots(rows, experts) * (size_t)pad8(dim) * 2;
+}
+
+extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int64_t dim, int64_t ldx, int dtype,
+                                             const int64_t* index, const float* w, const int64_t* offsets, int64_t rows,
+                                             int64_t experts, float* H, int64_t h_stride, int64_t ldh, int add, double* den,
+                                             void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace kq;
+    const char* what = "kq_accumulate_expert_hessians";
+    if (bad_sizes(rows, tokens, dim, experts, dtype) || (tokens > 1 && ldx < dim) || (dim > 1 && ldh < dim) ||
+        (experts > 1 && h_stride < (dim - 1) * ldh + dim) || (!index && rows > tokens)) {
+        set_error("%s: bad arguments (rows=%lld tokens=%lld dim=%lld experts=%lld ldx=%lld ldh=%lld dtype=%d)", what,
+                  (long long)rows, (long long)tokens, (long long)dim, (long long)experts, (long long)ldx, (long long)ldh, dtype);
+        return KQ_ERR_ARG;
+    }
+    if (experts > 1 && !offsets) { set_error("%s: several experts need offsets", what); return KQ_ERR_ARG; }
+    if (!H || !den || (rows > 0 && tokens > 0 && !x)) { set_error("%s: null pointer", what); return KQ_ERR_ARG; }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool weighted = w != nullptr;
+    const size_t need = kq_expert_hessian_workspace_bytes(rows, dim, experts, dtype, weighted);
+    if (need && (workspace_bytes < need || !workspace)) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
+    if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
+    Params q{};
+    if (int rc = wait_error_word(&q.err)) return rc;
+    const int ld = (int)pad8(dim);
+    const int64_t n_slots = slots(rows, experts);
+    int na, nb;
+    terms_of(dtype, weighted, na, nb);
+
+    OperandParams o{};
+    o.x = x;
+    o.index = index;
+    o.w = w;
+    o.offsets = offsets;
+    o.terms = static_cast<uint16_t*>(workspace);
+    o.den = den;
+    o.ldx = ldx;
+    o.tokens = tokens;
+    o.term_stride = n_slots * ld;
+    o.rows = (int)rows;
+    o.experts = (int)experts;
+    o.d = (int)dim;
+    o.ld = ld;
+    o.row_tiles = (int)(n_slots / BK);
+    o.vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
+    const dim3 grid((unsigned)(o.row_tiles + experts), (unsigned)((ld + 1023) / 1024));
+    if (dtype == KQ_FP32) operand_kernel<float, 3, 3><<<grid, 256, 0, s>>>(o);
+    else if (dtype == KQ_BF16 && weighted) operand_kernel<__nv_bfloat16, 1, 3><<<grid, 256, 0, s>>>(o);
+    else if (dtype == KQ_BF16) operand_kernel<__nv_bfloat16, 0, 0><<<grid, 256, 0, s>>>(o);
+    else if (weighted) operand_kernel<__half, 2, 3><<<grid, 256, 0, s>>>(o);
+    else operand_kernel<__half, 0, 0><<<grid, 256, 0, s>>>(o);
+    if (int rc = check_launch("operand_kernel")) return rc;
+
+    Maps maps;
+    const bool fp16 = dtype == KQ_FP16 && !weighted;
+    const int count = term_count(dtype, weighted);
+    CUtensorMap term[6];
+    const int64_t dims[2] = {dim, n_slots > 0 ? n_slots : 1}, strides[1] = {(int64_t)ld * 2};
+    const int box[2] = {64, BK};
+    for (int t = 0; t < count && rows > 0; ++t)
+        if (int rc = encode_tiles(&term[t], fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                  o.terms + t * o.term_stride, dims, strides, box, what))
+            return rc;
+    for (int t = 0; t < 3 && rows > 0; ++t) {
+        maps.a[t] = term[na ? (t < na ? t : 0) : 0];
+        maps.b[t] = term[na ? na + (t < nb ? t : 0) : 0];
+    }
+    q.offsets = offsets;
+    q.H = H;
+    q.h_stride = h_stride;
+    q.ldh = ldh;
+    q.rows = (int)rows;
+    q.experts = (int)experts;
+    q.d = (int)dim;
+    const int64_t nt = (dim + BN - 1) / BN;
+    q.tiles = (int)(nt * (nt + 1));
+    q.idesc = idesc_f16(!fp16, true, true, BM, BN);
+    q.add = add != 0;
+    q.vec = ((uintptr_t)H & 15) == 0 && ldh % 4 == 0 && h_stride % 4 == 0;
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    const int64_t tiles = (int64_t)q.tiles * experts;
+    const int g = (int)(tiles < sms ? tiles : sms);
+    if (na == 0) return launch_hessian<1, 1>(maps, q, g, s);
+    if (na == 1) return launch_hessian<1, 3>(maps, q, g, s);
+    if (na == 2) return launch_hessian<2, 3>(maps, q, g, s);
+    return launch_hessian<3, 3>(maps, q, g, s);
+}

@@ -86,3 +86,37 @@ def test_c_entries_refuse_null():
     assert L.kq_expert_linear_workspace_bytes(None) == 0
     # Nothing to do: no pointer is needed.
     assert L.kq_expert_linear(ctypes.byref(_product(rows=0, x=None, y=None)), None, 0, None) == 0
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(rows=fake(4, 8, dtype=torch.float64)), TypeError, "rows must be"),
+    (dict(rows=torch.zeros(4, 8)), _native.KQError, "CUDA"),
+    (dict(rows=fake(4, 16)[:, ::2]), ValueError, "unit stride"),
+    (dict(rows=fake(4, 0)), ValueError, "at least one column"),
+    (dict(offsets=fake(1, dtype=torch.int64)), ValueError, "experts"),
+    (dict(offsets=fake(3, dtype=torch.int32)), TypeError, "int64"),
+    (dict(index=fake(4, dtype=torch.int32)), TypeError, "int64"),
+    (dict(index=fake(8, dtype=torch.int64)[::2]), ValueError, "contiguous"),
+    (dict(weights=fake(3, dtype=torch.float32)), ValueError, "4 values"),
+    (dict(weights=fake(4)), TypeError, "float32"),
+    (dict(out=fake(2, 8, 7, dtype=torch.float32)), ValueError, "out must be"),
+    (dict(out=fake(2, 8, 8)), TypeError, "out must be"),
+])
+def test_expert_hessians_refuse(change, error, match):
+    from kquant_b200.capture import accumulate_expert_hessians
+    args = dict(rows=fake(4, 8), offsets=fake(3, dtype=torch.int64))
+    args.update(change)
+    with pytest.raises(error, match=match):
+        accumulate_expert_hessians(**args)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(tokens=-1), -1), (dict(dim=0), -1), (dict(ldx=7), -1), (dict(dtype=3), -1), (dict(offsets=None), -1), (dict(rows=5), -1),
+    (dict(experts=0), -1), (dict(experts=2000), -1), (dict(H=None), -1), (dict(h_stride=63), -1), (dict(ldh=7), -1), (dict(den=None), -1),
+    (dict(), -2), (dict(ws=200, size=1 << 20), -4), (dict(x=None), -1),
+])
+def test_expert_hessian_c_entry_refuses(change, status):
+    a = dict(x=64, tokens=4, dim=8, ldx=8, dtype=0, index=None, w=None, offsets=64, rows=4, experts=2, H=64, h_stride=64, ldh=8, add=0,
+             den=64, ws=None, size=0, stream=None)
+    a.update(change)
+    assert _native.load().kq_accumulate_expert_hessians(*a.values()) == status
