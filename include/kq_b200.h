@@ -347,6 +347,37 @@ int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int64_t dim, in
                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Products with encoded matrices, straight from the packed payload:
+ *     y[r] = had(had(x[r] * suh_e) What_e) * svh_e
+ * for rows grouped by expert as in kq_expert_linear, i.e. x times the weight
+ * that kq_reconstruct_rotated gives (128-block Hadamards normalised
+ * 1/sqrt(128), kquant/exl3_encoder_backend.py:2211-2216).  trellis
+ * [experts][k/16][n/16][16 bits] words of kq_pack_trellis, every expert at
+ * the same rate; suh [experts][k], svh [experts][n] binary16; x and y
+ * KQ_BF16 or KQ_FP16.  codebook: KQ_CB_MCG (table NULL), KQ_CB_SQG (table:
+ * 65,536 E4M3 bytes by state) or KQ_CB_LABELS (table: 65,536 binary16 labels
+ * by state, kq_build_labels).  The rotated row enters the tensor cores as
+ * binary16 with a power of two of its own; sums are fp32, y is rounded once.
+ * Rows of no expert as in kq_expert_linear.
+ */
+#define KQ_CB_LABELS 5
+typedef struct {
+    const void* x;
+    const uint16_t* trellis;
+    const uint16_t* suh;
+    const uint16_t* svh;
+    const int64_t* offsets;
+    const void* table;
+    void* y;
+    int64_t rows, k, n, experts;
+    int64_t ldx, ldy, suh_stride_e, svh_stride_e;
+    int32_t bits, codebook, dtype, zero_rest;
+} kq_trellis_product;
+
+size_t kq_trellis_linear_workspace_bytes(const kq_trellis_product* p);
+int kq_trellis_linear(const kq_trellis_product* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Writes 1 to *out (device int32) if an internal wait of an expert-layer
  * kernel ran out on this device since the last call, else 0, and clears it.
  */

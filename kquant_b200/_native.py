@@ -20,6 +20,7 @@ KQ_CB_3INST = 0
 KQ_CB_MCG = 1
 KQ_CB_MUL1 = 2
 KQ_CB_SQG = 4
+KQ_CB_LABELS = 5
 
 EXPORTED = (
     "kq_last_error",
@@ -50,6 +51,8 @@ EXPORTED = (
     "kq_wait_errors",
     "kq_expert_hessian_workspace_bytes",
     "kq_accumulate_expert_hessians",
+    "kq_trellis_linear_workspace_bytes",
+    "kq_trellis_linear",
 )
 
 KQ_CHAIN_MAX_ITEMS = 64
@@ -73,6 +76,16 @@ class ExpertProduct(ctypes.Structure):
                 ("w_stride_e", ctypes.c_int64), ("w_stride_k", ctypes.c_int64), ("w_stride_n", ctypes.c_int64),
                 ("bias_stride_e", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ldy", ctypes.c_int64),
                 ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("gated", ctypes.c_int32),
+                ("zero_rest", ctypes.c_int32)]
+
+
+class TrellisProduct(ctypes.Structure):
+    """kq_trellis_product of include/kq_b200.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("trellis", ctypes.c_void_p), ("suh", ctypes.c_void_p), ("svh", ctypes.c_void_p),
+                ("offsets", ctypes.c_void_p), ("table", ctypes.c_void_p), ("y", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("k", ctypes.c_int64), ("n", ctypes.c_int64), ("experts", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("ldy", ctypes.c_int64), ("suh_stride_e", ctypes.c_int64), ("svh_stride_e", ctypes.c_int64),
+                ("bits", ctypes.c_int32), ("codebook", ctypes.c_int32), ("dtype", ctypes.c_int32),
                 ("zero_rest", ctypes.c_int32)]
 
 
@@ -128,6 +141,10 @@ def load() -> ctypes.CDLL:
         L.kq_expert_weight_grad.argtypes = [EP, P, I64, P, P, SZ, P]
         L.kq_expert_bias_grad.argtypes = [P, I64, P, I64, I64, I64, I, P, I64, P]
         L.kq_wait_errors.argtypes = [P, P]
+        TP = ctypes.POINTER(TrellisProduct)
+        L.kq_trellis_linear_workspace_bytes.argtypes = [TP]
+        L.kq_trellis_linear_workspace_bytes.restype = SZ
+        L.kq_trellis_linear.argtypes = [TP, P, SZ, P]
         L.kq_expert_hessian_workspace_bytes.argtypes = [I64, I64, I64, I, I]
         L.kq_expert_hessian_workspace_bytes.restype = SZ
         L.kq_accumulate_expert_hessians.argtypes = [P, I64, I64, I64, I, P, P, P, I64, I64, P, I64, I64, I, P, P, SZ, P]
@@ -554,6 +571,14 @@ def accumulate_expert_hessians(x: torch.Tensor, dtype: int, index: torch.Tensor 
             int(add), den.data_ptr(), None if ws is None else ws.data_ptr(), n, _stream(device)),
             "kq_accumulate_expert_hessians")
     stats.launches += 2
+
+
+def trellis_linear(p: TrellisProduct, device: torch.device) -> None:
+    with torch.cuda.device(device):
+        n = load().kq_trellis_linear_workspace_bytes(p)
+        ws = scratch(n, device)
+        _check(load().kq_trellis_linear(p, None if ws is None else ws.data_ptr(), n, _stream(device)), "kq_trellis_linear")
+    stats.launches += 3
 
 
 def check_wait_errors(device: torch.device) -> None:

@@ -22,7 +22,7 @@
 // computes them and does not store them (a row meets only its own
 // accumulators); a sums tile zeroes the rows behind its expert's last in
 // shared memory before the product, because there they would be added in.
-#include "kq_expert.cuh"
+#include "kq_expert_rows.cuh"
 
 namespace kq {
 namespace {
@@ -36,12 +36,13 @@ constexpr int DRAIN_WARPS = 8, THREADS = 64 + 32 * DRAIN_WARPS;
 constexpr int GROUP_BYTES = (3 * kMaxExperts + 4) * 4;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GROUP_BYTES + 1024;
 
-enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS };
+enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS, EPI_ROTATED };
 
 struct Params {
     const int64_t* offsets;
     const void* bias;
-    const void* aux;       // residual (forward) or dy (gradient)
+    const void* aux;       // residual (forward), dy (gradient) or svh (rotated)
+    const float* row_scale;
     void* out;
     int64_t bias_stride, ld_aux, ld_out, out_stride;   // out_stride: per expert (sums)
     int rows, experts, k_steps, m_tiles, n_tiles, m_out, n_out;
@@ -205,8 +206,44 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 orow = static_cast<T*>(p.out) + t.e * p.out_stride + (int64_t)(t.m0 + r) * p.ld_out;
             } else {
                 orow = static_cast<T*>(p.out) + (int64_t)(t.row0 + r) * p.ld_out;
-                if (p.aux) arow = static_cast<const T*>(p.aux) + (int64_t)(t.row0 + r) * p.ld_aux;
+                if (EPI != EPI_ROTATED && p.aux) arow = static_cast<const T*>(p.aux) + (int64_t)(t.row0 + r) * p.ld_aux;
             }
+            if constexpr (EPI == EPI_ROTATED) {
+                // A thread holds one row of one 128-column Hadamard block: the transform stays in its registers.
+                if (n_base < p.n_out) {
+                    float z[128];
+#pragma unroll
+                    for (int c = 0; c < 128; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(base + h * HALF + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) z[c + e] = __uint_as_float(v[e]);
+                    }
+#pragma unroll
+                    for (int d = 1; d < 128; d <<= 1)
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            if (!(e & d)) {
+                                const float a = z[e], c = z[e + d];
+                                z[e] = a + c;
+                                z[e + d] = a - c;
+                            }
+                    if (live) {
+                        const float scale = p.row_scale[t.row0 + r] * 0.08838834764831845f;   // 1 / sqrt(128)
+                        const __half* svh = static_cast<const __half*>(p.aux) + t.e * p.ld_aux + n_base;
+#pragma unroll
+                        for (int c = 0; c < 128; c += 8) {
+                            float a[8];
+                            load8(svh + c, p.vec_aux, 8, a);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) a[e] *= z[c + e] * scale;
+                            store8(orow + n_base + c, p.vec_out, 8, a);
+                        }
+                    }
+                    __syncwarp();
+                }
+            } else {
 #pragma unroll 1
             for (int c = 0; c < HALF; c += 16) {
                 if (n_base + c >= p.n_out) break;
@@ -264,6 +301,7 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     store8(orow + j, p.vec_out && nv >= 8, nv, z);
                 }
                 __syncwarp();
+            }
             }
             tc_fence_before();
             __syncwarp();
@@ -500,6 +538,36 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
 __global__ void take_errors_kernel(int* out) { *out = atomicExch(&g_wait_error, 0); }
 
 }  // namespace
+
+int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
+                         int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
+                         bool bf16_out, cudaStream_t s) {
+    const char* what = "rows_product_rotated";
+    CUtensorMap ma, mb;
+    if (int rc = map_rows_2d(&ma, operand(x, 1, rows, k, 0, k), false, BK, BM, what)) return rc;
+    if (int rc = map_rows(&mb, operand(w, experts, n, k, n * k, k), false, BK, BN / 2, what)) return rc;
+    Params q{};
+    if (int rc = wait_error_word(&q.err)) return rc;
+    q.offsets = offsets;
+    q.aux = svh;
+    q.ld_aux = svh_stride;
+    q.row_scale = row_scale;
+    q.out = y;
+    q.ld_out = ldy;
+    q.rows = (int)rows;
+    q.experts = (int)experts;
+    q.k_steps = (int)((k + BK - 1) / BK);
+    q.n_tiles = (int)((n + BN - 1) / BN);
+    q.n_out = (int)n;
+    q.w_second = 128;
+    q.idesc = idesc_f16(false, false, false, BM, BN);
+    q.vec_aux = vec8(svh, svh_stride);
+    q.vec_out = vec8(y, ldy);
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    const int64_t most = ((rows + BM - 1) / BM + (experts < rows ? experts : rows)) * q.n_tiles;
+    return launch<EPI_ROTATED, false>(bf16_out, ma, mb, q, (int)(most < sms ? most : sms), s);
+}
 
 int wait_error_word(int** out) {
     void* p = nullptr;

@@ -1,0 +1,342 @@
+// Products with encoded matrices straight from their packed trellis payload:
+//
+//     y[r] = had(had(x[r] * suh_e) What_e) * svh_e       rows r of expert e
+//
+// which is x[r] times the reconstructed weight had_l(What) * suh, had_r, * svh
+// (kquant/exl3_encoder_backend.py:2211-2216), with What decoded from the
+// 16 K words of each 16 x 16 tile as it is needed.
+//
+// The input transform writes x' = had(x * suh) once, in binary16 with a power
+// of two per row that brings its bound to 2^14 (the labels are binary16, so
+// both operands of the tensor product are): 11 bits of x' against the 8 or 11
+// bits of x and y.  Products are summed in fp32, the output transform runs in
+// fp32, and y is rounded once.
+//
+// Decode.  State i of a tile is the 16-bit window of its cyclic bit stream
+// that ends with symbol i (kq_unpack_trellis_states).  Lane m of a warp owns
+// symbols 8m .. 8m+7: its eight windows lie in 7K + 16 consecutive bits, three
+// (K > 6: four) 32-bit words.  Trellis position 8m + s is row 2(m%4) + (s&1) +
+// 8((s>>1)&1), column m/4 + 8(s>>2) of the tile, so neighbouring symbols are
+// neighbouring rows: a packed pair along the contraction axis.
+// Labels: MCG is computed (a multiply, a logic op, half an add); E4M3 and
+// binary16 tables are looked up in shared memory, where 32 random lookups
+// meet about 3.5-fold bank conflicts.
+#include "kq_expert_rows.cuh"
+
+namespace kq {
+namespace {
+
+enum { DEC_MCG, DEC_E4M3, DEC_F16 };
+constexpr int kBlock = 128;
+
+__host__ __device__ constexpr int table_bytes(int dec) { return dec == DEC_MCG ? 0 : dec == DEC_E4M3 ? 65536 : 131072; }
+
+// Whole block: the label table into shared memory.
+template <int DEC>
+__device__ __forceinline__ void load_table(const void* table, uint8_t* smem) {
+    if constexpr (DEC != DEC_MCG) {
+        const uint4* src = static_cast<const uint4*>(table);
+        for (int i = threadIdx.x; i < table_bytes(DEC) / 16; i += blockDim.x) reinterpret_cast<uint4*>(smem)[i] = __ldg(src + i);
+    }
+}
+
+// Labels of two states as packed binary16.
+template <int DEC>
+__device__ __forceinline__ uint32_t label_pair(uint32_t s0, uint32_t s1, const uint8_t* table) {
+    if constexpr (DEC == DEC_MCG) {
+        const uint32_t y0 = ((s0 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
+        const uint32_t y1 = ((s1 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
+        const uint32_t lo = __byte_perm(y0, y1, 0x5410), hi = __byte_perm(y0, y1, 0x7632);
+        const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&hi));
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else if constexpr (DEC == DEC_E4M3) {
+        const uint16_t b = (uint16_t)(table[s0] | (table[s1] << 8));
+        uint32_t v;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v) : "h"(b));
+        return v;
+    } else {
+        const uint16_t* t = reinterpret_cast<const uint16_t*>(table);
+        return (uint32_t)t[s0] | ((uint32_t)t[s1] << 16);
+    }
+}
+
+// A tile's words, held by the warp: lane l has words l and (K > 4) l + 32, each 32 bits of the stream, first bit on top.
+template <int K>
+struct TileWords {
+    uint32_t w[K > 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const uint32_t* tile, int lane) {
+        if (K >= 4 || lane < 8 * K) w[0] = __ldg(tile + lane);
+        if constexpr (K > 4)
+            if (lane + 32 < 8 * K) w[1] = __ldg(tile + 32 + lane);
+    }
+    __device__ __forceinline__ uint32_t at(int i) const {       // word i mod 8K, i in -8K .. 8K
+        i = i < 0 ? i + 8 * K : i >= 8 * K ? i - 8 * K : i;
+        const uint32_t a = __shfl_sync(0xFFFFFFFFu, w[0], i & 31);
+        if constexpr (K > 4) {
+            const uint32_t b = __shfl_sync(0xFFFFFFFFu, w[1], i & 31);
+            return i >= 32 ? b : a;
+        }
+        return a;
+    }
+};
+
+// The four fragment pairs of this lane: rows (2q, 2q+1) and (2q+8, 2q+9) of column m/4, then of column m/4 + 8.
+template <int K, int DEC>
+__device__ __forceinline__ void decode_tile(const TileWords<K>& t, int lane, const uint8_t* table, uint32_t (&frag)[4]) {
+    const int end = 8 * K * (lane + 1), wi = end >> 5, off = end & 31;
+    const uint32_t c = t.at(wi), b = t.at(wi - 1), a = t.at(wi - 2);
+    // Stream bits [end-32, end), the 32 before them, and (K > 6) the 32 before those.
+    const uint32_t w0 = __funnelshift_l(c, b, off), w1 = __funnelshift_l(b, a, off);
+    uint32_t w2 = 0;
+    if constexpr (K > 6) w2 = __funnelshift_l(a, t.at(wi - 3), off);
+    uint32_t s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int sh = (7 - i) * K;
+        s[i] = (sh + 16 <= 32 ? w0 >> sh : sh < 32 ? __funnelshift_r(w0, w1, sh) : sh + 16 <= 64 ? w1 >> (sh - 32)
+                                                                                               : __funnelshift_r(w1, w2, sh - 32)) & 0xFFFFu;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) frag[i] = label_pair<DEC>(s[2 * i], s[2 * i + 1], table);
+}
+
+// Expert of one row, or -1: the block looks at all offsets at once.
+__device__ __forceinline__ int expert_of_row(const int64_t* offsets, int experts, int rows, int row, int* slot) {
+    if (threadIdx.x == 0) *slot = -1;
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int lo, n;
+        group_of(offsets, e, rows, lo, n);
+        if (row >= lo && row < lo + n) *slot = e;
+    }
+    __syncthreads();
+    return *slot;
+}
+
+__device__ __forceinline__ void had128_warp(float (&v)[4], int lane) {
+    const float a = v[0] + v[1], b = v[0] - v[1], c = v[2] + v[3], d = v[2] - v[3];
+    v[0] = a + c; v[2] = a - c; v[1] = b + d; v[3] = b - d;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float o = __shfl_xor_sync(0xFFFFFFFFu, v[i], m);
+            v[i] = (lane & m) ? o - v[i] : v[i] + o;
+        }
+}
+
+// x' = had(x * suh) * 2^s in binary16 and 2^-s; one block a row, a warp a Hadamard block.
+template <typename T>
+__global__ void __launch_bounds__(256) rotate_in_kernel(const T* __restrict__ x, int64_t ldx, const __half* __restrict__ suh,
+                                                        int64_t suh_stride, const int64_t* __restrict__ offsets, int rows,
+                                                        int experts, int k, __half* __restrict__ xr, float* __restrict__ scale) {
+    __shared__ int slot;
+    __shared__ float most[8];
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int e = expert_of_row(offsets, experts, rows, row, &slot);
+    if (e < 0) return;
+    const T* xp = x + (int64_t)row * ldx;
+    const __half* sp = suh + e * suh_stride;
+    float m = 0.f;
+    for (int i = threadIdx.x; i < k; i += 256) m = fmaxf(m, fabsf(to_f<T>(xp[i]) * __half2float(sp[i])));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    if (lane == 0) most[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, most[i]);
+    // |had(v)| <= sqrt(128) max |v| < 2^4 max |v|: the exponent that brings it to at most 2^14.
+    int ex = 0;
+    if (m > 0.f && m < 1e38f) {
+        frexpf(m, &ex);                                // m < 2^ex
+        ex = min(max(10 - ex, -120), 120);
+    }
+    const float up = ldexpf(0.08838834764831845f, ex);
+    for (int blk = warp; blk < k / kBlock; blk += 8) {
+        float v[4];
+        const int j = blk * kBlock + lane * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_f<T>(xp[j + i]) * __half2float(sp[j + i]);
+        had128_warp(v, lane);
+        __half2 o[2] = {__floats2half2_rn(v[0] * up, v[1] * up), __floats2half2_rn(v[2] * up, v[3] * up)};
+        *reinterpret_cast<uint2*>(xr + (int64_t)row * k + j) = *reinterpret_cast<const uint2*>(o);
+    }
+    if (threadIdx.x == 0) scale[row] = ldexpf(1.f, -ex);
+}
+
+// What_e as binary16 [n][k].  A block decodes 128 columns x 64 rows at a time through shared memory, so that it
+// reads 8 tiles' words in a row and writes whole 128-byte lines.
+constexpr int DN = 128, DK = 64, DPAD = 72;            // row stride of the staged tile in halves
+template <int K, int DEC>
+__global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict__ trellis, const void* __restrict__ table,
+                                                     const int64_t* __restrict__ offsets, int rows, int experts, int k, int n,
+                                                     __half* __restrict__ out) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __half* stage = reinterpret_cast<__half*>(smem + table_bytes(DEC));
+    load_table<DEC>(table, smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nb = n / DN, kb = (k + DK - 1) / DK, per = nb * kb;
+    int last = -1, busy = 0;
+    for (int64_t i = blockIdx.x; i < (int64_t)per * experts; i += gridDim.x) {
+        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per);
+        if (e != last) {
+            int lo;
+            group_of(offsets, e, rows, lo, busy);
+            last = e;
+        }
+        if (!busy) continue;                           // an expert without rows is not decoded
+        const int n0 = (l % nb) * DN, k0 = (l / nb) * DK, kts = min(DK, k - k0) / 16;
+        __syncthreads();
+        TileWords<K> w[4];
+        const int64_t tiles_n = n / 16;
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+            if (a < kts) w[a].load(trellis + (((int64_t)e * (k / 16) + k0 / 16 + a) * tiles_n + n0 / 16 + warp) * 8 * K, lane);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            if (a >= kts) break;
+            uint32_t f[4];
+            decode_tile<K, DEC>(w[a], lane, smem, f);
+            uint32_t* o = reinterpret_cast<uint32_t*>(stage + (warp * 16 + (lane >> 2)) * DPAD + a * 16 + 2 * (lane & 3));
+            o[0] = f[0];
+            o[4] = f[1];
+            o[8 * DPAD / 2] = f[2];
+            o[8 * DPAD / 2 + 4] = f[3];
+        }
+        __syncthreads();
+        const int lines = kts * 2;                     // 16-byte pieces of a row
+        for (int p = threadIdx.x; p < DN * lines; p += 256) {
+            const int r = p / lines, c = p % lines;
+            *reinterpret_cast<uint4*>(out + ((int64_t)e * n + n0 + r) * k + k0 + c * 8) =
+                *reinterpret_cast<const uint4*>(stage + r * DPAD + c * 8);
+        }
+    }
+}
+
+// Rows of no expert, zeroed in a fresh output.
+template <typename T>
+__global__ void zero_rest_kernel(const int64_t* offsets, int experts, int rows, int n, T* y, int64_t ldy) {
+    int first, last, c;
+    group_of(offsets, 0, rows, first, c);
+    group_of(offsets, experts - 1, rows, last, c);
+    last += c;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        if (row >= first && row < last) continue;
+        for (int j = threadIdx.x; j < n; j += blockDim.x) y[(int64_t)row * ldy + j] = from_f<T>(0.f);
+    }
+}
+
+int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
+
+struct Layout { int64_t xr, scale, w, bytes; };
+
+Layout layout(const kq_trellis_product& p) {
+    Layout l;
+    l.xr = 0;
+    l.scale = align128(p.rows * p.k * 2);
+    l.w = l.scale + align128(p.rows * 4);
+    l.bytes = l.w + p.experts * p.k * p.n * 2;
+    return l;
+}
+
+int check_trellis(const kq_trellis_product& p, const char* what) {
+    if (p.rows < 0 || p.rows > 0x7FFFFF00 || p.k <= 0 || p.n <= 0 || p.k % kBlock || p.n % kBlock || p.k > (1 << 24) ||
+        p.n > (1 << 24) || p.experts <= 0 || p.experts > kMaxExperts || p.bits < 1 || p.bits > 8) {
+        set_error("%s: need k and n multiples of 128, 1..1024 experts, 1..8 bits (rows=%lld k=%lld n=%lld experts=%lld bits=%d)", what,
+                  (long long)p.rows, (long long)p.k, (long long)p.n, (long long)p.experts, p.bits);
+        return KQ_ERR_ARG;
+    }
+    if (p.experts > 1 && !p.offsets) { set_error("%s: several experts need offsets", what); return KQ_ERR_ARG; }
+    if (p.dtype != KQ_BF16 && p.dtype != KQ_FP16) { set_error("%s: dtype must be KQ_BF16 or KQ_FP16", what); return KQ_ERR_ARG; }
+    if (p.codebook != KQ_CB_MCG && p.codebook != KQ_CB_SQG && p.codebook != KQ_CB_LABELS) {
+        set_error("%s: codebook must be KQ_CB_MCG, KQ_CB_SQG or KQ_CB_LABELS", what);
+        return KQ_ERR_ARG;
+    }
+    if (p.rows > 1 && (p.ldx < p.k || p.ldy < p.n)) { set_error("%s: row strides too small", what); return KQ_ERR_ARG; }
+    return KQ_OK;
+}
+
+template <int K, int DEC>
+int launch_decode(const kq_trellis_product& p, __half* out, cudaStream_t s) {
+    constexpr int smem = table_bytes(DEC) + DN * DPAD * 2;
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<K, DEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    const int64_t items = (p.n / DN) * ((p.k + DK - 1) / DK) * p.experts;
+    const int per_sm = DEC == DEC_F16 ? 1 : DEC == DEC_E4M3 ? 2 : 8;
+    const int grid = (int)(items < (int64_t)sms * per_sm ? items : (int64_t)sms * per_sm);
+    decode_kernel<K, DEC><<<grid, 256, smem, s>>>(reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, (int)p.rows,
+                                                  (int)p.experts, (int)p.k, (int)p.n, out);
+    return check_launch("decode_kernel");
+}
+
+template <int K>
+int launch_decode_k(const kq_trellis_product& p, __half* out, cudaStream_t s) {
+    if (p.codebook == KQ_CB_MCG) return launch_decode<K, DEC_MCG>(p, out, s);
+    if (p.codebook == KQ_CB_SQG) return launch_decode<K, DEC_E4M3>(p, out, s);
+    return launch_decode<K, DEC_F16>(p, out, s);
+}
+
+int decode_all(const kq_trellis_product& p, __half* out, cudaStream_t s) {
+    switch (p.bits) {
+        case 1: return launch_decode_k<1>(p, out, s);
+        case 2: return launch_decode_k<2>(p, out, s);
+        case 3: return launch_decode_k<3>(p, out, s);
+        case 4: return launch_decode_k<4>(p, out, s);
+        case 5: return launch_decode_k<5>(p, out, s);
+        case 6: return launch_decode_k<6>(p, out, s);
+        case 7: return launch_decode_k<7>(p, out, s);
+        default: return launch_decode_k<8>(p, out, s);
+    }
+}
+
+template <typename T>
+int rotate_in(const kq_trellis_product& p, __half* xr, float* scale, cudaStream_t s) {
+    rotate_in_kernel<T><<<(unsigned)p.rows, 256, 0, s>>>(static_cast<const T*>(p.x), p.ldx, reinterpret_cast<const __half*>(p.suh),
+                                                         p.suh_stride_e, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, xr, scale);
+    return check_launch("rotate_in_kernel");
+}
+
+}  // namespace
+}  // namespace kq
+
+extern "C" size_t kq_trellis_linear_workspace_bytes(const kq_trellis_product* p) {
+    if (!p || kq::check_trellis(*p, "kq_trellis_linear_workspace_bytes") || p->rows == 0) return 0;
+    return (size_t)kq::layout(*p).bytes;
+}
+
+extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace kq;
+    const char* what = "kq_trellis_linear";
+    if (!pp) { set_error("%s: null pointer", what); return KQ_ERR_ARG; }
+    const kq_trellis_product& p = *pp;
+    if (int rc = check_trellis(p, what)) return rc;
+    if (p.rows == 0) return KQ_OK;
+    if (!p.x || !p.trellis || !p.suh || !p.svh || !p.y || (p.codebook != KQ_CB_MCG && !p.table)) {
+        set_error("%s: null pointer", what);
+        return KQ_ERR_ARG;
+    }
+    if (((uintptr_t)p.trellis & 15) || ((uintptr_t)p.table & 15) || (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.suh | (uintptr_t)p.svh) & 1)) {
+        set_error("%s: trellis and table need 16-byte alignment", what);
+        return KQ_ERR_ALIGN;
+    }
+    const Layout l = layout(p);
+    if (!workspace || workspace_bytes < (size_t)l.bytes) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
+    if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    __half *xr = reinterpret_cast<__half*>(ws + l.xr), *w = reinterpret_cast<__half*>(ws + l.w);
+    float* scale = reinterpret_cast<float*>(ws + l.scale);
+    const bool bf16 = p.dtype == KQ_BF16;
+    if (int rc = bf16 ? rotate_in<__nv_bfloat16>(p, xr, scale, s) : rotate_in<__half>(p, xr, scale, s)) return rc;
+    if (p.zero_rest && p.offsets) {
+        const int grid = (int)(p.rows < 1024 ? p.rows : 1024);
+        if (bf16) zero_rest_kernel<<<grid, 256, 0, s>>>(p.offsets, (int)p.experts, (int)p.rows, (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy);
+        else zero_rest_kernel<<<grid, 256, 0, s>>>(p.offsets, (int)p.experts, (int)p.rows, (int)p.n, static_cast<__half*>(p.y), p.ldy);
+        if (int rc = check_launch("zero_rest_kernel")) return rc;
+    }
+    if (int rc = decode_all(p, w, s)) return rc;
+    return rows_product_rotated(reinterpret_cast<const uint16_t*>(xr), reinterpret_cast<const uint16_t*>(w), p.offsets, p.rows, p.k, p.n,
+                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, s);
+}

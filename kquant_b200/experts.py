@@ -161,3 +161,56 @@ def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offse
         db = torch.empty((E, n), dtype=dt, device=dev)
         _native.expert_bias_grad(dz, offsets, db, p.dtype)
     return dx, dw, db
+
+
+def trellis_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, svh: torch.Tensor,
+                   offsets: torch.Tensor | None = None, *, codebook: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """x[r] times the encoded matrix of each row's expert, decoded from its packed payload on the way.
+
+    x [rows, k] bf16 or fp16, trellis [experts, k/16, n/16, 16 K] int16 as the encoder packs it, suh [experts, k] and
+    svh [experts, n] fp16: ``{"suh", "svh", "trellis"}`` of the encoder's results, stacked over the experts of one
+    rate K.  One encoded matrix goes without the experts dimension and without offsets.  ``codebook``: None for MCG,
+    the 65,536 E4M3 bytes of an SQG table, or 65,536 binary16 labels (int16 bits, ``_native.build_labels``).
+    """
+    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES:
+        raise TypeError("x must be a torch.bfloat16 or torch.float16 tensor")
+    dev = x.device
+    if isinstance(trellis, torch.Tensor) and trellis.ndim == 3 and offsets is None:
+        trellis, suh, svh = trellis[None], suh[None], svh[None]
+    _operand(x, "x", 2, x.dtype, dev)
+    _operand(trellis, "trellis", 4, torch.int16, dev)
+    E, k, n, K = trellis.shape[0], 16 * trellis.shape[1], 16 * trellis.shape[2], trellis.shape[3] // 16
+    if not trellis.is_contiguous() or trellis.shape[3] % 16 or not 1 <= K <= 8:
+        raise ValueError("trellis must be contiguous [experts, k/16, n/16, 16 K] words with K in 1..8")
+    if E < 1 or k < 1 or n < 1 or k % 128 or n % 128:
+        raise ValueError(f"trellis must hold at least one matrix with k and n multiples of 128, got {E} of [{k}, {n}]")
+    _rows_operand(x, "x", x.shape[0], k, x.dtype, dev)
+    _check_offsets(offsets, E, dev)
+    for name, t, size in (("suh", suh, k), ("svh", svh, n)):
+        _operand(t, name, 2, torch.float16, dev)
+        if t.shape != (E, size) or t.stride(1) != 1:
+            raise ValueError(f"{name} must be [{E}, {size}] with unit stride along its last dimension")
+    p = _native.TrellisProduct()
+    p.codebook = _native.KQ_CB_MCG
+    if codebook is not None:
+        if not isinstance(codebook, torch.Tensor) or codebook.dtype not in (torch.uint8, torch.int16):
+            raise TypeError("codebook must be None, uint8 E4M3 bytes or int16 binary16 labels")
+        _operand(codebook, "codebook", 1, codebook.dtype, dev)
+        if codebook.numel() != 65536 or not codebook.is_contiguous():
+            raise ValueError("codebook must hold 65,536 contiguous values")
+        p.codebook = _native.KQ_CB_SQG if codebook.dtype == torch.uint8 else _native.KQ_CB_LABELS
+        p.table = codebook.data_ptr()
+    if out is None:
+        out = torch.empty((x.shape[0], n), dtype=x.dtype, device=dev)
+        p.zero_rest = 1
+    else:
+        _rows_operand(out, "out", x.shape[0], n, x.dtype, dev)
+    p.x, p.trellis, p.suh, p.svh, p.offsets, p.y = (x.data_ptr(), trellis.data_ptr(), suh.data_ptr(), svh.data_ptr(),
+                                                    _ptr(offsets), out.data_ptr())
+    p.rows, p.k, p.n, p.experts = x.shape[0], k, n, E
+    p.ldx, p.ldy, p.suh_stride_e, p.svh_stride_e = x.stride(0), out.stride(0), suh.stride(0), svh.stride(0)
+    p.bits, p.dtype = K, _DTYPES[x.dtype]
+    if p.rows:
+        _native.trellis_linear(p, dev)
+    return out

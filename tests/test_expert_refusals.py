@@ -120,3 +120,41 @@ def test_expert_hessian_c_entry_refuses(change, status):
              den=64, ws=None, size=0, stream=None)
     a.update(change)
     assert _native.load().kq_accumulate_expert_hessians(*a.values()) == status
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(x=torch.zeros(4, 128, dtype=torch.bfloat16)), _native.KQError, "CUDA"),
+    (dict(x=fake(4, 128, dtype=torch.float32)), TypeError, "bfloat16"),
+    (dict(x=fake(4, 256)), ValueError, "x must be"),
+    (dict(trellis=fake(2, 8, 8, 48, dtype=torch.int32)), TypeError, "int16"),
+    (dict(trellis=fake(2, 8, 8, 40, dtype=torch.int16)), ValueError, "16 K"),
+    (dict(trellis=fake(2, 8, 8, 144, dtype=torch.int16)), ValueError, "K in 1..8"),
+    (dict(trellis=fake(2, 8, 16, 48, dtype=torch.int16)[:, :, ::2]), ValueError, "contiguous"),
+    (dict(trellis=fake(2, 8, 9, 48, dtype=torch.int16)), ValueError, "multiples of 128"),
+    (dict(suh=fake(2, 128)), TypeError, "suh"),
+    (dict(svh=fake(2, 64, dtype=torch.float16)), ValueError, "svh"),
+    (dict(offsets=None), ValueError, "offsets"),
+    (dict(codebook=fake(65536, dtype=torch.int32)), TypeError, "codebook"),
+    (dict(codebook=fake(4096, dtype=torch.uint8)), ValueError, "65,536"),
+    (dict(out=fake(4, 64)), ValueError, "out"),
+])
+def test_trellis_linear_refuses(change, error, match):
+    args = dict(x=fake(4, 128), trellis=fake(2, 8, 8, 48, dtype=torch.int16), suh=fake(2, 128, dtype=torch.float16),
+                svh=fake(2, 128, dtype=torch.float16), offsets=fake(3, dtype=torch.int64))
+    args.update(change)
+    with pytest.raises(error, match=match):
+        experts.trellis_linear(**args)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(rows=-1), -1), (dict(k=64), -1), (dict(n=130), -1), (dict(experts=0), -1), (dict(bits=0), -1), (dict(bits=9), -1),
+    (dict(experts=2, offsets=None), -1), (dict(dtype=2), -1), (dict(codebook=2), -1), (dict(ldx=100), -1), (dict(x=None), -1),
+    (dict(codebook=4), -1), (dict(trellis=72), -4), (dict(), -2),
+])
+def test_trellis_c_entry_refuses(change, status):
+    p = _native.TrellisProduct(x=64, trellis=64, suh=64, svh=64, offsets=64, y=64, rows=4, k=128, n=128, experts=1, ldx=128, ldy=128,
+                               suh_stride_e=128, svh_stride_e=128, bits=3, codebook=1)
+    for k, v in change.items():
+        setattr(p, k, v)
+    assert _native.load().kq_trellis_linear(ctypes.byref(p), None, 0, None) == status
+    assert _native.load().kq_trellis_linear(None, None, 0, None) == -1
