@@ -8,13 +8,24 @@
 // activation (of the gate, times up, when gated) and adds the residual; its
 // gradient form turns the recomputed pre-activation z and dy into dz.
 //
-// One persistent CTA per SM, 128 x 256 output tiles (gated: 128 columns of
-// gate and the same 128 of up side by side).  Warp 0 issues TMA into a ring of
-// 64-deep stages, warp 1 issues tcgen05.mma, warps 2..9 drain; two 256-column
+// A pair of CTAs (cta_group::2) shares one output tile, persistent, one CTA
+// per SM.  The M axis of the tensor product is the output's contiguous axis:
+// 256 features of W, 128 per CTA (gated: 64 of gate and the same 64 of up in
+// each).  The N axis is the rows, 64 to 256 of them: an expert's last tile
+// costs what its rows need, where row tiles of 128 or 256 on the M axis would
+// waste 11% or 31% of the products of an unevenly routed prompt (8192 rows, 16
+// experts).  Against one CTA per tile a pair reads half as much of B into each
+// shared memory: 64 KB move per 512 tensor cycles instead of 96 KB, which had
+// held the one-CTA form at 0.55 of the tensor peak.
+//
+// Warp 0 of each CTA issues TMA into a ring of 64-deep stages; warp 1 of the
+// leader issues tcgen05.mma for the pair; warps 2..9 drain.  Two 256-column
 // accumulators alternate, so a tile's epilogue runs under the next tile's
-// products.  Both operands may be K-major or MN-major in shared memory: W is
-// taken as stored ([k][n] or [n][k]), and the sums product reads x and dz as
-// they are, contracting over their rows.
+// products.  A thread drains one feature (TMEM lane), so a warp's 2-byte
+// accesses to a row are 64 consecutive bytes, whatever the row stride.
+// Both operands may be K-major or MN-major in shared memory: W is taken as
+// stored ([k][n] or [n][k]), and the sums product reads x and dz as they are,
+// contracting over their rows.
 //
 // The offsets stay on the device: every CTA scans them into shared memory and
 // walks the same tile order, so a call captured into a graph follows new
@@ -29,89 +40,136 @@ namespace {
 
 __device__ int g_wait_error = 0;
 
-constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int CHUNK = 64 * 128;                 // 64 rows of 128 bytes: one MN-major box
+constexpr int BK = 64, STAGES = 6;
+constexpr int TILE = 256;                       // features and rows of a pair's tile, at most
+constexpr int SIDE_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * SIDE_BYTES;   // a CTA's half of A and of B
+constexpr int CHUNK = 64 * 128;                 // 64 rows of 128 bytes: one TMA box, one MN-major slab
 constexpr int DRAIN_WARPS = 8, THREADS = 64 + 32 * DRAIN_WARPS;
+constexpr int EXCHANGE_BYTES = DRAIN_WARPS * 2 * 8 * 32 * 4;
 constexpr int GROUP_BYTES = (3 * kMaxExperts + 4) * 4;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GROUP_BYTES + 1024;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EXCHANGE_BYTES + GROUP_BYTES + 1024;
 
-enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS, EPI_ROTATED };
+enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS };
 
 struct Params {
     const int64_t* offsets;
     const void* bias;
-    const void* aux;       // residual (forward), dy (gradient) or svh (rotated)
-    const float* row_scale;
+    const void* aux;       // residual (forward) or dy (gradient)
     void* out;
     int64_t bias_stride, ld_aux, ld_out, out_stride;   // out_stride: per expert (sums)
-    int rows, experts, k_steps, m_tiles, n_tiles, m_out, n_out;
-    int w_second;          // coordinate of the tile's second 128 columns, relative to its first
-    int out_second;        // column of dz's up half
+    int rows, experts, k_steps, m_tiles, n_tiles;
+    int m_out, n_out;      // output extents: features, and (sums) rows
+    int up;                // gated: first coordinate of the up half in W
     int* err;
-    uint32_t idesc;
+    uint32_t idesc;        // without N
     int act;
-    bool a_mn, b_mn, zero_rest, vec_bias, vec_aux, vec_out;
+    bool a_mn, b_mn, zero_rest;
 };
 
-struct Tile { int e, row0, count, m0, n0, k_steps; };
+struct Tile { int e, row0, count, m0, n0, n, k_steps; };
 
-// Tile t of the launch.  Rows: the row tiles of an expert run fastest, so the
-// CTAs that share a slice of W run together.
-template <int EPI>
+// Tile t of the launch; m0 in features, n the extent of the tensor product's N axis.
+template <int EPI, bool GATED>
 __device__ __forceinline__ bool tile_at(const Params& p, const int* lo, const int* cnt, const int* cum, int64_t t, Tile& o) {
     if constexpr (EPI == EPI_SUMS) {
         const int per = p.m_tiles * p.n_tiles;
         if (t >= (int64_t)per * p.experts) return false;
         o.e = (int)(t / per);
         const int l = (int)(t - (int64_t)o.e * per);
-        o.m0 = (l % p.m_tiles) * BM;
-        o.n0 = (l / p.m_tiles) * BN;
+        o.m0 = (l % p.m_tiles) * TILE;
+        o.n0 = (l / p.m_tiles) * TILE;
         o.row0 = lo[o.e];
         o.count = cnt[o.e];
+        o.n = p.n_out - o.n0 > 128 ? 256 : 128;
         o.k_steps = (o.count + BK - 1) / BK;
     } else {
-        if (t >= (int64_t)cum[p.experts] * p.n_tiles) return false;
-        o.e = expert_of(cum, p.experts, (int)(t / p.n_tiles));
-        const int mt = cum[o.e + 1] - cum[o.e];
-        const int64_t l = t - (int64_t)cum[o.e] * p.n_tiles;
-        o.m0 = (int)(l % mt) * BM;
-        o.n0 = (int)(l / mt);                   // tile index; the caller scales it
-        o.row0 = lo[o.e] + o.m0;
-        o.count = cnt[o.e] - o.m0;
+        // The row tiles of an expert run fastest: the pairs that share a slice of W run together.
+        if (t >= (int64_t)cum[p.experts] * p.m_tiles) return false;
+        o.e = expert_of(cum, p.experts, (int)(t / p.m_tiles));
+        const int nt = cum[o.e + 1] - cum[o.e];
+        const int64_t l = t - (int64_t)cum[o.e] * p.m_tiles;
+        const int r = (int)(l % nt) * TILE;
+        o.m0 = (int)(l / nt) * (GATED ? TILE / 2 : TILE);
+        o.n0 = 0;
+        o.row0 = lo[o.e] + r;
+        o.count = min(cnt[o.e] - r, TILE);
+        o.n = (o.count + 63) & ~63;
         o.k_steps = p.k_steps;
     }
     return true;
 }
 
+// Zeroes rows valid .. 63 of a sums stage in this CTA once its loads have landed.  Whole warp.
+__device__ __forceinline__ bool zero_tail(uint8_t* stage, int slabs, int valid, uint64_t* tail_bar, uint32_t parity, int lane) {
+    const bool ok = mbar_wait(tail_bar, parity);
+    const int missing = BK - valid, pieces = slabs * missing * 8;
+    for (int i = lane; i < pieces; i += 32) {
+        const int line = i >> 3, c = line / missing, r = valid + line % missing;
+        *reinterpret_cast<uint4*>(stage + c * CHUNK + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    return ok;
+}
+
+// W rows of one feature: pre-activations z (and up projections u) to results, the first `rows` stored.
+template <typename T, int EPI, bool GATED, int ACT, int W>
+__device__ __forceinline__ void finish(T* o, int64_t ld, int second, int rows, const float (&z)[W], const float (&u)[W],
+                                       const float (&a)[W]) {
+    T y[W], y2[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        if constexpr (EPI == EPI_FORWARD) {
+            y[j] = from_f<T>(activate<ACT>(z[j]) * (GATED ? u[j] : 1.f) + a[j]);
+        } else if constexpr (GATED) {
+            y[j] = from_f<T>(a[j] * u[j] * slope<ACT>(z[j]));
+            y2[j] = from_f<T>(a[j] * activate<ACT>(z[j]));
+        } else {
+            y[j] = from_f<T>(a[j] * slope<ACT>(z[j]));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        if (j < rows) {
+            o[j * ld] = y[j];
+            if constexpr (EPI == EPI_GRAD && GATED) o[j * ld + second] = y2[j];
+        }
+    }
+}
+
 template <typename T, int EPI, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
-expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+              const __grid_constant__ CUtensorMap map_b_full, const Params p) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tail_bar[STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    int* lo = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES);
+    float* exchange = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
+    int* lo = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + EXCHANGE_BYTES);
     int* cnt = lo + kMaxExperts;
     int* cum = cnt + kMaxExperts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int NW = GATED ? 128 : BN;        // output columns of a rows tile
+    const int rank = (int)cluster_rank();
+    const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
+            mbar_init(&tail_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], DRAIN_WARPS);
+            mbar_init(&acc_empty[b], 2 * DRAIN_WARPS);
         }
         mbar_init_fence();
     }
-    if (warp == 1) tmem_alloc(&tmem_slot, 2 * BN);
-    scan_groups(p.offsets, p.experts, p.rows, BM, lo, cnt, cum);
+    if (warp == 1) tmem2_alloc(&tmem_slot, 2 * TILE);
+    scan_groups(p.offsets, p.experts, p.rows, TILE, lo, cnt, cum);
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     bool ok = true;
@@ -120,29 +178,41 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
-            for (int64_t i = blockIdx.x; ok && tile_at<EPI>(p, lo, cnt, cum, i, t); i += gridDim.x) {
+            for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
+                const int half = t.n >> 1;
+                const uint32_t bytes = SIDE_BYTES + half * 128;
+                const int fa = t.m0 + rank * (GATED ? 64 : 128), fb = GATED ? p.up + fa : fa + 64;
                 for (int ks = 0; ks < t.k_steps; ++ks, ++it) {
                     const int s = it % STAGES;
                     if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
-                    mbar_expect_tx(&full_bar[s], STAGE_BYTES);
-                    uint8_t *sa = smem + s * STAGE_BYTES, *sb = sa + A_BYTES;
+                    uint8_t *sa = smem + s * STAGE_BYTES, *sb = sa + SIDE_BYTES;
+                    uint32_t bar = leader_addr(&full_bar[s]);
                     if constexpr (EPI == EPI_SUMS) {
                         const int r = t.row0 + ks * BK;
-#pragma unroll
-                        for (int c = 0; c < BM / 64; ++c) tma_load_2d(sa + c * CHUNK, &map_a, t.m0 + 64 * c, r, &full_bar[s]);
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c) tma_load_2d(sb + c * CHUNK, &map_b, t.n0 + 64 * c, r, &full_bar[s]);
+                        if (t.count - ks * BK < BK) {      // the tail is zeroed here before it counts as loaded
+                            bar = smem_addr(&tail_bar[s]);
+                            mbar_expect_tx(&tail_bar[s], bytes);
+                        } else if (rank == 0) {
+                            mbar_expect_tx(&full_bar[s], 2 * bytes);
+                        }
+                        tma2_load_2d(sa, &map_a, fa, r, bar);
+                        tma2_load_2d(sa + CHUNK, &map_a, fb, r, bar);
+                        for (int c = 0; c < half; c += 64)
+                            tma2_load_2d(sb + (c >> 6) * CHUNK, &map_b, t.n0 + rank * half + c, r, bar);
                     } else {
-                        const int n0 = t.n0 * NW, n1 = n0 + p.w_second;
-                        tma_load_2d(sa, &map_a, ks * BK, t.row0, &full_bar[s]);
-                        if (p.b_mn) {
-                            tma_load_3d(sb, &map_b, n0, ks * BK, t.e, &full_bar[s]);
-                            tma_load_3d(sb + CHUNK, &map_b, n0 + 64, ks * BK, t.e, &full_bar[s]);
-                            tma_load_3d(sb + 2 * CHUNK, &map_b, n1, ks * BK, t.e, &full_bar[s]);
-                            tma_load_3d(sb + 3 * CHUNK, &map_b, n1 + 64, ks * BK, t.e, &full_bar[s]);
+                        if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * bytes);
+                        if (p.a_mn) {
+                            tma2_load_3d(sa, &map_a, fa, ks * BK, t.e, bar);
+                            tma2_load_3d(sa + CHUNK, &map_a, fb, ks * BK, t.e, bar);
                         } else {
-                            tma_load_3d(sb, &map_b, ks * BK, n0, t.e, &full_bar[s]);
-                            tma_load_3d(sb + B_BYTES / 2, &map_b, ks * BK, n1, t.e, &full_bar[s]);
+                            tma2_load_3d(sa, &map_a, ks * BK, fa, t.e, bar);
+                            if (GATED) tma2_load_3d(sa + CHUNK, &map_a, ks * BK, fb, t.e, bar);
+                        }
+                        if (half == 128) {
+                            tma2_load_2d(sb, &map_b_full, ks * BK, t.row0 + rank * half, bar);
+                        } else {
+                            for (int c = 0; c < half; c += 32)
+                                tma2_load_2d(sb + c * 128, &map_b, ks * BK, t.row0 + rank * half + c, bar);
                         }
                     }
                 }
@@ -150,181 +220,150 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (!ok) report_wait_error(p.err);
         }
     } else if (warp == 1) {
-        uint32_t it = 0, tile_no = 0;
+        uint32_t it = 0, tile_no = 0, tails = 0;   // tails: the phase of every stage's tail_bar
         const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;   // 16 contraction values, in 16-byte units
-        for (int64_t i = blockIdx.x; ok && tile_at<EPI>(p, lo, cnt, cum, i, t); i += gridDim.x, ++tile_no) {
+        for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step, ++tile_no) {
             const int b = tile_no & 1;
-            if (!(ok = mbar_wait(&acc_empty[b], ((tile_no >> 1) & 1) ^ 1))) break;
+            const int tail_step = EPI == EPI_SUMS && t.count % BK ? t.k_steps - 1 : -1;
+            const int slabs = 2 + (t.n >> 7);
+            if (rank != 0) {                    // the leader issues for both; this CTA zeroes its own tails
+                if (tail_step >= 0) {
+                    const int s = (it + tail_step) % STAGES;
+                    ok = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane);
+                    if (lane == 0) mbar_arrive_remote(leader_addr(&full_bar[s]));
+                    tails ^= 1u << s;
+                }
+                it += t.k_steps;
+                continue;
+            }
+            if (!(ok = mbar_wait_cluster(&acc_empty[b], ((tile_no >> 1) & 1) ^ 1))) break;
             tc_fence_after();
+            const uint32_t idesc = p.idesc | ((uint32_t)(t.n >> 3) << 17);
             for (int ks = 0; ks < t.k_steps; ++ks, ++it) {
                 const int s = it % STAGES;
-                if (!(ok = mbar_wait(&full_bar[s], (it / STAGES) & 1))) break;
-                uint8_t* sa = smem + s * STAGE_BYTES;
-                if constexpr (EPI == EPI_SUMS) {
-                    const int valid = t.count - ks * BK;
-                    if (valid < BK) {           // rows of the next expert: one 128-byte line a row and chunk
-                        const int lines = (BK - valid) * (STAGE_BYTES / CHUNK);
-                        for (int l = lane; l < lines * 8; l += 32) {
-                            const int line = l >> 3, c = line / (BK - valid), r = valid + line % (BK - valid);
-                            *reinterpret_cast<uint4*>(sa + c * CHUNK + r * 128 + (l & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
+                if (ks == tail_step) {          // the only arrival on full_bar is the other CTA's, for its zeroed half
+                    ok = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane) &&
+                         mbar_wait_cluster(&full_bar[s], (it / STAGES) & 1);
+                    tails ^= 1u << s;
                 }
+                if (!(ok = ok && mbar_wait(&full_bar[s], (it / STAGES) & 1))) break;
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint32_t a = smem_addr(sa);
-                    const uint64_t ad = smem_desc(a, p.a_mn ? CHUNK : 16), bd = smem_desc(a + A_BYTES, p.b_mn ? CHUNK : 16);
+                    const uint32_t a = smem_addr(smem + s * STAGE_BYTES);
+                    const uint64_t ad = smem_desc(a, p.a_mn ? CHUNK : 16), bd = smem_desc(a + SIDE_BYTES, p.b_mn ? CHUNK : 16);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk)
-                        mma_f16(tmem + b * BN, ad + a_step * kk, bd + b_step * kk, p.idesc, (ks | kk) != 0);
-                    mma_commit(&empty_bar[s]);
+                        mma2_f16(tmem + b * TILE, ad + a_step * kk, bd + b_step * kk, idesc, (ks | kk) != 0);
+                    mma2_commit(&empty_bar[s]);
                 }
                 __syncwarp();
             }
-            if (ok && lane == 0) mma_commit(&acc_full[b]);
+            if (ok && lane == 0) mma2_commit(&acc_full[b]);
             __syncwarp();
         }
         if (!ok && lane == 0) report_wait_error(p.err);
     } else {
-        const int q = warp & 3, h = (warp - 2) >> 2;    // tensor-memory lanes 32q.., column half h
-        const int r = q * 32 + lane;
-        uint32_t tile_no = 0;
-        for (int64_t i = blockIdx.x; tile_at<EPI>(p, lo, cnt, cum, i, t); i += gridDim.x, ++tile_no) {
+        const int q = warp & 3, h = (warp - 2) >> 2;    // tensor-memory lanes 32q.., every other 16 columns
+        uint32_t tile_no = 0, turn = 0;
+        for (int64_t i = first; tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step, ++tile_no) {
             const int b = tile_no & 1;
             if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[b], (tile_no >> 1) & 1)))) break;
             tc_fence_after();
-            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN);
-            const bool live = EPI == EPI_SUMS ? t.m0 + r < p.m_out : r < t.count;
-            constexpr int HALF = EPI == EPI_SUMS ? BN / 2 : NW / 2;
-            const int n_base = (EPI == EPI_SUMS ? t.n0 : t.n0 * NW) + h * HALF;
-            const T* bias = p.bias ? static_cast<const T*>(p.bias) + t.e * p.bias_stride : nullptr;
-            T* orow;
-            const T* arow = nullptr;
+            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * TILE);
+            const int f = t.m0 + (GATED ? rank * 64 + (q & 1) * 32 : rank * 128 + q * 32) + lane;
+            const bool live = f < p.m_out;
             if constexpr (EPI == EPI_SUMS) {
-                orow = static_cast<T*>(p.out) + t.e * p.out_stride + (int64_t)(t.m0 + r) * p.ld_out;
-            } else {
-                orow = static_cast<T*>(p.out) + (int64_t)(t.row0 + r) * p.ld_out;
-                if (EPI != EPI_ROTATED && p.aux) arow = static_cast<const T*>(p.aux) + (int64_t)(t.row0 + r) * p.ld_aux;
-            }
-            if constexpr (EPI == EPI_ROTATED) {
-                // A thread holds one row of one 128-column Hadamard block: the transform stays in its registers.
-                if (n_base < p.n_out) {
-                    float z[128];
+                T* out = static_cast<T*>(p.out) + t.e * p.out_stride + f;
+                const int cols = min(p.n_out - t.n0, TILE);
+#pragma unroll 1
+                for (int c = h * 16; c < cols; c += 32) {
+                    uint32_t v[16];
+                    tmem_ld16(base + c, v);
+                    tmem_wait_ld();
+                    T* o = out + (int64_t)(t.n0 + c) * p.ld_out;
 #pragma unroll
-                    for (int c = 0; c < 128; c += 16) {
-                        uint32_t v[16];
-                        tmem_ld16(base + h * HALF + c, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) z[c + e] = __uint_as_float(v[e]);
-                    }
-#pragma unroll
-                    for (int d = 1; d < 128; d <<= 1)
-#pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            if (!(e & d)) {
-                                const float a = z[e], c = z[e + d];
-                                z[e] = a + c;
-                                z[e + d] = a - c;
-                            }
-                    if (live) {
-                        const float scale = p.row_scale[t.row0 + r] * 0.08838834764831845f;   // 1 / sqrt(128)
-                        const __half* svh = static_cast<const __half*>(p.aux) + t.e * p.ld_aux + n_base;
-#pragma unroll
-                        for (int c = 0; c < 128; c += 8) {
-                            float a[8];
-                            load8(svh + c, p.vec_aux, 8, a);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) a[e] *= z[c + e] * scale;
-                            store8(orow + n_base + c, p.vec_out, 8, a);
-                        }
-                    }
+                    for (int j = 0; j < 16; ++j)
+                        if (live && c + j < cols) o[j * p.ld_out] = from_f<T>(t.k_steps ? __uint_as_float(v[j]) : 0.f);
                     __syncwarp();
                 }
             } else {
+                const T* bias = static_cast<const T*>(p.bias) + t.e * p.bias_stride;
+                const bool up = GATED && q >= 2;        // this warp's lanes hold up, not gate
+                const float add = p.bias && live ? to_f<T>(bias[(up ? p.m_out : 0) + f]) : 0.f;
+                T* out = static_cast<T*>(p.out) + (int64_t)t.row0 * p.ld_out + f;
+                // Loads take rows and features clamped into the tile, so that none of them hangs on a branch.
+                const T* aux = p.aux ? static_cast<const T*>(p.aux) + (int64_t)t.row0 * p.ld_aux + min(f, p.m_out - 1) : nullptr;
+                const int last = t.count - 1;
+                constexpr int W = GATED ? 8 : 16;       // rows that a thread finishes of each 16
+                T next[W];
+                auto fetch = [&](int c) {
+                    const int r0 = c + (up ? 8 : 0);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) next[j] = aux[(int64_t)min(r0 + j, last) * p.ld_aux];
+                };
+                if (aux && h * 16 < t.count) fetch(h * 16);
 #pragma unroll 1
-            for (int c = 0; c < HALF; c += 16) {
-                if (n_base + c >= p.n_out) break;
-                uint32_t v[16], u[16];
-                tmem_ld16(base + h * HALF + c, v);
-                if constexpr (GATED) tmem_ld16(base + 128 + h * HALF + c, u);
-                tmem_wait_ld();
-                if (EPI == EPI_SUMS && t.k_steps == 0) {
+                for (int c = h * 16; c < t.count; c += 32) {
+                    uint32_t v[16];
+                    tmem_ld16(base + c, v);
+                    float a[W], z[W], u[W];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = 0;
+                    for (int j = 0; j < W; ++j) a[j] = aux ? to_f<T>(next[j]) : 0.f;
+                    if (aux && c + 32 < t.count) fetch(c + 32);       // under this chunk's arithmetic
+                    tmem_wait_ld();
+                    if constexpr (GATED) {
+                        // Gate and up of a feature lie in two warps: each sends the other 8 of its 16 rows.
+                        float* mine = exchange + ((warp - 2) * 2 + (turn & 1)) * 256;
+                        const float* theirs = exchange + (((warp - 2) ^ 2) * 2 + (turn & 1)) * 256;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) mine[j * 32 + lane] = __uint_as_float(up ? v[j] : v[8 + j]) + add;
+                        asm volatile("bar.sync %0, 64;" ::"r"(1 + h * 2 + (q & 1)) : "memory");
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float own_v = __uint_as_float(up ? v[8 + j] : v[j]) + add, other = theirs[j * 32 + lane];
+                            z[j] = up ? other : own_v;
+                            u[j] = up ? own_v : other;
+                        }
+                        ++turn;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) z[j] = __uint_as_float(v[j]) + add;
+                    }
+                    const int r0 = c + (up ? 8 : 0);
+                    T* o = out + (int64_t)r0 * p.ld_out;
+                    const int rows = live ? min(t.count - r0, W) : 0;
+                    switch (p.act) {
+                        case KQ_ACT_RELU: finish<T, EPI, GATED, KQ_ACT_RELU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
+                        case KQ_ACT_SILU: finish<T, EPI, GATED, KQ_ACT_SILU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
+                        case KQ_ACT_GELU: finish<T, EPI, GATED, KQ_ACT_GELU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
+                        default: finish<T, EPI, GATED, KQ_ACT_NONE, W>(o, p.ld_out, p.m_out, rows, z, u, a);
+                    }
+                    __syncwarp();
                 }
-#pragma unroll
-                for (int g = 0; g < 2 && live; ++g) {
-                    const int j = n_base + c + 8 * g, nv = p.n_out - j;
-                    if (nv <= 0) break;
-                    float z[8], w[8], a[8], d[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        z[e] = __uint_as_float(v[8 * g + e]);
-                        if constexpr (GATED) w[e] = __uint_as_float(u[8 * g + e]);
-                    }
-                    if constexpr (EPI != EPI_SUMS) {
-                        if (bias) {
-                            load8(bias + j, p.vec_bias && nv >= 8, nv, a);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) z[e] += a[e];
-                            if constexpr (GATED) {
-                                load8(bias + p.n_out + j, p.vec_bias && nv >= 8, nv, a);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) w[e] += a[e];
-                            }
-                        }
-                        if (arow) load8(arow + j, p.vec_aux && nv >= 8, nv, a);
-                    }
-                    if constexpr (EPI == EPI_FORWARD) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            z[e] = activate(p.act, z[e]);
-                            if constexpr (GATED) z[e] *= w[e];
-                            if (arow) z[e] += a[e];
-                        }
-                    }
-                    if constexpr (EPI == EPI_GRAD) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if constexpr (GATED) {
-                                d[e] = a[e] * activate(p.act, z[e]);
-                                z[e] = a[e] * w[e] * slope(p.act, z[e]);
-                            } else {
-                                z[e] = a[e] * slope(p.act, z[e]);
-                            }
-                        }
-                        if constexpr (GATED) store8(orow + p.out_second + j, p.vec_out && nv >= 8, nv, d);
-                    }
-                    store8(orow + j, p.vec_out && nv >= 8, nv, z);
-                }
-                __syncwarp();
-            }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            if (lane == 0) mbar_arrive_remote(leader_addr(&acc_empty[b]));
         }
         if (!ok && lane == 0) report_wait_error(p.err);
         // Rows of no expert: zero in a fresh output, untouched otherwise.
         if (EPI != EPI_SUMS && p.zero_rest && p.offsets) {
-            int first, last, n;
-            group_of(p.offsets, 0, p.rows, first, n);
-            group_of(p.offsets, p.experts - 1, p.rows, last, n);
-            last += n;
-            const int width = EPI == EPI_GRAD && GATED ? p.out_second + p.n_out : p.n_out;
+            int begin, end, n;
+            group_of(p.offsets, 0, p.rows, begin, n);
+            group_of(p.offsets, p.experts - 1, p.rows, end, n);
+            end += n;
             for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
-                if (row >= first && row < last) { continue; }
+                if (row >= begin && row < end) continue;
                 T* o = static_cast<T*>(p.out) + (int64_t)row * p.ld_out;
-                for (int j = threadIdx.x - 64; j < width; j += 32 * DRAIN_WARPS) o[j] = from_f<T>(0.f);
+                for (int j = threadIdx.x - 64; j < p.m_out; j += 32 * DRAIN_WARPS) o[j] = from_f<T>(0.f);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) tmem_free(tmem, 2 * BN);
+    cluster_sync();                              // the pair's memory and barriers are in use until both are here
+    tc_fence_after();
+    if (warp == 1) tmem2_free(tmem, 2 * TILE);
 }
 
 // 16-bit rows [batch][r][c] -> [batch][r][cols_out]: an operand whose base or
@@ -421,21 +460,59 @@ int map_rows_2d(CUtensorMap* m, const Operand& o, bool bf16, int box_c, int box_
                         strides, box, what);
 }
 
+// Pairs of CTAs that run at once (every instance needs a whole SM); asked once for each device.
+template <typename K>
+int pairs_at_once(K kernel, int* out) {
+    static int known[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev < 64 && known[dev]) { *out = known[dev]; return KQ_OK; }
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(sms & ~1));
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = SMEM_BYTES;
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim = {2, 1, 1};
+    c.attrs = &a;
+    c.numAttrs = 1;
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &c);
+    if (e != cudaSuccess || n < 1) { set_error("cudaOccupancyMaxActiveClusters: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+    if (dev < 64) known[dev] = n;
+    *out = n;
+    return KQ_OK;
+}
+
 template <typename T, int EPI, bool GATED>
-int launch_as(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(expert_kernel<T, EPI, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+int launch_as(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b_full, const Params& p, int64_t tiles, cudaStream_t s) {
+    auto kernel = expert_kernel<T, EPI, GATED>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
-    expert_kernel<T, EPI, GATED><<<grid, THREADS, SMEM_BYTES, s>>>(a, b, p);
+    int pairs;
+    if (int rc = pairs_at_once(kernel, &pairs)) return rc;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)));
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = SMEM_BYTES;
+    c.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim = {2, 1, 1};
+    c.attrs = &at;
+    c.numAttrs = 1;
+    e = cudaLaunchKernelEx(&c, kernel, a, b, b_full, p);
+    if (e != cudaSuccess) { set_error("expert_kernel: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     return check_launch("expert_kernel");
 }
 
 template <int EPI, bool GATED>
-int launch(bool bf16, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t s) {
-    return bf16 ? launch_as<__nv_bfloat16, EPI, GATED>(a, b, p, grid, s) : launch_as<__half, EPI, GATED>(a, b, p, grid, s);
-}
-
-bool vec8(const void* base, int64_t ld, int64_t ld2 = 0) {
-    return ((uintptr_t)base & 15) == 0 && ld % 8 == 0 && ld2 % 8 == 0;
+int launch(bool bf16, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b_full, const Params& p, int64_t tiles,
+           cudaStream_t s) {
+    return bf16 ? launch_as<__nv_bfloat16, EPI, GATED>(a, b, b_full, p, tiles, s)
+                : launch_as<__half, EPI, GATED>(a, b, b_full, p, tiles, s);
 }
 
 // The matrices of `p` as stored: columns contiguous along n or along k.
@@ -500,9 +577,11 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     const bool gated_copy = mn && p.gated && !w.direct;
     if (int rc = relayout(x, ws, 1, s)) return rc;
     if (int rc = relayout(w, ws, gated_copy ? 2 : 1, s)) return rc;
-    CUtensorMap ma, mb;
-    if (int rc = map_rows_2d(&ma, x, bf16, BK, BM, what)) return rc;
-    if (int rc = map_rows(&mb, w, bf16, mn ? 64 : BK, mn ? BK : BN / 2, what)) return rc;
+    CUtensorMap ma, mb, mf;
+    // Large boxes where the tile takes them whole: every TMA instruction of a stage costs issue time.
+    if (int rc = map_rows(&ma, w, bf16, 64, mn || p.gated ? 64 : 128, what)) return rc;
+    if (int rc = map_rows_2d(&mb, x, bf16, BK, 32, what)) return rc;
+    if (int rc = map_rows_2d(&mf, x, bf16, BK, 128, what)) return rc;
     Params q{};
     if (int rc = wait_error_word(&q.err)) return rc;
     q.offsets = p.offsets;
@@ -515,59 +594,22 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     q.rows = (int)p.rows;
     q.experts = (int)p.experts;
     q.k_steps = (int)((p.k + BK - 1) / BK);
-    const int width = p.gated ? 128 : BN;
-    q.n_tiles = (int)((n_out + width - 1) / width);
-    q.n_out = (int)n_out;
-    q.w_second = p.gated ? (int)(gated_copy ? round8(n_out) : n_out) : 128;
-    q.out_second = (int)n_out;
-    q.idesc = idesc_f16(bf16, false, mn, BM, BN);
+    const int width = p.gated ? TILE / 2 : TILE;
+    q.m_tiles = (int)((n_out + width - 1) / width);
+    q.m_out = (int)n_out;
+    q.up = (int)(gated_copy ? round8(n_out) : n_out);
+    q.idesc = idesc_f16(bf16, mn, false, TILE, 0);
     q.act = p.activation;
-    q.b_mn = mn;
+    q.a_mn = mn;
     q.zero_rest = p.zero_rest != 0;
-    q.vec_bias = vec8(p.bias, p.bias_stride_e, p.gated ? n_out : 0);
-    q.vec_aux = vec8(q.aux, q.ld_aux);
-    q.vec_out = vec8(p.y, p.ldy, grad && p.gated ? n_out : 0);
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
-    const int64_t most = ((p.rows + BM - 1) / BM + (p.experts < p.rows ? p.experts : p.rows)) * q.n_tiles;
-    const int grid = (int)(most < sms ? most : sms);
-    if (grad) return p.gated ? launch<EPI_GRAD, true>(bf16, ma, mb, q, grid, s) : launch<EPI_GRAD, false>(bf16, ma, mb, q, grid, s);
-    return p.gated ? launch<EPI_FORWARD, true>(bf16, ma, mb, q, grid, s) : launch<EPI_FORWARD, false>(bf16, ma, mb, q, grid, s);
+    const int64_t tiles = ((p.rows + TILE - 1) / TILE + (p.experts < p.rows ? p.experts : p.rows)) * q.m_tiles;
+    if (grad) return p.gated ? launch<EPI_GRAD, true>(bf16, ma, mb, mf, q, tiles, s) : launch<EPI_GRAD, false>(bf16, ma, mb, mf, q, tiles, s);
+    return p.gated ? launch<EPI_FORWARD, true>(bf16, ma, mb, mf, q, tiles, s) : launch<EPI_FORWARD, false>(bf16, ma, mb, mf, q, tiles, s);
 }
 
 __global__ void take_errors_kernel(int* out) { *out = atomicExch(&g_wait_error, 0); }
 
 }  // namespace
-
-int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
-                         int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
-                         bool bf16_out, cudaStream_t s) {
-    const char* what = "rows_product_rotated";
-    CUtensorMap ma, mb;
-    if (int rc = map_rows_2d(&ma, operand(x, 1, rows, k, 0, k), false, BK, BM, what)) return rc;
-    if (int rc = map_rows(&mb, operand(w, experts, n, k, n * k, k), false, BK, BN / 2, what)) return rc;
-    Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
-    q.offsets = offsets;
-    q.aux = svh;
-    q.ld_aux = svh_stride;
-    q.row_scale = row_scale;
-    q.out = y;
-    q.ld_out = ldy;
-    q.rows = (int)rows;
-    q.experts = (int)experts;
-    q.k_steps = (int)((k + BK - 1) / BK);
-    q.n_tiles = (int)((n + BN - 1) / BN);
-    q.n_out = (int)n;
-    q.w_second = 128;
-    q.idesc = idesc_f16(false, false, false, BM, BN);
-    q.vec_aux = vec8(svh, svh_stride);
-    q.vec_out = vec8(y, ldy);
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
-    const int64_t most = ((rows + BM - 1) / BM + (experts < rows ? experts : rows)) * q.n_tiles;
-    return launch<EPI_ROTATED, false>(bf16_out, ma, mb, q, (int)(most < sms ? most : sms), s);
-}
 
 int wait_error_word(int** out) {
     void* p = nullptr;
@@ -599,12 +641,12 @@ extern "C" int kq_expert_linear_grad_z(const kq_expert_product* p, const void* d
 namespace kq {
 namespace {
 
-// dW as stored: rows along k (columns n contiguous) or rows along n.
-struct SumsSides { Operand a, b; int64_t m, n; };
+// The sides of dW: its contiguous axis is the tensor product's M axis (a), the other its N axis (b).
+struct SumsSides { Operand a, b; };
 
 SumsSides sums_sides(const kq_expert_product& p, const void* dz, int64_t ld_dz) {
     const Operand x = operand(p.x, 1, p.rows, p.k, 0, p.ldx), z = operand(dz, 1, p.rows, p.n, 0, ld_dz);
-    return n_contiguous(p) ? SumsSides{x, z, p.k, p.n} : SumsSides{z, x, p.n, p.k};
+    return n_contiguous(p) ? SumsSides{z, x} : SumsSides{x, z};
 }
 
 }  // namespace
@@ -662,18 +704,14 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     q.out_stride = p.w_stride_e;
     q.rows = (int)p.rows;
     q.experts = (int)p.experts;
-    q.m_tiles = (int)((o.m + BM - 1) / BM);
-    q.n_tiles = (int)((o.n + BN - 1) / BN);
-    q.m_out = (int)o.m;
-    q.n_out = (int)o.n;
-    q.idesc = idesc_f16(bf16, true, true, BM, BN);
+    q.m_tiles = (int)((cols + TILE - 1) / TILE);
+    q.n_tiles = (int)((lines + TILE - 1) / TILE);
+    q.m_out = (int)cols;
+    q.n_out = (int)lines;
+    q.idesc = idesc_f16(bf16, true, true, TILE, 0);
     q.a_mn = q.b_mn = true;
-    q.vec_out = vec8(dw, ld, p.experts > 1 ? p.w_stride_e : 0);
     if ((int64_t)q.m_tiles * q.n_tiles > 0x7FFFFFFF) { set_error("%s: problem too large", what); return KQ_ERR_ARG; }
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
-    const int64_t tiles = (int64_t)q.m_tiles * q.n_tiles * p.experts;
-    return launch<EPI_SUMS, false>(bf16, ma, mb, q, (int)(tiles < sms ? tiles : sms), s);
+    return launch<EPI_SUMS, false>(bf16, ma, mb, mb, q, (int64_t)q.m_tiles * q.n_tiles * p.experts, s);
 }
 
 extern "C" int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n,

@@ -58,26 +58,23 @@ __device__ __forceinline__ int expert_of(const int* cum, int experts, int t) {
     return a;
 }
 
-__device__ __forceinline__ float activate(int act, float z) {
-    switch (act) {
-        case KQ_ACT_RELU: return z < 0.f ? 0.f : z;      // NaN stays NaN
-        case KQ_ACT_SILU: return __fdividef(z, 1.f + __expf(-z));
-        case KQ_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        default: return z;
-    }
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == KQ_ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays NaN
+    else if constexpr (ACT == KQ_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
+    else if constexpr (ACT == KQ_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    else return z;
 }
 
-__device__ __forceinline__ float slope(int act, float z) {
-    switch (act) {
-        case KQ_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case KQ_ACT_SILU: {
-            const float p = __fdividef(1.f, 1.f + __expf(-z));
-            return p * (1.f + z * (1.f - p));
-        }
-        case KQ_ACT_GELU:
-            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
-        default: return 1.f;
-    }
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == KQ_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    else if constexpr (ACT == KQ_ACT_SILU) {
+        const float p = __fdividef(1.f, 1.f + __expf(-z));
+        return p * (1.f + z * (1.f - p));
+    } else if constexpr (ACT == KQ_ACT_GELU) {
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    } else return 1.f;
 }
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
