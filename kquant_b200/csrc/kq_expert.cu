@@ -10,19 +10,24 @@
 //
 // A pair of CTAs (cta_group::2) shares one output tile, persistent, one CTA
 // per SM.  The M axis of the tensor product is the output's contiguous axis:
-// 256 features of W, 128 per CTA (gated: 64 of gate and the same 64 of up in
-// each).  The N axis is the rows, 64 to 256 of them: an expert's last tile
-// costs what its rows need, where row tiles of 128 or 256 on the M axis would
-// waste 11% or 31% of the products of an unevenly routed prompt (8192 rows, 16
-// experts).  Against one CTA per tile a pair reads half as much of B into each
-// shared memory: 64 KB move per 512 tensor cycles instead of 96 KB, which had
-// held the one-CTA form at 0.55 of the tensor peak.
+// 512 features of W in two accumulators of 256, 128 lanes of each per CTA
+// (gated: 256 of gate in one and the same 256 of up in the other).  The N axis
+// is the rows, 64 to 256 of them: an expert's last tile costs what its rows
+// need, where row tiles of 128 or 256 on the M axis would waste 11% or 31% of
+// the products of an unevenly routed prompt (8192 rows, 16 experts).  A CTA
+// moves 48 KB a stage for 1024 tensor cycles; one CTA with a 128 x 256 tile
+// moved the same for 512 and stood at 0.55 of the tensor peak, a pair with 256
+// x 256 at 0.63 (bytes into and out of shared memory, and TMA issue).
 //
 // Warp 0 of each CTA issues TMA into a ring of 64-deep stages; warp 1 of the
-// leader issues tcgen05.mma for the pair; warps 2..9 drain.  Two 256-column
-// accumulators alternate, so a tile's epilogue runs under the next tile's
-// products.  A thread drains one feature (TMEM lane), so a warp's 2-byte
-// accesses to a row are 64 consecutive bytes, whatever the row stride.
+// leader issues tcgen05.mma for the pair; warps 2..17 drain.  The accumulators
+// fill the tensor memory: the next tile's products into the first one start
+// as soon as it is drained and run ahead of the second by up to the ring's
+// stages.  Tiles of up to 128 rows take half of it, so two of them alternate.
+// A thread drains one feature (TMEM lane); 8 rows of a warp's 32 features turn
+// in shared memory and leave (and the residual or dy enters) as 16-byte
+// accesses.  With 2-byte accesses straight from the lanes, an address each,
+// the epilogue took longer than the products at k = 1536.
 // Both operands may be K-major or MN-major in shared memory: W is taken as
 // stored ([k][n] or [n][k]), and the sums product reads x and dz as they are,
 // contracting over their rows.
@@ -40,14 +45,16 @@ namespace {
 
 __device__ int g_wait_error = 0;
 
-constexpr int BK = 64, STAGES = 6;
-constexpr int TILE = 256;                       // features and rows of a pair's tile, at most
-constexpr int SIDE_BYTES = 128 * BK * 2, STAGE_BYTES = 2 * SIDE_BYTES;   // a CTA's half of A and of B
-constexpr int CHUNK = 64 * 128;                 // 64 rows of 128 bytes: one TMA box, one MN-major slab
-constexpr int DRAIN_WARPS = 8, THREADS = 64 + 32 * DRAIN_WARPS;
-constexpr int EXCHANGE_BYTES = DRAIN_WARPS * 2 * 8 * 32 * 4;
+constexpr int BK = 64, STAGES = 4;
+constexpr int TILE = 256;                       // features of an accumulator pair, rows of a tile at most
+constexpr int SIDE_BYTES = 128 * BK * 2, STAGE_BYTES = 3 * SIDE_BYTES;   // a CTA's share of A (two accumulators) and of B
+constexpr int CHUNK = 64 * 128;                 // 64 rows of 128 bytes: one MN-major slab
+constexpr int DRAIN_WARPS = 16, THREADS = 64 + 32 * DRAIN_WARPS;
+constexpr int TR = 8, STRIDE = TR * DRAIN_WARPS / 4;   // rows that a drain warp turns at a time; the warps of a quadrant alternate
 constexpr int GROUP_BYTES = (3 * kMaxExperts + 4) * 4;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EXCHANGE_BYTES + GROUP_BYTES + 1024;
+constexpr int TURN = TR * 32;
+constexpr int TURN_BYTES = DRAIN_WARPS * 2 * TURN * 2;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + TURN_BYTES + GROUP_BYTES + 1024;
 
 enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS };
 
@@ -59,14 +66,15 @@ struct Params {
     int64_t bias_stride, ld_aux, ld_out, out_stride;   // out_stride: per expert (sums)
     int rows, experts, k_steps, m_tiles, n_tiles;
     int m_out, n_out;      // output extents: features, and (sums) rows
+    int span;              // features of a tile: one accumulator's or two's (gated: of gate and of up)
     int up;                // gated: first coordinate of the up half in W
     int* err;
     uint32_t idesc;        // without N
     int act;
-    bool a_mn, b_mn, zero_rest;
+    bool a_mn, b_mn, zero_rest, vec_aux, vec_out;
 };
 
-struct Tile { int e, row0, count, m0, n0, n, k_steps; };
+struct Tile { int e, row0, count, m0, n0, n, k_steps, accs; };   // accs: accumulators with live features
 
 // Tile t of the launch; m0 in features, n the extent of the tensor product's N axis.
 template <int EPI, bool GATED>
@@ -76,7 +84,7 @@ __device__ __forceinline__ bool tile_at(const Params& p, const int* lo, const in
         if (t >= (int64_t)per * p.experts) return false;
         o.e = (int)(t / per);
         const int l = (int)(t - (int64_t)o.e * per);
-        o.m0 = (l % p.m_tiles) * TILE;
+        o.m0 = (l % p.m_tiles) * p.span;
         o.n0 = (l / p.m_tiles) * TILE;
         o.row0 = lo[o.e];
         o.count = cnt[o.e];
@@ -89,13 +97,14 @@ __device__ __forceinline__ bool tile_at(const Params& p, const int* lo, const in
         const int nt = cum[o.e + 1] - cum[o.e];
         const int64_t l = t - (int64_t)cum[o.e] * p.m_tiles;
         const int r = (int)(l % nt) * TILE;
-        o.m0 = (int)(l / nt) * (GATED ? TILE / 2 : TILE);
+        o.m0 = (int)(l / nt) * p.span;
         o.n0 = 0;
         o.row0 = lo[o.e] + r;
         o.count = min(cnt[o.e] - r, TILE);
         o.n = (o.count + 63) & ~63;
         o.k_steps = p.k_steps;
     }
+    o.accs = GATED || (p.span > TILE && p.m_out - o.m0 > TILE) ? 2 : 1;
     return true;
 }
 
@@ -112,27 +121,60 @@ __device__ __forceinline__ bool zero_tail(uint8_t* stage, int slabs, int valid, 
     return ok;
 }
 
-// W rows of one feature: pre-activations z (and up projections u) to results, the first `rows` stored.
-template <typename T, int EPI, bool GATED, int ACT, int W>
-__device__ __forceinline__ void finish(T* o, int64_t ld, int second, int rows, const float (&z)[W], const float (&u)[W],
-                                       const float (&a)[W]) {
-    T y[W], y2[W];
+// TR rows of one feature: pre-activations z (and up projections u) and a (residual or dy) to the results.
+template <int EPI, bool GATED, int ACT>
+__device__ __forceinline__ void finish(float (&z)[TR], float (&u)[TR], const float (&a)[TR]) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
+    for (int j = 0; j < TR; ++j) {
         if constexpr (EPI == EPI_FORWARD) {
-            y[j] = from_f<T>(activate<ACT>(z[j]) * (GATED ? u[j] : 1.f) + a[j]);
+            z[j] = activate<ACT>(z[j]) * (GATED ? u[j] : 1.f) + a[j];
         } else if constexpr (GATED) {
-            y[j] = from_f<T>(a[j] * u[j] * slope<ACT>(z[j]));
-            y2[j] = from_f<T>(a[j] * activate<ACT>(z[j]));
+            const float du = a[j] * activate<ACT>(z[j]);
+            z[j] = a[j] * u[j] * slope<ACT>(z[j]);
+            u[j] = du;
         } else {
-            y[j] = from_f<T>(a[j] * slope<ACT>(z[j]));
+            z[j] = a[j] * slope<ACT>(z[j]);
         }
     }
+}
+
+// TR rows x 32 features of a warp between global memory (row stride ld, 8 features a lane) and its turning buffer
+// [TR][32].  `rows` and `cols` bound what exists.
+template <typename T>
+__device__ __forceinline__ uint4 fetch_turn(const T* src, int64_t ld, int rows, int cols, bool vec, int lane) {
+    const int row = lane >> 2, col = (lane & 3) * 8;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (row < rows && col < cols) {
+        const T* p = src + row * ld + col;
+        if (vec && col + 8 <= cols) {
+            q = *reinterpret_cast<const uint4*>(p);
+        } else {
+            T* e = reinterpret_cast<T*>(&q);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-        if (j < rows) {
-            o[j * ld] = y[j];
-            if constexpr (EPI == EPI_GRAD && GATED) o[j * ld + second] = y2[j];
+            for (int k = 0; k < 8; ++k)
+                if (col + k < cols) e[k] = p[k];
+        }
+    }
+    return q;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_turn(T* turn, const float (&v)[TR], T* dst, int64_t ld, int rows, int cols, bool vec, int lane) {
+    __syncwarp();                                // the buffer's last readers are done
+#pragma unroll
+    for (int j = 0; j < TR; ++j) turn[j * 32 + lane] = from_f<T>(v[j]);
+    __syncwarp();
+    const int row = lane >> 2, col = (lane & 3) * 8;
+    if (row < rows && col < cols) {
+        const uint4 q = *reinterpret_cast<const uint4*>(turn + lane * 8);
+        T* p = dst + row * ld + col;
+        if (vec && col + 8 <= cols) {
+            *reinterpret_cast<uint4*>(p) = q;
+        } else {
+            const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (col + k < cols) p[k] = e[k];
         }
     }
 }
@@ -145,8 +187,8 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tail_bar[STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* exchange = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
-    int* lo = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + EXCHANGE_BYTES);
+    T* turns = reinterpret_cast<T*>(smem + STAGES * STAGE_BYTES);
+    int* lo = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + TURN_BYTES);
     int* cnt = lo + kMaxExperts;
     int* cum = cnt + kMaxExperts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -175,60 +217,63 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     bool ok = true;
     Tile t;
 
+    // Halves of the tensor memory (256 columns) are used in turn.  A tile with two accumulators of more than 128 rows
+    // takes two turns, any other tile one (its second accumulator at column 128).
+    auto two_turns = [](const Tile& t) { return t.accs == 2 && t.n > 128; };
+
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
             for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
                 const int half = t.n >> 1;
-                const uint32_t bytes = SIDE_BYTES + half * 128;
-                const int fa = t.m0 + rank * (GATED ? 64 : 128), fb = GATED ? p.up + fa : fa + 64;
+                const uint32_t bytes = t.accs * SIDE_BYTES + half * 128;
                 for (int ks = 0; ks < t.k_steps; ++ks, ++it) {
                     const int s = it % STAGES;
                     if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
-                    uint8_t *sa = smem + s * STAGE_BYTES, *sb = sa + SIDE_BYTES;
+                    uint8_t *sa = smem + s * STAGE_BYTES, *sb = sa + 2 * SIDE_BYTES;
                     uint32_t bar = leader_addr(&full_bar[s]);
-                    if constexpr (EPI == EPI_SUMS) {
-                        const int r = t.row0 + ks * BK;
-                        if (t.count - ks * BK < BK) {      // the tail is zeroed here before it counts as loaded
-                            bar = smem_addr(&tail_bar[s]);
-                            mbar_expect_tx(&tail_bar[s], bytes);
-                        } else if (rank == 0) {
-                            mbar_expect_tx(&full_bar[s], 2 * bytes);
+                    const int r = t.row0 + ks * BK;
+                    if (EPI == EPI_SUMS && t.count - ks * BK < BK) {   // the tail is zeroed here before it counts as loaded
+                        bar = smem_addr(&tail_bar[s]);
+                        mbar_expect_tx(&tail_bar[s], bytes);
+                    } else if (rank == 0) {
+                        mbar_expect_tx(&full_bar[s], 2 * bytes);
+                    }
+                    for (int a = 0; a < t.accs; ++a) {
+                        const int f = t.m0 + rank * 128 + (a ? (GATED ? p.up : TILE) : 0);
+                        uint8_t* dst = sa + a * SIDE_BYTES;
+                        if constexpr (EPI == EPI_SUMS) {
+                            tma2_load_2d(dst, &map_a, f, r, bar);
+                            tma2_load_2d(dst + CHUNK, &map_a, f + 64, r, bar);
+                        } else if (p.a_mn) {
+                            tma2_load_3d(dst, &map_a, f, ks * BK, t.e, bar);
+                            tma2_load_3d(dst + CHUNK, &map_a, f + 64, ks * BK, t.e, bar);
+                        } else {
+                            tma2_load_3d(dst, &map_a, ks * BK, f, t.e, bar);
                         }
-                        tma2_load_2d(sa, &map_a, fa, r, bar);
-                        tma2_load_2d(sa + CHUNK, &map_a, fb, r, bar);
+                    }
+                    if constexpr (EPI == EPI_SUMS) {
                         for (int c = 0; c < half; c += 64)
                             tma2_load_2d(sb + (c >> 6) * CHUNK, &map_b, t.n0 + rank * half + c, r, bar);
+                    } else if (half == 128) {
+                        tma2_load_2d(sb, &map_b_full, ks * BK, t.row0 + rank * half, bar);
                     } else {
-                        if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * bytes);
-                        if (p.a_mn) {
-                            tma2_load_3d(sa, &map_a, fa, ks * BK, t.e, bar);
-                            tma2_load_3d(sa + CHUNK, &map_a, fb, ks * BK, t.e, bar);
-                        } else {
-                            tma2_load_3d(sa, &map_a, ks * BK, fa, t.e, bar);
-                            if (GATED) tma2_load_3d(sa + CHUNK, &map_a, ks * BK, fb, t.e, bar);
-                        }
-                        if (half == 128) {
-                            tma2_load_2d(sb, &map_b_full, ks * BK, t.row0 + rank * half, bar);
-                        } else {
-                            for (int c = 0; c < half; c += 32)
-                                tma2_load_2d(sb + c * 128, &map_b, ks * BK, t.row0 + rank * half + c, bar);
-                        }
+                        for (int c = 0; c < half; c += 32)
+                            tma2_load_2d(sb + c * 128, &map_b, ks * BK, t.row0 + rank * half + c, bar);
                     }
                 }
             }
             if (!ok) report_wait_error(p.err);
         }
     } else if (warp == 1) {
-        uint32_t it = 0, tile_no = 0, tails = 0;   // tails: the phase of every stage's tail_bar
+        uint32_t it = 0, turn = 0, tails = 0;   // tails: the phase of every stage's tail_bar
         const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;   // 16 contraction values, in 16-byte units
-        for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step, ++tile_no) {
-            const int b = tile_no & 1;
-            const int tail_step = EPI == EPI_SUMS && t.count % BK ? t.k_steps - 1 : -1;
-            const int slabs = 2 + (t.n >> 7);
+        for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
+            const int tail_step = EPI == EPI_SUMS && (t.count % BK) != 0 ? t.k_steps - 1 : -1;
+            const int slabs = 4 + (t.n >> 7);
             if (rank != 0) {                    // the leader issues for both; this CTA zeroes its own tails
                 if (tail_step >= 0) {
-                    const int s = (it + tail_step) % STAGES;
+                    const int s = (it + (uint32_t)tail_step) % STAGES;
                     ok = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane);
                     if (lane == 0) mbar_arrive_remote(leader_addr(&full_bar[s]));
                     tails ^= 1u << s;
@@ -236,114 +281,158 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 it += t.k_steps;
                 continue;
             }
-            if (!(ok = mbar_wait_cluster(&acc_empty[b], ((tile_no >> 1) & 1) ^ 1))) break;
-            tc_fence_after();
+            const bool two = two_turns(t);
+            const int h0 = turn & 1, h1 = (turn + 1) & 1;
+            const uint32_t col[2] = {tmem + h0 * TILE, two ? tmem + h1 * TILE : tmem + h0 * TILE + 128};
             const uint32_t idesc = p.idesc | ((uint32_t)(t.n >> 3) << 17);
-            for (int ks = 0; ks < t.k_steps; ++ks, ++it) {
-                const int s = it % STAGES;
-                if (ks == tail_step) {          // the only arrival on full_bar is the other CTA's, for its zeroed half
-                    ok = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane) &&
-                         mbar_wait_cluster(&full_bar[s], (it / STAGES) & 1);
-                    tails ^= 1u << s;
-                }
-                if (!(ok = ok && mbar_wait(&full_bar[s], (it / STAGES) & 1))) break;
-                tc_fence_after();
+            auto products = [&](int a, int ks) {
+                const int s = (it + ks) % STAGES;
                 if (lane == 0) {
-                    const uint32_t a = smem_addr(smem + s * STAGE_BYTES);
-                    const uint64_t ad = smem_desc(a, p.a_mn ? CHUNK : 16), bd = smem_desc(a + SIDE_BYTES, p.b_mn ? CHUNK : 16);
+                    const uint32_t base = smem_addr(smem + s * STAGE_BYTES);
+                    const uint64_t ad = smem_desc(base + a * SIDE_BYTES, p.a_mn ? CHUNK : 16);
+                    const uint64_t bd = smem_desc(base + 2 * SIDE_BYTES, p.b_mn ? CHUNK : 16);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk)
-                        mma2_f16(tmem + b * TILE, ad + a_step * kk, bd + b_step * kk, idesc, (ks | kk) != 0);
-                    mma2_commit(&empty_bar[s]);
+                        mma2_f16(col[a], ad + a_step * kk, bd + b_step * kk, idesc, (ks | kk) != 0);
+                    if (a == t.accs - 1) mma2_commit(&empty_bar[s]);
                 }
                 __syncwarp();
+            };
+            auto loaded = [&](int ks) {
+                const int s = (it + ks) % STAGES;
+                const uint32_t parity = ((it + ks) / STAGES) & 1;
+                bool got = true;
+                if (ks == tail_step) {          // the only arrival on full_bar is the other CTA's, for its zeroed half
+                    got = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane) &&
+                          mbar_wait_cluster(&full_bar[s], parity);
+                    tails ^= 1u << s;
+                }
+                got = got && mbar_wait(&full_bar[s], parity);
+                tc_fence_after();
+                return got;
+            };
+            if (!(ok = mbar_wait_cluster(&acc_empty[h0], ((turn >> 1) & 1) ^ 1))) break;
+            tc_fence_after();
+            int done0 = 0;                      // k steps issued into the first accumulator
+            if (two) {
+                // Until the second accumulator is drained, the first goes ahead through the stages in the ring.
+                const uint32_t parity = (((turn + 1) >> 1) & 1) ^ 1;
+                const int ahead = min(t.k_steps, STAGES);
+                while (done0 < ahead && ok && !__shfl_sync(0xFFFFFFFFu, (int)mbar_test(&acc_empty[h1], parity), 0)) {
+                    if ((ok = loaded(done0))) products(0, done0++);
+                }
+                if (!(ok = ok && mbar_wait_cluster(&acc_empty[h1], parity))) break;
+                tc_fence_after();
             }
-            if (ok && lane == 0) mma2_commit(&acc_full[b]);
+            for (int ks = 0; ks < t.k_steps; ++ks) {
+                if (ks == done0) {
+                    if (!(ok = loaded(ks))) break;
+                    products(0, ks);
+                    ++done0;
+                }
+                if (two && ks == t.k_steps - 1 && lane == 0) mma2_commit(&acc_full[h0]);
+                if (t.accs == 2) products(1, ks);
+            }
+            if (ok && lane == 0) {
+                if (two && t.k_steps == 0) mma2_commit(&acc_full[h0]);
+                mma2_commit(&acc_full[two ? h1 : h0]);
+            }
             __syncwarp();
+            it += t.k_steps;
+            turn += two ? 2 : 1;
         }
         if (!ok && lane == 0) report_wait_error(p.err);
     } else {
-        const int q = warp & 3, h = (warp - 2) >> 2;    // tensor-memory lanes 32q.., every other 16 columns
-        uint32_t tile_no = 0, turn = 0;
-        for (int64_t i = first; tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step, ++tile_no) {
-            const int b = tile_no & 1;
-            if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[b], (tile_no >> 1) & 1)))) break;
+        const int q = warp & 3, h = (warp - 2) >> 2;    // tensor-memory lanes 32q.., TR of every STRIDE columns
+        T *turn_in = turns + (warp - 2) * 2 * TURN, *turn_out = turn_in + TURN;
+        uint32_t turn = 0;
+        for (int64_t i = first; tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
+            const bool two = two_turns(t);
+            const int h0 = turn & 1, h1 = (turn + 1) & 1;
+            const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+            const uint32_t col[2] = {lanes + h0 * TILE, two ? lanes + h1 * TILE : lanes + h0 * TILE + 128};
+            ok = mbar_wait(&acc_full[h0], (turn >> 1) & 1);
+            if (GATED && two) ok = ok && mbar_wait(&acc_full[h1], ((turn + 1) >> 1) & 1);
+            if (!(ok = __all_sync(0xFFFFFFFFu, ok))) break;
             tc_fence_after();
-            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * TILE);
-            const int f = t.m0 + (GATED ? rank * 64 + (q & 1) * 32 : rank * 128 + q * 32) + lane;
-            const bool live = f < p.m_out;
-            if constexpr (EPI == EPI_SUMS) {
-                T* out = static_cast<T*>(p.out) + t.e * p.out_stride + f;
-                const int cols = min(p.n_out - t.n0, TILE);
-#pragma unroll 1
-                for (int c = h * 16; c < cols; c += 32) {
-                    uint32_t v[16];
-                    tmem_ld16(base + c, v);
-                    tmem_wait_ld();
-                    T* o = out + (int64_t)(t.n0 + c) * p.ld_out;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (live && c + j < cols) o[j * p.ld_out] = from_f<T>(t.k_steps ? __uint_as_float(v[j]) : 0.f);
+            for (int a = 0; a < (GATED ? 1 : t.accs); ++a) {
+                if (a == 1 && two) {                    // the first accumulator is free before the second is looked at
+                    tc_fence_before();
                     __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(leader_addr(&acc_empty[h0]));
+                    if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[h1], ((turn + 1) >> 1) & 1)))) break;
+                    tc_fence_after();
                 }
-            } else {
-                const T* bias = static_cast<const T*>(p.bias) + t.e * p.bias_stride;
-                const bool up = GATED && q >= 2;        // this warp's lanes hold up, not gate
-                const float add = p.bias && live ? to_f<T>(bias[(up ? p.m_out : 0) + f]) : 0.f;
-                T* out = static_cast<T*>(p.out) + (int64_t)t.row0 * p.ld_out + f;
-                // Loads take rows and features clamped into the tile, so that none of them hangs on a branch.
-                const T* aux = p.aux ? static_cast<const T*>(p.aux) + (int64_t)t.row0 * p.ld_aux + min(f, p.m_out - 1) : nullptr;
-                const int last = t.count - 1;
-                constexpr int W = GATED ? 8 : 16;       // rows that a thread finishes of each 16
-                T next[W];
-                auto fetch = [&](int c) {
-                    const int r0 = c + (up ? 8 : 0);
-#pragma unroll
-                    for (int j = 0; j < W; ++j) next[j] = aux[(int64_t)min(r0 + j, last) * p.ld_aux];
-                };
-                if (aux && h * 16 < t.count) fetch(h * 16);
-#pragma unroll 1
-                for (int c = h * 16; c < t.count; c += 32) {
-                    uint32_t v[16];
-                    tmem_ld16(base + c, v);
-                    float a[W], z[W], u[W];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) a[j] = aux ? to_f<T>(next[j]) : 0.f;
-                    if (aux && c + 32 < t.count) fetch(c + 32);       // under this chunk's arithmetic
+                const uint32_t base = col[a];
+                const int f0 = t.m0 + a * TILE + rank * 128 + q * 32, cols = p.m_out - f0;   // this warp's features
+                if (cols <= 0) continue;
+                const int n = EPI == EPI_SUMS ? min(p.n_out - t.n0, TILE) : t.count;         // rows of the output
+                T* out;
+                const T* aux = nullptr;
+                float add = 0.f, add_up = 0.f;
+                if constexpr (EPI == EPI_SUMS) {
+                    out = static_cast<T*>(p.out) + t.e * p.out_stride + (int64_t)t.n0 * p.ld_out + f0;
+                } else {
+                    out = static_cast<T*>(p.out) + (int64_t)t.row0 * p.ld_out + f0;
+                    if (p.aux) aux = static_cast<const T*>(p.aux) + (int64_t)t.row0 * p.ld_aux + f0;
+                    if (p.bias && lane < cols) {
+                        const T* bias = static_cast<const T*>(p.bias) + t.e * p.bias_stride + f0 + lane;
+                        add = to_f<T>(bias[0]);
+                        if constexpr (GATED) add_up = to_f<T>(bias[p.m_out]);
+                    }
+                }
+                const int begin = h * TR;
+                uint4 ahead = make_uint4(0, 0, 0, 0);
+                if (aux) ahead = fetch_turn(aux + (int64_t)begin * p.ld_aux, p.ld_aux, n - begin, cols, p.vec_aux, lane);
+                uint32_t v[TR], w[TR];
+                if (begin < n) {
+                    tmem_ld8(base + begin, v);
+                    if constexpr (GATED) tmem_ld8(col[1] + begin, w);
                     tmem_wait_ld();
-                    if constexpr (GATED) {
-                        // Gate and up of a feature lie in two warps: each sends the other 8 of its 16 rows.
-                        float* mine = exchange + ((warp - 2) * 2 + (turn & 1)) * 256;
-                        const float* theirs = exchange + (((warp - 2) ^ 2) * 2 + (turn & 1)) * 256;
+                }
+#pragma unroll 1
+                for (int c = begin; c < n; c += STRIDE) {
+                    float z[TR], u[TR], x[TR];
+                    if (aux) {
+                        __syncwarp();
+                        *reinterpret_cast<uint4*>(turn_in + lane * 8) = ahead;
+                        if (c + STRIDE < n)
+                            ahead = fetch_turn(aux + (int64_t)(c + STRIDE) * p.ld_aux, p.ld_aux, n - c - STRIDE, cols, p.vec_aux, lane);
+                        __syncwarp();
+                    }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) mine[j * 32 + lane] = __uint_as_float(up ? v[j] : v[8 + j]) + add;
-                        asm volatile("bar.sync %0, 64;" ::"r"(1 + h * 2 + (q & 1)) : "memory");
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float own_v = __uint_as_float(up ? v[8 + j] : v[j]) + add, other = theirs[j * 32 + lane];
-                            z[j] = up ? other : own_v;
-                            u[j] = up ? own_v : other;
+                    for (int j = 0; j < TR; ++j) {
+                        x[j] = aux ? to_f<T>(turn_in[j * 32 + lane]) : 0.f;
+                        z[j] = __uint_as_float(v[j]) + add;
+                        if constexpr (GATED) u[j] = __uint_as_float(w[j]) + add_up;
+                        if (EPI == EPI_SUMS && t.k_steps == 0) z[j] = 0.f;
+                    }
+                    if (c + STRIDE < n) {               // the next rows, under this chunk's arithmetic
+                        tmem_ld8(base + c + STRIDE, v);
+                        if constexpr (GATED) tmem_ld8(col[1] + c + STRIDE, w);
+                    }
+                    if constexpr (EPI != EPI_SUMS) {
+                        switch (p.act) {
+                            case KQ_ACT_RELU: finish<EPI, GATED, KQ_ACT_RELU>(z, u, x); break;
+                            case KQ_ACT_SILU: finish<EPI, GATED, KQ_ACT_SILU>(z, u, x); break;
+                            case KQ_ACT_GELU: finish<EPI, GATED, KQ_ACT_GELU>(z, u, x); break;
+                            default: finish<EPI, GATED, KQ_ACT_NONE>(z, u, x);
                         }
-                        ++turn;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < W; ++j) z[j] = __uint_as_float(v[j]) + add;
                     }
-                    const int r0 = c + (up ? 8 : 0);
-                    T* o = out + (int64_t)r0 * p.ld_out;
-                    const int rows = live ? min(t.count - r0, W) : 0;
-                    switch (p.act) {
-                        case KQ_ACT_RELU: finish<T, EPI, GATED, KQ_ACT_RELU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
-                        case KQ_ACT_SILU: finish<T, EPI, GATED, KQ_ACT_SILU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
-                        case KQ_ACT_GELU: finish<T, EPI, GATED, KQ_ACT_GELU, W>(o, p.ld_out, p.m_out, rows, z, u, a); break;
-                        default: finish<T, EPI, GATED, KQ_ACT_NONE, W>(o, p.ld_out, p.m_out, rows, z, u, a);
-                    }
-                    __syncwarp();
+                    store_turn(turn_out, z, out + (int64_t)c * p.ld_out, p.ld_out, n - c, cols, p.vec_out, lane);
+                    if constexpr (EPI == EPI_GRAD && GATED)
+                        store_turn(turn_out, u, out + (int64_t)c * p.ld_out + p.m_out, p.ld_out, n - c, cols, p.vec_out, lane);
+                    tmem_wait_ld();
                 }
             }
+            if (!ok) break;
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(leader_addr(&acc_empty[b]));
+            if (lane == 0) {
+                mbar_arrive_remote(leader_addr(&acc_empty[two ? h1 : h0]));
+                if (GATED && two) mbar_arrive_remote(leader_addr(&acc_empty[h0]));
+            }
+            turn += two ? 2 : 1;
         }
         if (!ok && lane == 0) report_wait_error(p.err);
         // Rows of no expert: zero in a fresh output, untouched otherwise.
@@ -403,25 +492,6 @@ bias_grad_kernel(const T* __restrict__ dz, int64_t ld, const int64_t* __restrict
     }
 }
 
-int64_t round8(int64_t v) { return (v + 7) & ~(int64_t)7; }
-
-// A 16-bit operand of `batch` matrices of `r` rows and `c` contiguous columns,
-// as it is or laid out again in the workspace.
-struct Operand {
-    const uint16_t* base;
-    int64_t batch, r, c, sb, sr;
-    bool direct;
-};
-
-Operand operand(const void* base, int64_t batch, int64_t r, int64_t c, int64_t sb, int64_t sr) {
-    Operand o{static_cast<const uint16_t*>(base), batch, r, c, sb, sr, true};
-    if (r == 1) o.sr = round8(c);
-    if (batch == 1) o.sb = round8(o.sr * r);
-    o.direct = ((uintptr_t)base & 15) == 0 && o.sr % 8 == 0 && o.sb % 8 == 0 && o.sr >= c && o.sb >= (batch > 1 ? o.sr : 0) &&
-               o.sr < ((int64_t)1 << 38) && o.sb < ((int64_t)1 << 38);
-    return o;
-}
-
 size_t relayout_bytes(const Operand& o) {
     return o.direct ? 0 : (size_t)(o.batch * o.r * round8(o.c)) * 2;
 }
@@ -446,18 +516,8 @@ int relayout(Operand& o, uint16_t*& ws, int halves, cudaStream_t s) {
     return KQ_OK;
 }
 
-int map_rows(CUtensorMap* m, const Operand& o, bool bf16, int box_c, int box_r, const char* what) {
-    const int64_t dims[3] = {o.c, o.r, o.batch}, strides[2] = {o.sr * 2, o.sb * 2};
-    const int box[3] = {box_c, box_r, 1};
-    return encode_tiles(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, o.base, dims,
-                        strides, box, what);
-}
-
-int map_rows_2d(CUtensorMap* m, const Operand& o, bool bf16, int box_c, int box_r, const char* what) {
-    const int64_t dims[2] = {o.c, o.r}, strides[1] = {o.sr * 2};
-    const int box[2] = {box_c, box_r};
-    return encode_tiles(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, o.base, dims,
-                        strides, box, what);
+bool vec8(const void* base, int64_t ld, int64_t ld2 = 0) {
+    return ((uintptr_t)base & 15) == 0 && ld % 8 == 0 && ld2 % 8 == 0;
 }
 
 // Pairs of CTAs that run at once (every instance needs a whole SM); asked once for each device.
@@ -560,6 +620,51 @@ size_t product_workspace(const kq_expert_product& p) {
     return n ? n + 64 : 0;                      // each part is rounded up to 16 bytes
 }
 
+// Two accumulators a tile where that leaves at least three tiles for every pair: fewer would stand idle, which costs
+// more than what the shared B tile saves (256 rows, 8192 -> 18944: 94 us with one accumulator, 145 us with two).
+int span_for(int64_t features, int64_t other_tiles, bool gated, int* span) {
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    *span = !gated && (features + 2 * TILE - 1) / (2 * TILE) * other_tiles >= 3 * (sms / 2) ? 2 * TILE : TILE;
+    return KQ_OK;
+}
+
+int many_rows_product(const RowsProduct& p, cudaStream_t s) {
+    CUtensorMap ma, mb, mf;
+    // Large boxes where the tile takes them whole: every TMA instruction of a stage costs issue time.
+    if (int rc = map_rows(&ma, p.w, p.bf16, 64, p.mn ? 64 : 128, p.what)) return rc;
+    if (int rc = map_rows_2d(&mb, p.x, p.bf16, BK, 32, p.what)) return rc;
+    if (int rc = map_rows_2d(&mf, p.x, p.bf16, BK, 128, p.what)) return rc;
+    Params q{};
+    if (int rc = wait_error_word(&q.err)) return rc;
+    q.offsets = p.offsets;
+    q.bias = p.bias;
+    q.aux = p.aux;
+    q.out = p.out;
+    q.bias_stride = p.bias_stride;
+    q.ld_aux = p.ld_aux;
+    q.ld_out = p.ld_out;
+    q.rows = (int)p.rows;
+    q.experts = (int)p.experts;
+    q.k_steps = (int)((p.k + BK - 1) / BK);
+    const int64_t r_tiles = (p.rows + TILE - 1) / TILE + (p.experts < p.rows ? p.experts : p.rows) - 1;
+    if (int rc = span_for(p.n_out, r_tiles, p.gated, &q.span)) return rc;
+    q.m_tiles = (int)((p.n_out + q.span - 1) / q.span);
+    q.m_out = (int)p.n_out;
+    q.up = p.up;
+    q.idesc = idesc_f16(p.bf16, p.mn, false, TILE, 0);
+    q.act = p.act;
+    q.a_mn = p.mn;
+    q.zero_rest = p.zero_rest;
+    q.vec_aux = vec8(p.aux, p.ld_aux);
+    q.vec_out = vec8(p.out, p.ld_out, p.grad && p.gated ? p.n_out : 0);
+    const int64_t tiles = r_tiles * q.m_tiles;
+    if (p.grad)
+        return p.gated ? launch<EPI_GRAD, true>(p.bf16, ma, mb, mf, q, tiles, s) : launch<EPI_GRAD, false>(p.bf16, ma, mb, mf, q, tiles, s);
+    return p.gated ? launch<EPI_FORWARD, true>(p.bf16, ma, mb, mf, q, tiles, s)
+                   : launch<EPI_FORWARD, false>(p.bf16, ma, mb, mf, q, tiles, s);
+}
+
 int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void* workspace, size_t workspace_bytes,
                  cudaStream_t s, const char* what) {
     if (int rc = check_product(p, what)) return rc;
@@ -577,34 +682,29 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     const bool gated_copy = mn && p.gated && !w.direct;
     if (int rc = relayout(x, ws, 1, s)) return rc;
     if (int rc = relayout(w, ws, gated_copy ? 2 : 1, s)) return rc;
-    CUtensorMap ma, mb, mf;
-    // Large boxes where the tile takes them whole: every TMA instruction of a stage costs issue time.
-    if (int rc = map_rows(&ma, w, bf16, 64, mn || p.gated ? 64 : 128, what)) return rc;
-    if (int rc = map_rows_2d(&mb, x, bf16, BK, 32, what)) return rc;
-    if (int rc = map_rows_2d(&mf, x, bf16, BK, 128, what)) return rc;
-    Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
-    q.offsets = p.offsets;
-    q.bias = p.bias;
-    q.aux = grad ? dy : p.residual;
-    q.out = p.y;
-    q.bias_stride = p.bias_stride_e;
-    q.ld_aux = grad ? ld_dy : p.ld_residual;
-    q.ld_out = p.ldy;
-    q.rows = (int)p.rows;
-    q.experts = (int)p.experts;
-    q.k_steps = (int)((p.k + BK - 1) / BK);
-    const int width = p.gated ? TILE / 2 : TILE;
-    q.m_tiles = (int)((n_out + width - 1) / width);
-    q.m_out = (int)n_out;
-    q.up = (int)(gated_copy ? round8(n_out) : n_out);
-    q.idesc = idesc_f16(bf16, mn, false, TILE, 0);
-    q.act = p.activation;
-    q.a_mn = mn;
-    q.zero_rest = p.zero_rest != 0;
-    const int64_t tiles = ((p.rows + TILE - 1) / TILE + (p.experts < p.rows ? p.experts : p.rows)) * q.m_tiles;
-    if (grad) return p.gated ? launch<EPI_GRAD, true>(bf16, ma, mb, mf, q, tiles, s) : launch<EPI_GRAD, false>(bf16, ma, mb, mf, q, tiles, s);
-    return p.gated ? launch<EPI_FORWARD, true>(bf16, ma, mb, mf, q, tiles, s) : launch<EPI_FORWARD, false>(bf16, ma, mb, mf, q, tiles, s);
+    RowsProduct r{};
+    r.x = x;
+    r.w = w;
+    r.offsets = p.offsets;
+    r.bias = p.bias;
+    r.aux = grad ? dy : p.residual;
+    r.out = p.y;
+    r.bias_stride = p.bias_stride_e;
+    r.ld_aux = grad ? ld_dy : p.ld_residual;
+    r.ld_out = p.ldy;
+    r.rows = p.rows;
+    r.k = p.k;
+    r.n_out = n_out;
+    r.experts = p.experts;
+    r.up = (int)(gated_copy ? round8(n_out) : n_out);
+    r.act = p.activation;
+    r.bf16 = bf16;
+    r.mn = mn;
+    r.gated = p.gated != 0;
+    r.grad = grad;
+    r.zero_rest = p.zero_rest != 0;
+    r.what = what;
+    return few_rows(r) ? few_rows_product(r, s) : many_rows_product(r, s);
 }
 
 __global__ void take_errors_kernel(int* out) { *out = atomicExch(&g_wait_error, 0); }
@@ -704,12 +804,14 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     q.out_stride = p.w_stride_e;
     q.rows = (int)p.rows;
     q.experts = (int)p.experts;
-    q.m_tiles = (int)((cols + TILE - 1) / TILE);
     q.n_tiles = (int)((lines + TILE - 1) / TILE);
+    if (int rc = span_for(cols, (int64_t)q.n_tiles * p.experts, false, &q.span)) return rc;
+    q.m_tiles = (int)((cols + q.span - 1) / q.span);
     q.m_out = (int)cols;
     q.n_out = (int)lines;
     q.idesc = idesc_f16(bf16, true, true, TILE, 0);
     q.a_mn = q.b_mn = true;
+    q.vec_out = vec8(dw, ld, p.experts > 1 ? p.w_stride_e : 0);
     if ((int64_t)q.m_tiles * q.n_tiles > 0x7FFFFFFF) { set_error("%s: problem too large", what); return KQ_ERR_ARG; }
     return launch<EPI_SUMS, false>(bf16, ma, mb, mb, q, (int64_t)q.m_tiles * q.n_tiles * p.experts, s);
 }
