@@ -24,10 +24,10 @@
 // fill the tensor memory: the next tile's products into the first one start
 // as soon as it is drained and run ahead of the second by up to the ring's
 // stages.  Tiles of up to 128 rows take half of it, so two of them alternate.
-// A thread drains one feature (TMEM lane); 8 rows of a warp's 32 features turn
-// in shared memory and leave (and the residual or dy enters) as 16-byte
-// accesses.  With 2-byte accesses straight from the lanes, an address each,
-// the epilogue took longer than the products at k = 1536.
+// A thread drains one feature (TMEM lane): a warp's 2-byte access to a row is
+// 64 consecutive bytes, whatever the row stride.  (Turning 8 rows in shared
+// memory for 16-byte accesses takes twice the shared-memory cycles, of which
+// the products leave 15%: 8% slower.)
 // Both operands may be K-major or MN-major in shared memory: W is taken as
 // stored ([k][n] or [n][k]), and the sums product reads x and dz as they are,
 // contracting over their rows.
@@ -45,16 +45,15 @@ namespace {
 
 __device__ int g_wait_error = 0;
 
-constexpr int BK = 64, STAGES = 4;
+constexpr int BK = 64, MAX_STAGES = 6;
 constexpr int TILE = 256;                       // features of an accumulator pair, rows of a tile at most
-constexpr int SIDE_BYTES = 128 * BK * 2, STAGE_BYTES = 3 * SIDE_BYTES;   // a CTA's share of A (two accumulators) and of B
+constexpr int SIDE_BYTES = 128 * BK * 2;        // a CTA's share of one accumulator's A, or of B
+constexpr int RING_BYTES = 12 * SIDE_BYTES;     // 4 stages with two accumulators' A, or 6 with one
 constexpr int CHUNK = 64 * 128;                 // 64 rows of 128 bytes: one MN-major slab
 constexpr int DRAIN_WARPS = 16, THREADS = 64 + 32 * DRAIN_WARPS;
-constexpr int TR = 8, STRIDE = TR * DRAIN_WARPS / 4;   // rows that a drain warp turns at a time; the warps of a quadrant alternate
+constexpr int TR = 8, STRIDE = TR * DRAIN_WARPS / 4;   // rows that a drain warp takes at a time; the warps of a quadrant alternate
 constexpr int GROUP_BYTES = (3 * kMaxExperts + 4) * 4;
-constexpr int TURN = TR * 32;
-constexpr int TURN_BYTES = DRAIN_WARPS * 2 * TURN * 2;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + TURN_BYTES + GROUP_BYTES + 1024;
+constexpr int SMEM_BYTES = RING_BYTES + GROUP_BYTES + 1024;
 
 enum { EPI_FORWARD, EPI_GRAD, EPI_SUMS };
 
@@ -71,7 +70,7 @@ struct Params {
     int* err;
     uint32_t idesc;        // without N
     int act;
-    bool a_mn, b_mn, zero_rest, vec_aux, vec_out;
+    bool a_mn, b_mn, zero_rest;
 };
 
 struct Tile { int e, row0, count, m0, n0, n, k_steps, accs; };   // accs: accumulators with live features
@@ -108,6 +107,19 @@ __device__ __forceinline__ bool tile_at(const Params& p, const int* lo, const in
     return true;
 }
 
+// Position in a ring of stages.
+struct Ring {
+    uint32_t s = 0, phase = 0;
+    __device__ __forceinline__ void next(uint32_t stages) {
+        if (++s == stages) { s = 0; phase ^= 1; }
+    }
+    __device__ __forceinline__ void skip(uint32_t n, uint32_t stages) {
+        s += n;
+        phase ^= (s / stages) & 1;
+        s %= stages;
+    }
+};
+
 // Zeroes rows valid .. 63 of a sums stage in this CTA once its loads have landed.  Whole warp.
 __device__ __forceinline__ bool zero_tail(uint8_t* stage, int slabs, int valid, uint64_t* tail_bar, uint32_t parity, int lane) {
     const bool ok = mbar_wait(tail_bar, parity);
@@ -138,44 +150,22 @@ __device__ __forceinline__ void finish(float (&z)[TR], float (&u)[TR], const flo
     }
 }
 
-// TR rows x 32 features of a warp between global memory (row stride ld, 8 features a lane) and its turning buffer
-// [TR][32].  `rows` and `cols` bound what exists.
+// TR rows of one feature, row stride ld: a warp's access to a row is 64 consecutive bytes.
 template <typename T>
-__device__ __forceinline__ uint4 fetch_turn(const T* src, int64_t ld, int rows, int cols, bool vec, int lane) {
-    const int row = lane >> 2, col = (lane & 3) * 8;
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (row < rows && col < cols) {
-        const T* p = src + row * ld + col;
-        if (vec && col + 8 <= cols) {
-            q = *reinterpret_cast<const uint4*>(p);
-        } else {
-            T* e = reinterpret_cast<T*>(&q);
+__device__ __forceinline__ void fetch_rows(T (&v)[TR], const T* src, int64_t ld, int rows) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (col + k < cols) e[k] = p[k];
-        }
+    for (int j = 0; j < TR; ++j) {
+        v[j] = src[0];
+        src += j + 1 < rows ? ld : 0;            // the last row again behind the end: no branch around a load
     }
-    return q;
 }
 
 template <typename T>
-__device__ __forceinline__ void store_turn(T* turn, const float (&v)[TR], T* dst, int64_t ld, int rows, int cols, bool vec, int lane) {
-    __syncwarp();                                // the buffer's last readers are done
+__device__ __forceinline__ void store_rows(T* dst, int64_t ld, int rows, const float (&v)[TR]) {
 #pragma unroll
-    for (int j = 0; j < TR; ++j) turn[j * 32 + lane] = from_f<T>(v[j]);
-    __syncwarp();
-    const int row = lane >> 2, col = (lane & 3) * 8;
-    if (row < rows && col < cols) {
-        const uint4 q = *reinterpret_cast<const uint4*>(turn + lane * 8);
-        T* p = dst + row * ld + col;
-        if (vec && col + 8 <= cols) {
-            *reinterpret_cast<uint4*>(p) = q;
-        } else {
-            const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (col + k < cols) p[k] = e[k];
-        }
+    for (int j = 0; j < TR; ++j) {
+        if (j < rows) dst[0] = from_f<T>(v[j]);
+        dst += ld;
     }
 }
 
@@ -184,19 +174,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
               const __grid_constant__ CUtensorMap map_b_full, const Params p) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tail_bar[STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], tail_bar[MAX_STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    T* turns = reinterpret_cast<T*>(smem + STAGES * STAGE_BYTES);
-    int* lo = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + TURN_BYTES);
+    int* lo = reinterpret_cast<int*>(smem + RING_BYTES);
     int* cnt = lo + kMaxExperts;
     int* cum = cnt + kMaxExperts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int a_parts = GATED || p.span > TILE ? 2 : 1;      // accumulators a stage has room for
+    const uint32_t stages = 12 / (a_parts + 1), stage_bytes = (a_parts + 1) * SIDE_BYTES, b_at = a_parts * SIDE_BYTES;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < MAX_STAGES; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
             mbar_init(&tail_bar[s], 1);
@@ -223,14 +214,14 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;
+            Ring ring;
             for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
                 const int half = t.n >> 1;
                 const uint32_t bytes = t.accs * SIDE_BYTES + half * 128;
-                for (int ks = 0; ks < t.k_steps; ++ks, ++it) {
-                    const int s = it % STAGES;
-                    if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
-                    uint8_t *sa = smem + s * STAGE_BYTES, *sb = sa + 2 * SIDE_BYTES;
+                for (int ks = 0; ks < t.k_steps; ++ks, ring.next(stages)) {
+                    const uint32_t s = ring.s;
+                    if (!(ok = mbar_wait(&empty_bar[s], ring.phase ^ 1))) break;
+                    uint8_t *sa = smem + s * stage_bytes, *sb = sa + b_at;
                     uint32_t bar = leader_addr(&full_bar[s]);
                     const int r = t.row0 + ks * BK;
                     if (EPI == EPI_SUMS && t.count - ks * BK < BK) {   // the tail is zeroed here before it counts as loaded
@@ -266,31 +257,31 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (!ok) report_wait_error(p.err);
         }
     } else if (warp == 1) {
-        uint32_t it = 0, turn = 0, tails = 0;   // tails: the phase of every stage's tail_bar
+        Ring at;                                // the stage of the next products into the tile's last accumulator
+        uint32_t turn = 0, tails = 0;           // tails: the phase of every stage's tail_bar
         const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;   // 16 contraction values, in 16-byte units
         for (int64_t i = first; ok && tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
             const int tail_step = EPI == EPI_SUMS && (t.count % BK) != 0 ? t.k_steps - 1 : -1;
-            const int slabs = 4 + (t.n >> 7);
+            const int slabs = b_at / CHUNK + (t.n >> 7);
             if (rank != 0) {                    // the leader issues for both; this CTA zeroes its own tails
+                at.skip(t.k_steps, stages);
                 if (tail_step >= 0) {
-                    const int s = (it + (uint32_t)tail_step) % STAGES;
-                    ok = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane);
+                    const uint32_t s = at.s ? at.s - 1 : stages - 1;
+                    ok = zero_tail(smem + s * stage_bytes, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane);
                     if (lane == 0) mbar_arrive_remote(leader_addr(&full_bar[s]));
                     tails ^= 1u << s;
                 }
-                it += t.k_steps;
                 continue;
             }
             const bool two = two_turns(t);
             const int h0 = turn & 1, h1 = (turn + 1) & 1;
             const uint32_t col[2] = {tmem + h0 * TILE, two ? tmem + h1 * TILE : tmem + h0 * TILE + 128};
             const uint32_t idesc = p.idesc | ((uint32_t)(t.n >> 3) << 17);
-            auto products = [&](int a, int ks) {
-                const int s = (it + ks) % STAGES;
+            auto products = [&](int a, int ks, uint32_t s) {
                 if (lane == 0) {
-                    const uint32_t base = smem_addr(smem + s * STAGE_BYTES);
+                    const uint32_t base = smem_addr(smem + s * stage_bytes);
                     const uint64_t ad = smem_desc(base + a * SIDE_BYTES, p.a_mn ? CHUNK : 16);
-                    const uint64_t bd = smem_desc(base + 2 * SIDE_BYTES, p.b_mn ? CHUNK : 16);
+                    const uint64_t bd = smem_desc(base + b_at, p.b_mn ? CHUNK : 16);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk)
                         mma2_f16(col[a], ad + a_step * kk, bd + b_step * kk, idesc, (ks | kk) != 0);
@@ -298,12 +289,11 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 }
                 __syncwarp();
             };
-            auto loaded = [&](int ks) {
-                const int s = (it + ks) % STAGES;
-                const uint32_t parity = ((it + ks) / STAGES) & 1;
+            auto loaded = [&](int ks, const Ring& r) {
+                const uint32_t s = r.s, parity = r.phase;
                 bool got = true;
                 if (ks == tail_step) {          // the only arrival on full_bar is the other CTA's, for its zeroed half
-                    got = zero_tail(smem + s * STAGE_BYTES, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane) &&
+                    got = zero_tail(smem + s * stage_bytes, slabs, t.count % BK, &tail_bar[s], (tails >> s) & 1, lane) &&
                           mbar_wait_cluster(&full_bar[s], parity);
                     tails ^= 1u << s;
                 }
@@ -313,38 +303,38 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             };
             if (!(ok = mbar_wait_cluster(&acc_empty[h0], ((turn >> 1) & 1) ^ 1))) break;
             tc_fence_after();
-            int done0 = 0;                      // k steps issued into the first accumulator
+            int done0 = 0;                      // k steps issued into the first accumulator, at `lead` in the ring
+            Ring lead = at;
             if (two) {
                 // Until the second accumulator is drained, the first goes ahead through the stages in the ring.
                 const uint32_t parity = (((turn + 1) >> 1) & 1) ^ 1;
-                const int ahead = min(t.k_steps, STAGES);
+                const int ahead = min(t.k_steps, (int)stages);
                 while (done0 < ahead && ok && !__shfl_sync(0xFFFFFFFFu, (int)mbar_test(&acc_empty[h1], parity), 0)) {
-                    if ((ok = loaded(done0))) products(0, done0++);
+                    if ((ok = loaded(done0, lead))) products(0, done0++, lead.s);
+                    lead.next(stages);
                 }
                 if (!(ok = ok && mbar_wait_cluster(&acc_empty[h1], parity))) break;
                 tc_fence_after();
             }
-            for (int ks = 0; ks < t.k_steps; ++ks) {
+            for (int ks = 0; ks < t.k_steps; ++ks, at.next(stages)) {
                 if (ks == done0) {
-                    if (!(ok = loaded(ks))) break;
-                    products(0, ks);
+                    if (!(ok = loaded(ks, at))) break;
+                    products(0, ks, at.s);
                     ++done0;
                 }
                 if (two && ks == t.k_steps - 1 && lane == 0) mma2_commit(&acc_full[h0]);
-                if (t.accs == 2) products(1, ks);
+                if (t.accs == 2) products(1, ks, at.s);
             }
             if (ok && lane == 0) {
                 if (two && t.k_steps == 0) mma2_commit(&acc_full[h0]);
                 mma2_commit(&acc_full[two ? h1 : h0]);
             }
             __syncwarp();
-            it += t.k_steps;
             turn += two ? 2 : 1;
         }
         if (!ok && lane == 0) report_wait_error(p.err);
     } else {
         const int q = warp & 3, h = (warp - 2) >> 2;    // tensor-memory lanes 32q.., TR of every STRIDE columns
-        T *turn_in = turns + (warp - 2) * 2 * TURN, *turn_out = turn_in + TURN;
         uint32_t turn = 0;
         for (int64_t i = first; tile_at<EPI, GATED>(p, lo, cnt, cum, i, t); i += step) {
             const bool two = two_turns(t);
@@ -382,8 +372,11 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     }
                 }
                 const int begin = h * TR;
-                uint4 ahead = make_uint4(0, 0, 0, 0);
-                if (aux) ahead = fetch_turn(aux + (int64_t)begin * p.ld_aux, p.ld_aux, n - begin, cols, p.vec_aux, lane);
+                const bool live = lane < cols;
+                out += min(lane, cols - 1);
+                if (aux) aux += min(lane, cols - 1);
+                T ahead[TR];
+                if (aux && begin < n) fetch_rows(ahead, aux + (int64_t)begin * p.ld_aux, p.ld_aux, n - begin);
                 uint32_t v[TR], w[TR];
                 if (begin < n) {
                     tmem_ld8(base + begin, v);
@@ -393,21 +386,15 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll 1
                 for (int c = begin; c < n; c += STRIDE) {
                     float z[TR], u[TR], x[TR];
-                    if (aux) {
-                        __syncwarp();
-                        *reinterpret_cast<uint4*>(turn_in + lane * 8) = ahead;
-                        if (c + STRIDE < n)
-                            ahead = fetch_turn(aux + (int64_t)(c + STRIDE) * p.ld_aux, p.ld_aux, n - c - STRIDE, cols, p.vec_aux, lane);
-                        __syncwarp();
-                    }
 #pragma unroll
                     for (int j = 0; j < TR; ++j) {
-                        x[j] = aux ? to_f<T>(turn_in[j * 32 + lane]) : 0.f;
+                        x[j] = aux ? to_f<T>(ahead[j]) : 0.f;
                         z[j] = __uint_as_float(v[j]) + add;
                         if constexpr (GATED) u[j] = __uint_as_float(w[j]) + add_up;
                         if (EPI == EPI_SUMS && t.k_steps == 0) z[j] = 0.f;
                     }
                     if (c + STRIDE < n) {               // the next rows, under this chunk's arithmetic
+                        if (aux) fetch_rows(ahead, aux + (int64_t)(c + STRIDE) * p.ld_aux, p.ld_aux, n - c - STRIDE);
                         tmem_ld8(base + c + STRIDE, v);
                         if constexpr (GATED) tmem_ld8(col[1] + c + STRIDE, w);
                     }
@@ -419,9 +406,9 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             default: finish<EPI, GATED, KQ_ACT_NONE>(z, u, x);
                         }
                     }
-                    store_turn(turn_out, z, out + (int64_t)c * p.ld_out, p.ld_out, n - c, cols, p.vec_out, lane);
+                    store_rows(out + (int64_t)c * p.ld_out, p.ld_out, live ? n - c : 0, z);
                     if constexpr (EPI == EPI_GRAD && GATED)
-                        store_turn(turn_out, u, out + (int64_t)c * p.ld_out + p.m_out, p.ld_out, n - c, cols, p.vec_out, lane);
+                        store_rows(out + (int64_t)c * p.ld_out + p.m_out, p.ld_out, live ? n - c : 0, u);
                     tmem_wait_ld();
                 }
             }
@@ -514,10 +501,6 @@ int relayout(Operand& o, uint16_t*& ws, int halves, cudaStream_t s) {
     ws += (o.batch * o.r * cols + 7) & ~(int64_t)7;
     o.direct = true;
     return KQ_OK;
-}
-
-bool vec8(const void* base, int64_t ld, int64_t ld2 = 0) {
-    return ((uintptr_t)base & 15) == 0 && ld % 8 == 0 && ld2 % 8 == 0;
 }
 
 // Pairs of CTAs that run at once (every instance needs a whole SM); asked once for each device.
@@ -621,11 +604,14 @@ size_t product_workspace(const kq_expert_product& p) {
 }
 
 // Two accumulators a tile where that leaves at least three tiles for every pair: fewer would stand idle, which costs
-// more than what the shared B tile saves (256 rows, 8192 -> 18944: 94 us with one accumulator, 145 us with two).
-int span_for(int64_t features, int64_t other_tiles, bool gated, int* span) {
+// more than what the shared B tile saves (256 rows, 8192 -> 18944: 94 us with one accumulator, 145 us with two).  The
+// epilogue of two is under fewer products than that of one, so a short contraction whose epilogue also reads rows takes
+// one (8192 rows, 1536 -> 12288 with residual: 303 us with one, 345 us with two; 7168 -> 7168: 767 and 728).
+int span_for(int64_t features, int64_t other_tiles, int64_t k, bool reads_rows, bool gated, int* span) {
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    *span = !gated && (features + 2 * TILE - 1) / (2 * TILE) * other_tiles >= 3 * (sms / 2) ? 2 * TILE : TILE;
+    const bool enough = (features + 2 * TILE - 1) / (2 * TILE) * other_tiles >= 3 * (sms / 2);
+    *span = !gated && enough && !(reads_rows && k <= 2048) ? 2 * TILE : TILE;
     return KQ_OK;
 }
 
@@ -648,7 +634,7 @@ int many_rows_product(const RowsProduct& p, cudaStream_t s) {
     q.experts = (int)p.experts;
     q.k_steps = (int)((p.k + BK - 1) / BK);
     const int64_t r_tiles = (p.rows + TILE - 1) / TILE + (p.experts < p.rows ? p.experts : p.rows) - 1;
-    if (int rc = span_for(p.n_out, r_tiles, p.gated, &q.span)) return rc;
+    if (int rc = span_for(p.n_out, r_tiles, p.k, p.aux != nullptr, p.gated, &q.span)) return rc;
     q.m_tiles = (int)((p.n_out + q.span - 1) / q.span);
     q.m_out = (int)p.n_out;
     q.up = p.up;
@@ -656,8 +642,6 @@ int many_rows_product(const RowsProduct& p, cudaStream_t s) {
     q.act = p.act;
     q.a_mn = p.mn;
     q.zero_rest = p.zero_rest;
-    q.vec_aux = vec8(p.aux, p.ld_aux);
-    q.vec_out = vec8(p.out, p.ld_out, p.grad && p.gated ? p.n_out : 0);
     const int64_t tiles = r_tiles * q.m_tiles;
     if (p.grad)
         return p.gated ? launch<EPI_GRAD, true>(p.bf16, ma, mb, mf, q, tiles, s) : launch<EPI_GRAD, false>(p.bf16, ma, mb, mf, q, tiles, s);
@@ -805,13 +789,12 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     q.rows = (int)p.rows;
     q.experts = (int)p.experts;
     q.n_tiles = (int)((lines + TILE - 1) / TILE);
-    if (int rc = span_for(cols, (int64_t)q.n_tiles * p.experts, false, &q.span)) return rc;
+    if (int rc = span_for(cols, (int64_t)q.n_tiles * p.experts, p.rows, false, false, &q.span)) return rc;
     q.m_tiles = (int)((cols + q.span - 1) / q.span);
     q.m_out = (int)cols;
     q.n_out = (int)lines;
     q.idesc = idesc_f16(bf16, true, true, TILE, 0);
     q.a_mn = q.b_mn = true;
-    q.vec_out = vec8(dw, ld, p.experts > 1 ? p.w_stride_e : 0);
     if ((int64_t)q.m_tiles * q.n_tiles > 0x7FFFFFFF) { set_error("%s: problem too large", what); return KQ_ERR_ARG; }
     return launch<EPI_SUMS, false>(bf16, ma, mb, mb, q, (int64_t)q.m_tiles * q.n_tiles * p.experts, s);
 }
