@@ -31,20 +31,28 @@
 namespace kq {
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 32;
-constexpr int CHUNK = BK * 128;                 // 32 rows x 64 columns of 16 bits
-constexpr int A_BYTES = BM / 64 * CHUNK, B_BYTES = BN / 64 * CHUNK;
+constexpr int BM = 128, BN = 256;
+constexpr int SLOT = 32;                        // experts are padded to whole slots of rows
 constexpr int THREADS = 320;
 constexpr int GROUP_BYTES = (kMaxExperts + 4) * 4;
+constexpr int PIECE_BYTES = 8192;               // a drain warp's 32 x 32 piece of H and its mirror image
 
-constexpr int stage_bytes(int na, int nb) { return na * A_BYTES + nb * B_BYTES; }
+constexpr int products(int na, int nb) { return na == 1 ? nb : na == 2 ? 5 : 6; }
+// Rows of a stage: one product needs 32 for its loads to be worth a barrier; with more terms 16 keep four stages.
+constexpr int stage_rows(int na, int nb) { return products(na, nb) == 1 ? 32 : 16; }
+// 64 columns of a stage: rows of 128 bytes.
+constexpr int chunk_bytes(int na, int nb) { return stage_rows(na, nb) * 128; }
+constexpr int stage_bytes(int na, int nb) { return (na * (BM / 64) + nb * (BN / 64)) * chunk_bytes(na, nb); }
+// Pieces that a drain warp has under way: one product of few rows is all output.
+constexpr int pieces(int na, int nb) { return products(na, nb) == 1 ? 2 : 1; }
 constexpr int stages_for(int na, int nb) {
-    const int fit = (227 * 1024 - 1024 - GROUP_BYTES - 512) / stage_bytes(na, nb);
+    const int fit = (227 * 1024 - 1024 - GROUP_BYTES - pieces(na, nb) * 8 * PIECE_BYTES - 512) / stage_bytes(na, nb);
     return fit > 8 ? 8 : fit;
 }
-constexpr int products(int na, int nb) { return na == 1 ? nb : na == 2 ? 5 : 6; }
 // Stages per drain: 128 rows of one product, 64 of three, 32 of more.
-constexpr int seg_stages(int na, int nb) { return products(na, nb) == 1 ? 4 : products(na, nb) == 3 ? 2 : 1; }
+constexpr int seg_stages(int na, int nb) {
+    return (products(na, nb) == 1 ? 128 : products(na, nb) == 3 ? 64 : 32) / stage_rows(na, nb);
+}
 
 struct Maps { CUtensorMap a[3], b[3]; };
 
@@ -55,7 +63,7 @@ struct Params {
     int64_t h_stride, ldh;
     int rows, experts, d, tiles;   // tiles per expert
     uint32_t idesc;
-    bool add, vec;
+    bool add, tma;
 };
 
 // Tile l of an expert: column block ni holds the row blocks 0 .. 2 ni + 1.
@@ -77,13 +85,16 @@ __device__ __forceinline__ void product_terms(int i, int& a, int& b) {
 
 template <int NA, int NB>
 __global__ void __launch_bounds__(THREADS, 1)
-hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
+hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_h, const Params p) {
     constexpr int STAGES = stages_for(NA, NB), STAGE = stage_bytes(NA, NB), SEG = seg_stages(NA, NB);
+    constexpr int BK = stage_rows(NA, NB), PER_SLOT = SLOT / BK, CHUNK = chunk_bytes(NA, NB);
+    constexpr int A_BYTES = BM / 64 * CHUNK, B_BYTES = BN / 64 * CHUNK;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], seg_full[2], seg_empty[2];
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    int* cum = reinterpret_cast<int*>(smem + STAGES * STAGE);
+    uint8_t* out_smem = smem + STAGES * STAGE;
+    int* cum = reinterpret_cast<int*>(out_smem + pieces(NA, NB) * 8 * PIECE_BYTES);
     int* lo = reinterpret_cast<int*>(smem);     // needed by the scan alone, before the first stage is loaded
     int* cnt = lo + kMaxExperts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,7 +111,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
         mbar_init_fence();
     }
     if (warp == 8) tmem_alloc(&tmem_slot, 2 * BN);
-    scan_groups(p.offsets, p.experts, p.rows, BK, lo, cnt, cum);
+    scan_groups(p.offsets, p.experts, p.rows, SLOT, lo, cnt, cum);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -116,21 +127,16 @@ hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
                 const int e = (int)(i / p.tiles);
                 int m0, n0;
                 tri_tile((int)(i - (int64_t)e * p.tiles), m0, n0);
-                for (int ks = cum[e]; ks < cum[e + 1]; ++ks, ++it) {
+                for (int ks = cum[e] * PER_SLOT; ks < cum[e + 1] * PER_SLOT; ++ks, ++it) {
                     const int s = it % STAGES;
                     if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
                     mbar_expect_tx(&full_bar[s], STAGE);
                     uint8_t* dst = smem + s * STAGE;
 #pragma unroll
-                    for (int t = 0; t < NA; ++t)
-#pragma unroll
-                        for (int c = 0; c < BM / 64; ++c, dst += CHUNK)
-                            tma_load_2d(dst, &maps.a[t], m0 + 64 * c, ks * BK, &full_bar[s]);
+                    for (int t = 0; t < NA; ++t) tma_load_3d(dst + t * A_BYTES, &maps.a[t], 0, ks * BK, m0 / 64, &full_bar[s]);
 #pragma unroll
                     for (int t = 0; t < NB; ++t)
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c, dst += CHUNK)
-                            tma_load_2d(dst, &maps.b[t], n0 + 64 * c, ks * BK, &full_bar[s]);
+                        tma_load_3d(dst + NA * A_BYTES + t * B_BYTES, &maps.b[t], 0, ks * BK, n0 / 64, &full_bar[s]);
                 }
             }
             if (!ok) report_wait_error(p.err);
@@ -140,8 +146,8 @@ hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
             uint32_t it = 0, seg = 0;
             bool ok = true;
             for (int64_t i = blockIdx.x; i < all && ok; i += gridDim.x) {
-                const int e = (int)(i / p.tiles), ks_end = cum[e + 1];
-                for (int ks0 = cum[e]; ks0 < ks_end && ok; ks0 += SEG, ++seg) {
+                const int e = (int)(i / p.tiles), ks_end = cum[e + 1] * PER_SLOT;
+                for (int ks0 = cum[e] * PER_SLOT; ks0 < ks_end && ok; ks0 += SEG, ++seg) {
                     const int b = seg & 1;
                     if (!(ok = mbar_wait(&seg_empty[b], ((seg >> 1) & 1) ^ 1))) break;
                     tc_fence_after();
@@ -173,67 +179,123 @@ hessian_kernel(const __grid_constant__ Maps maps, const Params p) {
         const int q = warp & 3, h = warp >> 2;
         uint32_t seg = 0;
         bool ok = true;
+        constexpr int PIECES = pieces(NA, NB);
+        int piece_no = 0;
         for (int64_t it = blockIdx.x; it < all && ok; it += gridDim.x) {
-            const int e = (int)(it / p.tiles), ks_end = cum[e + 1];
+            const int e = (int)(it / p.tiles), ks_begin = cum[e] * PER_SLOT, ks_end = cum[e + 1] * PER_SLOT;
             int m0, n0;
             tri_tile((int)(it - (int64_t)e * p.tiles), m0, n0);
+            const int i0 = m0 + q * 32, j0 = n0 + h * (BN / 2);
+            float* H = p.H + e * p.h_stride;
+            // Columns j0 + c .. + 31 of this warp's 32 rows: a block above the diagonal and its mirror image, or the block
+            // on it made symmetric.  Whole 128-byte lines either way: 32-byte pieces of 32 rows at a time ran at a third.
+            auto put = [&](const float* v, int c) {
+                const int j = j0 + c;
+                if (i0 >= p.d || j >= p.d || j < i0) return;
+                uint8_t* piece = out_smem + (warp * PIECES + piece_no) * PIECE_BYTES;
+                uint8_t* mirror = piece + PIECE_BYTES / 2;
+                piece_no = (piece_no + 1) % PIECES;
+                const bool diagonal = i0 == j;
+                // Element (row, col) of a 32 x 32 block, 16-byte units swizzled by the row as the TMA map has them.
+                auto at = [](uint8_t* block, int row, int col) {
+                    return reinterpret_cast<float*>(block + row * 128 + (((col >> 2) ^ (row & 7)) << 4) + (col & 3) * 4);
+                };
+                if (lane == 0) bulk_wait_read<PIECES - 1>();
+                __syncwarp();
+                if (!diagonal) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        *reinterpret_cast<float4*>(at(piece, lane, 4 * k)) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) *at(mirror, k, lane) = v[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        if (k >= lane) {
+                            *at(piece, lane, k) = v[k];
+                            *at(piece, k, lane) = v[k];
+                        }
+                    }
+                }
+                if (p.tma) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (p.add) {
+                            tma_add_3d(&map_h, piece, j, i0, e);
+                            if (!diagonal) tma_add_3d(&map_h, mirror, i0, j, e);
+                        } else {
+                            tma_store_3d(&map_h, piece, j, i0, e);
+                            if (!diagonal) tma_store_3d(&map_h, mirror, i0, j, e);
+                        }
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
+                        const int row0 = side ? j : i0, col = (side ? i0 : j) + lane;
+                        uint8_t* block = side ? mirror : piece;
+                        if (col >= p.d) continue;
+                        float* dst = H + (int64_t)row0 * p.ldh + col;
+                        for (int k = 0; k < min(32, p.d - row0); ++k, dst += p.ldh) {
+                            if (p.add) atomicAdd(dst, *at(block, k, lane));
+                            else *dst = *at(block, k, lane);
+                        }
+                    }
+                    __syncwarp();
+                }
+            };
+            auto wait_seg = [&]() {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[seg & 1], (seg >> 1) & 1));
+                tc_fence_after();
+                return tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((seg & 1) * BN + h * (BN / 2));
+            };
+            auto free_seg = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&seg_empty[seg & 1]);
+                ++seg;
+            };
+            if (ks_end > ks_begin && ks_end - ks_begin <= SEG) {
+                // All rows in one segment: from tensor memory to H, 32 columns at a time.
+                const uint32_t base = wait_seg();
+                if (!ok) break;
+#pragma unroll 1
+                for (int c = 0; c < BN / 2; c += 32) {
+                    uint32_t u[32];
+                    float v[32];
+                    tmem_ld32(base + c, u);
+                    tmem_wait_ld();
+                    if (c + 32 == BN / 2) free_seg();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(u[k]);
+                    put(v, c);
+                }
+                continue;
+            }
             float r[BN / 2];
 #pragma unroll
-            for (int i = 0; i < BN / 2; ++i) r[i] = 0.f;
-            for (int ks0 = cum[e]; ks0 < ks_end; ks0 += SEG, ++seg) {
-                const int b = seg & 1;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[b], (seg >> 1) & 1));
+            for (int k = 0; k < BN / 2; ++k) r[k] = 0.f;
+            for (int ks0 = ks_begin; ks0 < ks_end; ks0 += SEG) {
+                const uint32_t base = wait_seg();
                 if (!ok) break;
-                tc_fence_after();
-                const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + h * (BN / 2));
 #pragma unroll
                 for (int c0 = 0; c0 < BN / 2; c0 += 16) {
                     uint32_t v[16];
                     tmem_ld16(base + (uint32_t)c0, v);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) r[c0 + i] += __uint_as_float(v[i]);
+                    for (int k = 0; k < 16; ++k) r[c0 + k] += __uint_as_float(v[k]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&seg_empty[b]);
+                free_seg();
             }
-            if (!ok || (p.add && cum[e] == ks_end)) continue;
-            const int i = m0 + q * 32 + lane, j0 = n0 + h * (BN / 2);
-            if (i < p.d) {
-                float* H = p.H + e * p.h_stride;
-                float* drow = H + (int64_t)i * p.ldh;
+            if (!ok) break;
+            if (p.add && ks_begin == ks_end) continue;
 #pragma unroll
-                for (int c = 0; c < BN / 2; c += 4) {
-                    const int j = j0 + c;
-                    if (p.vec && j + 3 < p.d && j >= i) {
-                        float4* dp = reinterpret_cast<float4*>(drow + j);
-                        const float4 v = make_float4(r[c], r[c + 1], r[c + 2], r[c + 3]);
-                        if (p.add) atomicAdd(dp, v);
-                        else __stcs(dp, v);
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if (j + x < p.d && j + x >= i) {
-                                if (p.add) atomicAdd(drow + j + x, r[c + x]);
-                                else drow[j + x] = r[c + x];
-                            }
-                        }
-                    }
-                }
-                // (col, row) above the diagonal: lanes hold consecutive rows, one 128-byte access a column.
-#pragma unroll
-                for (int c = 0; c < BN / 2; ++c) {
-                    const int j = j0 + c;
-                    if (j > i && j < p.d) {
-                        float* dp = H + (int64_t)j * p.ldh + i;
-                        if (p.add) atomicAdd(dp, r[c]);
-                        else __stcs(dp, r[c]);
-                    }
-                }
-            }
+            for (int c = 0; c < BN / 2; c += 32) put(r + c, c);
             __syncwarp();
         }
+        if (lane == 0) bulk_wait_all();
         if (!ok && lane == 0) report_wait_error(p.err);
     }
     tc_fence_before();
@@ -292,11 +354,11 @@ __global__ void __launch_bounds__(256) operand_kernel(const OperandParams p) {
         if (threadIdx.x == 0) p.den[e] = part[0];
         return;
     }
-    scan_groups(p.offsets, p.experts, p.rows, BK, lo, cnt, cum);
+    scan_groups(p.offsets, p.experts, p.rows, SLOT, lo, cnt, cum);
     const int t = blockIdx.x;
     if (t >= cum[p.experts]) return;
-    const int e = expert_of(cum, p.experts, t), first = (t - cum[e]) * BK;
-    for (int i = threadIdx.x; i < BK * 128; i += 256) {        // 8 columns of one row at a time
+    const int e = expert_of(cum, p.experts, t), first = (t - cum[e]) * SLOT;
+    for (int i = threadIdx.x; i < SLOT * 128; i += 256) {        // 8 columns of one row at a time
         const int r = i >> 7, c = blockIdx.y * 1024 + (i & 127) * 8;
         if (c >= p.ld) continue;
         float v[8];
@@ -323,7 +385,7 @@ __global__ void __launch_bounds__(256) operand_kernel(const OperandParams p) {
                 }
             }
         }
-        uint16_t* dst = p.terms + ((int64_t)t * BK + r) * p.ld + c;
+        uint16_t* dst = p.terms + ((int64_t)t * SLOT + r) * p.ld + c;
         if constexpr (NA == 0) {
             T o[8];
 #pragma unroll
@@ -347,9 +409,9 @@ __global__ void __launch_bounds__(256) operand_kernel(const OperandParams p) {
     }
 }
 
-int64_t pad8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+int64_t pad_width(int64_t v) { return (v + 63) & ~(int64_t)63; }
 
-int64_t slots(int64_t rows, int64_t experts) { return ((rows + BK - 1) / BK + (experts < rows ? experts : rows)) * BK; }
+int64_t slots(int64_t rows, int64_t experts) { return ((rows + SLOT - 1) / SLOT + (experts < rows ? experts : rows)) * SLOT; }
 
 void terms_of(int dtype, bool weighted, int& na, int& nb) {
     if (dtype == KQ_FP32) { na = 3; nb = 3; }
@@ -366,11 +428,11 @@ int term_count(int dtype, bool weighted) {
 }
 
 template <int NA, int NB>
-int launch_hessian(const Maps& m, const Params& p, int grid, cudaStream_t s) {
-    constexpr int smem = stages_for(NA, NB) * stage_bytes(NA, NB) + GROUP_BYTES + 1024;
+int launch_hessian(const Maps& m, const CUtensorMap& h, const Params& p, int grid, cudaStream_t s) {
+    constexpr int smem = stages_for(NA, NB) * stage_bytes(NA, NB) + pieces(NA, NB) * 8 * PIECE_BYTES + GROUP_BYTES + 1024;
     cudaError_t e = cudaFuncSetAttribute(hessian_kernel<NA, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
-    hessian_kernel<NA, NB><<<grid, THREADS, smem, s>>>(m, p);
+    hessian_kernel<NA, NB><<<grid, THREADS, smem, s>>>(m, h, p);
     return check_launch("hessian_kernel");
 }
 
@@ -385,7 +447,7 @@ bool bad_sizes(int64_t rows, int64_t tokens, int64_t d, int64_t experts, int dty
 extern "C" size_t kq_expert_hessian_workspace_bytes(int64_t rows, int64_t dim, int64_t experts, int dtype, int weighted) {
     using namespace kq;
     if (bad_sizes(rows, 0, dim, experts, dtype) || rows == 0) return 0;
-    return (size_t)term_count(dtype, weighted != 0) * (size_t)slots(rows, experts) * (size_t)pad8(dim) * 2;
+    return (size_t)term_count(dtype, weighted != 0) * (size_t)slots(rows, experts) * (size_t)pad_width(dim) * 2;
 }
 
 extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int64_t dim, int64_t ldx, int dtype,
@@ -409,7 +471,7 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
     Params q{};
     if (int rc = wait_error_word(&q.err)) return rc;
-    const int ld = (int)pad8(dim);
+    const int ld = (int)pad_width(dim);
     const int64_t n_slots = slots(rows, experts);
     int na, nb;
     terms_of(dtype, weighted, na, nb);
@@ -428,7 +490,7 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     o.experts = (int)experts;
     o.d = (int)dim;
     o.ld = ld;
-    o.row_tiles = (int)(n_slots / BK);
+    o.row_tiles = (int)(n_slots / SLOT);
     o.vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     const dim3 grid((unsigned)(o.row_tiles + experts), (unsigned)((ld + 1023) / 1024));
     if (dtype == KQ_FP32) operand_kernel<float, 3, 3><<<grid, 256, 0, s>>>(o);
@@ -438,20 +500,17 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     else operand_kernel<__half, 0, 0><<<grid, 256, 0, s>>>(o);
     if (int rc = check_launch("operand_kernel")) return rc;
 
-    Maps maps;
+    Maps maps{};
     const bool fp16 = dtype == KQ_FP16 && !weighted;
-    const int count = term_count(dtype, weighted);
-    CUtensorMap term[6];
-    const int64_t dims[2] = {dim, n_slots > 0 ? n_slots : 1}, strides[1] = {(int64_t)ld * 2};
-    const int box[2] = {64, BK};
-    for (int t = 0; t < count && rows > 0; ++t)
-        if (int rc = encode_tiles(&term[t], fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                  o.terms + t * o.term_stride, dims, strides, box, what))
-            return rc;
-    for (int t = 0; t < 3 && rows > 0; ++t) {
-        maps.a[t] = term[na ? (t < na ? t : 0) : 0];
-        maps.b[t] = term[na ? na + (t < nb ? t : 0) : 0];
-    }
+    // A term as [64-column slab][row][64]: one TMA instruction brings all slabs of a side (its issue bounded the loads).
+    const int64_t dims[3] = {64, n_slots > 0 ? n_slots : 1, ld / 64}, strides[2] = {(int64_t)ld * 2, 128};
+    const int box_rows = na ? stage_rows(na, nb) : stage_rows(1, 1);
+    const int box_a[3] = {64, box_rows, BM / 64}, box_b[3] = {64, box_rows, BN / 64};
+    const CUtensorMapDataType type = fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int t = 0; t < (na ? na : 1) && rows > 0; ++t)
+        if (int rc = encode_tiles(&maps.a[t], type, 3, o.terms + t * o.term_stride, dims, strides, box_a, what)) return rc;
+    for (int t = 0; t < (na ? nb : 1) && rows > 0; ++t)
+        if (int rc = encode_tiles(&maps.b[t], type, 3, o.terms + (na + t) * o.term_stride, dims, strides, box_b, what)) return rc;
     q.offsets = offsets;
     q.H = H;
     q.h_stride = h_stride;
@@ -463,13 +522,20 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     q.tiles = (int)(nt * (nt + 1));
     q.idesc = idesc_f16(!fp16, true, true, BM, BN);
     q.add = add != 0;
-    q.vec = ((uintptr_t)H & 15) == 0 && ldh % 4 == 0 && h_stride % 4 == 0;
+    const bool vec = ((uintptr_t)H & 15) == 0 && ldh % 4 == 0 && h_stride % 4 == 0;
+    CUtensorMap map_h{};
+    q.tma = vec && (dim == 1 || ldh >= dim) && ldh < ((int64_t)1 << 36) && h_stride < ((int64_t)1 << 36);
+    if (q.tma) {
+        const int64_t hd[3] = {dim, dim, experts}, hs[2] = {ldh * 4, (experts > 1 ? h_stride : ldh * dim) * 4};
+        const int hb[3] = {32, 32, 1};
+        if (int rc = encode_tiles(&map_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, H, hd, hs, hb, what)) return rc;
+    }
     int sms;
     if (int rc = sm_count(&sms)) return rc;
     const int64_t tiles = (int64_t)q.tiles * experts;
     const int g = (int)(tiles < sms ? tiles : sms);
-    if (na == 0) return launch_hessian<1, 1>(maps, q, g, s);
-    if (na == 1) return launch_hessian<1, 3>(maps, q, g, s);
-    if (na == 2) return launch_hessian<2, 3>(maps, q, g, s);
-    return launch_hessian<3, 3>(maps, q, g, s);
+    if (na == 0) return launch_hessian<1, 1>(maps, map_h, q, g, s);
+    if (na == 1) return launch_hessian<1, 3>(maps, map_h, q, g, s);
+    if (na == 2) return launch_hessian<2, 3>(maps, map_h, q, g, s);
+    return launch_hessian<3, 3>(maps, map_h, q, g, s);
 }
