@@ -21,11 +21,11 @@
 // are stored, since an MN-major tcgen05 operand needs no transpose.
 //
 // One persistent CTA per SM walks the 128 x 256 output tiles on or above the
-// diagonal.  A stage holds 32 rows of every term, so each is fetched once for
-// all products.  The tensor-core accumulator truncates: it holds only a few
+// diagonal.  A stage holds 16 or 32 rows of every term, so each is fetched once
+// for all products.  The tensor-core accumulator truncates: it holds only a few
 // stages (up to 128 rows), which the drain warps add into fp32 registers with
-// rounding.  Elements above the diagonal are written twice, so H is exactly
-// symmetric.  With few rows the kernel is bound by writing H.
+// rounding.  Blocks above the diagonal are written twice, so H is exactly
+// symmetric.  With few rows writing H is what it costs (see `whole` below).
 #include "kq_expert.cuh"
 
 namespace kq {
@@ -33,9 +33,10 @@ namespace {
 
 constexpr int BM = 128, BN = 256;
 constexpr int SLOT = 32;                        // experts are padded to whole slots of rows
-constexpr int THREADS = 320;
+constexpr int drain_warps(bool whole) { return whole ? 16 : 8; }
+constexpr int threads(bool whole) { return 64 + 32 * drain_warps(whole); }
 constexpr int GROUP_BYTES = (kMaxExperts + 4) * 4;
-constexpr int PIECE_BYTES = 8192;               // a drain warp's 32 x 32 piece of H and its mirror image
+constexpr int PIECE_BYTES = 8192;               // a drain warp's 32 x 32 block of H and its mirror image, or 32 x 64 block
 
 constexpr int products(int na, int nb) { return na == 1 ? nb : na == 2 ? 5 : 6; }
 // Rows of a stage: one product needs 32 for its loads to be worth a barrier; with more terms 16 keep four stages.
@@ -43,10 +44,8 @@ constexpr int stage_rows(int na, int nb) { return products(na, nb) == 1 ? 32 : 1
 // 64 columns of a stage: rows of 128 bytes.
 constexpr int chunk_bytes(int na, int nb) { return stage_rows(na, nb) * 128; }
 constexpr int stage_bytes(int na, int nb) { return (na * (BM / 64) + nb * (BN / 64)) * chunk_bytes(na, nb); }
-// Pieces that a drain warp has under way: one product of few rows is all output.
-constexpr int pieces(int na, int nb) { return products(na, nb) == 1 ? 2 : 1; }
-constexpr int stages_for(int na, int nb) {
-    const int fit = (227 * 1024 - 1024 - GROUP_BYTES - pieces(na, nb) * 8 * PIECE_BYTES - 512) / stage_bytes(na, nb);
+constexpr int stages_for(int na, int nb, bool whole) {
+    const int fit = (227 * 1024 - 1024 - GROUP_BYTES - drain_warps(whole) * PIECE_BYTES - 512) / stage_bytes(na, nb);
     return fit > 8 ? 8 : fit;
 }
 // Stages per drain: 128 rows of one product, 64 of three, 32 of more.
@@ -61,13 +60,19 @@ struct Params {
     float* H;
     int* err;
     int64_t h_stride, ldh;
-    int rows, experts, d, tiles;   // tiles per expert
+    int rows, experts, d, tiles, n_tiles;   // tiles per expert, and in a row of them
     uint32_t idesc;
-    bool add, tma;
+    bool add, vec;
 };
 
-// Tile l of an expert: column block ni holds the row blocks 0 .. 2 ni + 1.
-__device__ __forceinline__ void tri_tile(int l, int& m0, int& n0) {
+// Tile l of an expert.  On or above the diagonal: column block ni holds the row blocks 0 .. 2 ni + 1.  Whole: row by row.
+template <bool WHOLE>
+__device__ __forceinline__ void tile_at(int l, int n_tiles, int& m0, int& n0) {
+    if constexpr (WHOLE) {
+        m0 = l / n_tiles * BM;
+        n0 = l % n_tiles * BN;
+        return;
+    }
     int ni = (int)((sqrtf(4.f * l + 1.f) - 1.f) * 0.5f);
     while (ni * (ni + 1) > l) --ni;
     while ((ni + 1) * (ni + 2) <= l) ++ni;
@@ -83,10 +88,11 @@ __device__ __forceinline__ void product_terms(int i, int& a, int& b) {
     else { a = (0x0052 >> (i * 2)) & 3; b = (0x0118 >> (i * 2)) & 3; }
 }
 
-template <int NA, int NB>
-__global__ void __launch_bounds__(THREADS, 1)
+// WHOLE: every tile of H, without mirror images.
+template <int NA, int NB, bool WHOLE>
+__global__ void __launch_bounds__(threads(WHOLE), 1)
 hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_h, const Params p) {
-    constexpr int STAGES = stages_for(NA, NB), STAGE = stage_bytes(NA, NB), SEG = seg_stages(NA, NB);
+    constexpr int STAGES = stages_for(NA, NB, WHOLE), STAGE = stage_bytes(NA, NB), SEG = seg_stages(NA, NB);
     constexpr int BK = stage_rows(NA, NB), PER_SLOT = SLOT / BK, CHUNK = chunk_bytes(NA, NB);
     constexpr int A_BYTES = BM / 64 * CHUNK, B_BYTES = BN / 64 * CHUNK;
     extern __shared__ uint8_t smem_raw[];
@@ -94,7 +100,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* out_smem = smem + STAGES * STAGE;
-    int* cum = reinterpret_cast<int*>(out_smem + pieces(NA, NB) * 8 * PIECE_BYTES);
+    int* cum = reinterpret_cast<int*>(out_smem + drain_warps(WHOLE) * PIECE_BYTES);
     int* lo = reinterpret_cast<int*>(smem);     // needed by the scan alone, before the first stage is loaded
     int* cnt = lo + kMaxExperts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -110,7 +116,8 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
         }
         mbar_init_fence();
     }
-    if (warp == 8) tmem_alloc(&tmem_slot, 2 * BN);
+    constexpr int DRAINS = drain_warps(WHOLE);
+    if (warp == DRAINS) tmem_alloc(&tmem_slot, 2 * BN);
     scan_groups(p.offsets, p.experts, p.rows, SLOT, lo, cnt, cum);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
@@ -119,14 +126,14 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     const uint32_t tmem = tmem_slot;
     const int64_t all = (int64_t)p.tiles * p.experts;
 
-    if (warp == 8) {
+    if (warp == DRAINS) {
         if (lane == 0) {
             uint32_t it = 0;
             bool ok = true;
             for (int64_t i = blockIdx.x; i < all && ok; i += gridDim.x) {
                 const int e = (int)(i / p.tiles);
                 int m0, n0;
-                tri_tile((int)(i - (int64_t)e * p.tiles), m0, n0);
+                tile_at<WHOLE>((int)(i - (int64_t)e * p.tiles), p.n_tiles, m0, n0);
                 for (int ks = cum[e] * PER_SLOT; ks < cum[e + 1] * PER_SLOT; ++ks, ++it) {
                     const int s = it % STAGES;
                     if (!(ok = mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1))) break;
@@ -141,7 +148,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
             }
             if (!ok) report_wait_error(p.err);
         }
-    } else if (warp == 9) {
+    } else if (warp == DRAINS + 1) {
         if (lane == 0) {
             uint32_t it = 0, seg = 0;
             bool ok = true;
@@ -175,16 +182,89 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
             }
             if (!ok) report_wait_error(p.err);
         }
+    } else if constexpr (WHOLE) {
+        // Two groups of eight warps take tiles in turn (four quarters of the rows, two halves of the columns): one stores
+        // while the other fills its buffers.  A tile's further segments (an expert of more rows) are added to what its
+        // first one wrote, by the same thread.
+        const int q = warp & 3, h = (warp >> 2) & 1, group = warp >> 3;
+        uint8_t* stage = out_smem + warp * PIECE_BYTES;          // two 32 x 32 pieces under way
+        uint32_t seg = 0, piece_no = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; it < all && ok; it += gridDim.x) {
+            const int e = (int)(it / p.tiles), ks_begin = cum[e] * PER_SLOT, ks_end = cum[e + 1] * PER_SLOT;
+            int m0, n0;
+            tile_at<WHOLE>((int)(it - (int64_t)e * p.tiles), p.n_tiles, m0, n0);
+            const int i0 = m0 + q * 32, j0 = n0 + h * (BN / 2);
+            // Columns j0 + c .. + 31 of this warp's 32 rows.
+            auto put = [&](const uint32_t (&v)[32], int c, bool add) {
+                uint8_t* piece = stage + (piece_no++ & 1) * (PIECE_BYTES / 2);
+                auto unit = [&](int row, int u) { return reinterpret_cast<uint4*>(piece + row * 128 + ((u ^ (row & 7)) << 4)); };
+                if (lane == 0) bulk_wait_read<1>();
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 8; ++u) *unit(lane, u) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                if (p.vec) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (i0 < p.d && j0 + c < p.d) {
+                            if (add) tma_add_3d(&map_h, piece, j0 + c, i0, e);
+                            else tma_store_3d(&map_h, piece, j0 + c, i0, e);
+                        }
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    const int j = j0 + c + lane;
+                    float* dst = p.H + e * p.h_stride + (int64_t)i0 * p.ldh + j;
+                    for (int k = 0; k < min(32, p.d - i0) && j < p.d; ++k, dst += p.ldh) {
+                        const float x = reinterpret_cast<const float*>(unit(k, lane >> 2))[lane & 3];
+                        if (add) atomicAdd(dst, x);
+                        else *dst = x;
+                    }
+                    __syncwarp();
+                }
+            };
+            if (ks_begin == ks_end) {
+                if (p.add || ((it / gridDim.x) & 1) != group) continue;
+                const uint32_t zero[32] = {};
+                for (int c = 0; c < BN / 2; c += 32) put(zero, c, false);
+                continue;
+            }
+            const int owner = seg & 1;
+            for (int ks0 = ks_begin; ks0 < ks_end; ks0 += SEG, ++seg) {
+                if (owner != group) continue;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[seg & 1], (seg >> 1) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                if (ks0 > ks_begin && lane == 0) bulk_wait_all();      // what this adds to is there
+                __syncwarp();
+                const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((seg & 1) * BN + h * (BN / 2));
+#pragma unroll 1
+                for (int c = 0; c < BN / 2; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(base + c, v);
+                    tmem_wait_ld();
+                    if (c + 32 == BN / 2) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&seg_empty[seg & 1]);
+                    }
+                    put(v, c, p.add || ks0 > ks_begin);
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+        if (!ok && lane == 0) report_wait_error(p.err);
     } else {
         const int q = warp & 3, h = warp >> 2;
         uint32_t seg = 0;
         bool ok = true;
-        constexpr int PIECES = pieces(NA, NB);
-        int piece_no = 0;
+        uint8_t *piece = out_smem + warp * PIECE_BYTES, *mirror = piece + PIECE_BYTES / 2;
         for (int64_t it = blockIdx.x; it < all && ok; it += gridDim.x) {
             const int e = (int)(it / p.tiles), ks_begin = cum[e] * PER_SLOT, ks_end = cum[e + 1] * PER_SLOT;
             int m0, n0;
-            tri_tile((int)(it - (int64_t)e * p.tiles), m0, n0);
+            tile_at<WHOLE>((int)(it - (int64_t)e * p.tiles), p.n_tiles, m0, n0);
             const int i0 = m0 + q * 32, j0 = n0 + h * (BN / 2);
             float* H = p.H + e * p.h_stride;
             // Columns j0 + c .. + 31 of this warp's 32 rows: a block above the diagonal and its mirror image, or the block
@@ -192,16 +272,11 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
             auto put = [&](const float* v, int c) {
                 const int j = j0 + c;
                 if (i0 >= p.d || j >= p.d || j < i0) return;
-                uint8_t* piece = out_smem + (warp * PIECES + piece_no) * PIECE_BYTES;
-                uint8_t* mirror = piece + PIECE_BYTES / 2;
-                piece_no = (piece_no + 1) % PIECES;
                 const bool diagonal = i0 == j;
                 // Element (row, col) of a 32 x 32 block, 16-byte units swizzled by the row as the TMA map has them.
                 auto at = [](uint8_t* block, int row, int col) {
                     return reinterpret_cast<float*>(block + row * 128 + (((col >> 2) ^ (row & 7)) << 4) + (col & 3) * 4);
                 };
-                if (lane == 0) bulk_wait_read<PIECES - 1>();
-                __syncwarp();
                 if (!diagonal) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
@@ -217,21 +292,24 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                         }
                     }
                 }
-                if (p.tma) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (p.add) {
-                            tma_add_3d(&map_h, piece, j, i0, e);
-                            if (!diagonal) tma_add_3d(&map_h, mirror, i0, j, e);
-                        } else {
-                            tma_store_3d(&map_h, piece, j, i0, e);
-                            if (!diagonal) tma_store_3d(&map_h, mirror, i0, j, e);
+                __syncwarp();
+                if (p.vec) {
+                    // 16 bytes a lane, four rows an access.
+                    for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
+                        const int row0 = (side ? j : i0) + (lane >> 3), col = (side ? i0 : j) + (lane & 7) * 4;
+                        uint8_t* block = side ? mirror : piece;
+                        if (col >= p.d) continue;
+                        float* dst = H + (int64_t)row0 * p.ldh + col;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4, dst += 4 * p.ldh) {
+                            if (row0 + k >= p.d) break;
+                            const float4 x = *reinterpret_cast<const float4*>(at(block, (lane >> 3) + k, (lane & 7) * 4));
+                            if (p.add) atomicAdd(reinterpret_cast<float4*>(dst), x);
+                            else __stcs(reinterpret_cast<float4*>(dst), x);
                         }
-                        bulk_commit();
                     }
-                } else {
                     __syncwarp();
+                } else {
                     for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
                         const int row0 = side ? j : i0, col = (side ? i0 : j) + lane;
                         uint8_t* block = side ? mirror : piece;
@@ -257,18 +335,20 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                 ++seg;
             };
             if (ks_end > ks_begin && ks_end - ks_begin <= SEG) {
-                // All rows in one segment: from tensor memory to H, 32 columns at a time.
+                // All rows in one segment: from tensor memory to H.
                 const uint32_t base = wait_seg();
                 if (!ok) break;
+                constexpr int STEP = 32;
 #pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
-                    uint32_t u[32];
-                    float v[32];
-                    tmem_ld32(base + c, u);
-                    tmem_wait_ld();
-                    if (c + 32 == BN / 2) free_seg();
+                for (int c = 0; c < BN / 2; c += STEP) {
+                    uint32_t u[STEP / 32][32];
+                    float v[STEP];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(u[k]);
+                    for (int k = 0; k < STEP; k += 32) tmem_ld32(base + c + k, u[k / 32]);
+                    tmem_wait_ld();
+                    if (c + STEP == BN / 2) free_seg();
+#pragma unroll
+                    for (int k = 0; k < STEP; ++k) v[k] = __uint_as_float(u[k >> 5][k & 31]);
                     put(v, c);
                 }
                 continue;
@@ -295,12 +375,11 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
             for (int c = 0; c < BN / 2; c += 32) put(r + c, c);
             __syncwarp();
         }
-        if (lane == 0) bulk_wait_all();
         if (!ok && lane == 0) report_wait_error(p.err);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_free(tmem, 2 * BN);
+    if (warp == DRAINS) tmem_free(tmem, 2 * BN);
 }
 
 // Operand rows.  Block (t, c): slots 32 t .. of the padded rows, columns
@@ -427,12 +506,12 @@ int term_count(int dtype, bool weighted) {
     return na == 0 ? 1 : na + nb;
 }
 
-template <int NA, int NB>
+template <int NA, int NB, bool WHOLE>
 int launch_hessian(const Maps& m, const CUtensorMap& h, const Params& p, int grid, cudaStream_t s) {
-    constexpr int smem = stages_for(NA, NB) * stage_bytes(NA, NB) + pieces(NA, NB) * 8 * PIECE_BYTES + GROUP_BYTES + 1024;
-    cudaError_t e = cudaFuncSetAttribute(hessian_kernel<NA, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr int smem = stages_for(NA, NB, WHOLE) * stage_bytes(NA, NB) + drain_warps(WHOLE) * PIECE_BYTES + GROUP_BYTES + 1024;
+    cudaError_t e = cudaFuncSetAttribute(hessian_kernel<NA, NB, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
-    hessian_kernel<NA, NB><<<grid, THREADS, smem, s>>>(m, h, p);
+    hessian_kernel<NA, NB, WHOLE><<<grid, threads(WHOLE), smem, s>>>(m, h, p);
     return check_launch("hessian_kernel");
 }
 
@@ -519,13 +598,19 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     q.experts = (int)experts;
     q.d = (int)dim;
     const int64_t nt = (dim + BN - 1) / BN;
-    q.tiles = (int)(nt * (nt + 1));
+    // One product of few rows is bound by writing H: all of it as TMA tiles takes 290 us for 512 rows of 8 experts and d
+    // 7168 (222 us at the write rate of a fill), blocks above the diagonal and their mirror images 330 us.  From about 256
+    // rows an expert the products of half the tiles weigh more (4096 rows: 570 us in halves, 610 us for 2048 rows whole).
+    // x x^T comes out symmetric by itself, its sums being the same products in the same order on both sides.
+    const bool whole = na == 0 && rows <= 128 * experts;
+    q.n_tiles = (int)nt;
+    q.tiles = (int)(whole ? (dim + BM - 1) / BM * nt : nt * (nt + 1));
     q.idesc = idesc_f16(!fp16, true, true, BM, BN);
     q.add = add != 0;
     const bool vec = ((uintptr_t)H & 15) == 0 && ldh % 4 == 0 && h_stride % 4 == 0;
+    q.vec = vec && dim % 4 == 0 && ldh < ((int64_t)1 << 36) && h_stride < ((int64_t)1 << 36);
     CUtensorMap map_h{};
-    q.tma = vec && (dim == 1 || ldh >= dim) && ldh < ((int64_t)1 << 36) && h_stride < ((int64_t)1 << 36);
-    if (q.tma) {
+    if (q.vec && whole) {
         const int64_t hd[3] = {dim, dim, experts}, hs[2] = {ldh * 4, (experts > 1 ? h_stride : ldh * dim) * 4};
         const int hb[3] = {32, 32, 1};
         if (int rc = encode_tiles(&map_h, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, H, hd, hs, hb, what)) return rc;
@@ -534,8 +619,9 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     if (int rc = sm_count(&sms)) return rc;
     const int64_t tiles = (int64_t)q.tiles * experts;
     const int g = (int)(tiles < sms ? tiles : sms);
-    if (na == 0) return launch_hessian<1, 1>(maps, map_h, q, g, s);
-    if (na == 1) return launch_hessian<1, 3>(maps, map_h, q, g, s);
-    if (na == 2) return launch_hessian<2, 3>(maps, map_h, q, g, s);
-    return launch_hessian<3, 3>(maps, map_h, q, g, s);
+    if (whole) return launch_hessian<1, 1, true>(maps, map_h, q, g, s);
+    if (na == 0) return launch_hessian<1, 1, false>(maps, map_h, q, g, s);
+    if (na == 1) return launch_hessian<1, 3, false>(maps, map_h, q, g, s);
+    if (na == 2) return launch_hessian<2, 3, false>(maps, map_h, q, g, s);
+    return launch_hessian<3, 3, false>(maps, map_h, q, g, s);
 }
