@@ -12,93 +12,16 @@
 // bits of x and y.  Products are summed in fp32, the output transform runs in
 // fp32, and y is rounded once.
 //
-// Decode.  State i of a tile is the 16-bit window of its cyclic bit stream
-// that ends with symbol i (kq_unpack_trellis_states).  Lane m of a warp owns
-// symbols 8m .. 8m+7: its eight windows lie in 7K + 16 consecutive bits, three
-// (K > 6: four) 32-bit words.  Trellis position 8m + s is row 2(m%4) + (s&1) +
-// 8((s>>1)&1), column m/4 + 8(s>>2) of the tile, so neighbouring symbols are
-// neighbouring rows: a packed pair along the contraction axis.
-// Labels: MCG is computed (a multiply, a logic op, half an add); E4M3 and
-// binary16 tables are looked up in shared memory, where 32 random lookups
-// meet about 3.5-fold bank conflicts.
+// Up to a mean of MEAN rows an expert, the payload is decoded in registers next
+// to the product (kq_trellis_few.cuh) and partial sums over ranges of k are
+// added up by the output transform.  With more rows it is decoded once, to
+// binary16 in the workspace, and the tensor-core product with the rotation in
+// its epilogue reads that (kq_expert_rotated.cu).
 #include "kq_expert_rows.cuh"
+#include "kq_trellis_decode.cuh"
 
 namespace kq {
 namespace {
-
-enum { DEC_MCG, DEC_E4M3, DEC_F16 };
-constexpr int kBlock = 128;
-
-__host__ __device__ constexpr int table_bytes(int dec) { return dec == DEC_MCG ? 0 : dec == DEC_E4M3 ? 65536 : 131072; }
-
-// Whole block: the label table into shared memory.
-template <int DEC>
-__device__ __forceinline__ void load_table(const void* table, uint8_t* smem) {
-    if constexpr (DEC != DEC_MCG) {
-        const uint4* src = static_cast<const uint4*>(table);
-        for (int i = threadIdx.x; i < table_bytes(DEC) / 16; i += blockDim.x) reinterpret_cast<uint4*>(smem)[i] = __ldg(src + i);
-    }
-}
-
-// Labels of two states as packed binary16.
-template <int DEC>
-__device__ __forceinline__ uint32_t label_pair(uint32_t s0, uint32_t s1, const uint8_t* table) {
-    if constexpr (DEC == DEC_MCG) {
-        const uint32_t y0 = ((s0 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
-        const uint32_t y1 = ((s1 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
-        const uint32_t lo = __byte_perm(y0, y1, 0x5410), hi = __byte_perm(y0, y1, 0x7632);
-        const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&hi));
-        return *reinterpret_cast<const uint32_t*>(&v);
-    } else if constexpr (DEC == DEC_E4M3) {
-        const uint16_t b = (uint16_t)(table[s0] | (table[s1] << 8));
-        uint32_t v;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v) : "h"(b));
-        return v;
-    } else {
-        const uint16_t* t = reinterpret_cast<const uint16_t*>(table);
-        return (uint32_t)t[s0] | ((uint32_t)t[s1] << 16);
-    }
-}
-
-// A tile's words, held by the warp: lane l has words l and (K > 4) l + 32, each 32 bits of the stream, first bit on top.
-template <int K>
-struct TileWords {
-    uint32_t w[K > 4 ? 2 : 1];
-    __device__ __forceinline__ void load(const uint32_t* tile, int lane) {
-        if (K >= 4 || lane < 8 * K) w[0] = __ldg(tile + lane);
-        if constexpr (K > 4)
-            if (lane + 32 < 8 * K) w[1] = __ldg(tile + 32 + lane);
-    }
-    __device__ __forceinline__ uint32_t at(int i) const {       // word i mod 8K, i in -8K .. 8K
-        i = i < 0 ? i + 8 * K : i >= 8 * K ? i - 8 * K : i;
-        const uint32_t a = __shfl_sync(0xFFFFFFFFu, w[0], i & 31);
-        if constexpr (K > 4) {
-            const uint32_t b = __shfl_sync(0xFFFFFFFFu, w[1], i & 31);
-            return i >= 32 ? b : a;
-        }
-        return a;
-    }
-};
-
-// The four fragment pairs of this lane: rows (2q, 2q+1) and (2q+8, 2q+9) of column m/4, then of column m/4 + 8.
-template <int K, int DEC>
-__device__ __forceinline__ void decode_tile(const TileWords<K>& t, int lane, const uint8_t* table, uint32_t (&frag)[4]) {
-    const int end = 8 * K * (lane + 1), wi = end >> 5, off = end & 31;
-    const uint32_t c = t.at(wi), b = t.at(wi - 1), a = t.at(wi - 2);
-    // Stream bits [end-32, end), the 32 before them, and (K > 6) the 32 before those.
-    const uint32_t w0 = __funnelshift_l(c, b, off), w1 = __funnelshift_l(b, a, off);
-    uint32_t w2 = 0;
-    if constexpr (K > 6) w2 = __funnelshift_l(a, t.at(wi - 3), off);
-    uint32_t s[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int sh = (7 - i) * K;
-        s[i] = (sh + 16 <= 32 ? w0 >> sh : sh < 32 ? __funnelshift_r(w0, w1, sh) : sh + 16 <= 64 ? w1 >> (sh - 32)
-                                                                                               : __funnelshift_r(w1, w2, sh - 32)) & 0xFFFFu;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) frag[i] = label_pair<DEC>(s[2 * i], s[2 * i + 1], table);
-}
 
 // Expert of one row, or -1: the block looks at all offsets at once.
 __device__ __forceinline__ int expert_of_row(const int64_t* offsets, int experts, int rows, int row, int* slot) {
@@ -164,6 +87,36 @@ __global__ void __launch_bounds__(256) rotate_in_kernel(const T* __restrict__ x,
     if (threadIdx.x == 0) scale[row] = ldexpf(1.f, -ex);
 }
 
+// y = had(sum of the partial sums) * svh * 2^-s; a warp a Hadamard block of one row.  Rows of no expert: zeros in a fresh
+// output.
+template <typename T>
+__global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict__ partial, int splits, const float* __restrict__ scale,
+                                                         const __half* __restrict__ svh, int64_t svh_stride,
+                                                         const int64_t* __restrict__ offsets, int rows, int experts, int n,
+                                                         T* __restrict__ y, int64_t ldy, bool zero_rest) {
+    __shared__ int slot;
+    const int row = blockIdx.x, lane = threadIdx.x & 31, blk = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int e = expert_of_row(offsets, experts, rows, row, &slot);
+    if (blk >= n / kBlock || (e < 0 && !zero_rest)) return;
+    const int j = blk * kBlock + lane * 4;
+    T* o = y + (int64_t)row * ldy + j;
+    if (e < 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = from_f<T>(0.f);
+        return;
+    }
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float4 q = __ldcs(reinterpret_cast<const float4*>(partial + ((int64_t)s * rows + row) * n + j));
+        v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+    }
+    had128_warp(v, lane);
+    const float f = scale[row] * 0.08838834764831845f;      // 1 / sqrt(128)
+    const __half* sv = svh + e * svh_stride + j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_f<T>(v[i] * f * __half2float(sv[i]));
+}
+
 // What_e as binary16 [n][k].  A block decodes 128 columns x 64 rows at a time through shared memory, so that it
 // reads 8 tiles' words in a row and writes whole 128-byte lines.
 constexpr int DN = 128, DK = 64, DPAD = 72;            // row stride of the staged tile in halves
@@ -226,16 +179,25 @@ __global__ void zero_rest_kernel(const int64_t* offsets, int experts, int rows, 
     }
 }
 
+constexpr int kFewMean = 64;
+
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
-struct Layout { int64_t xr, scale, w, bytes; };
+// Few rows: k is split until every SM has several items (64 or 32 columns of one row tile and range of k).
+struct Plan { bool few, wide; int splits; int64_t xr, scale, rest, bytes; };
 
-Layout layout(const kq_trellis_product& p) {
-    Layout l;
-    l.xr = 0;
+Plan plan(const kq_trellis_product& p, int sms) {
+    Plan l{};
+    const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
+    l.few = p.rows <= kFewMean * busy;
+    l.wide = p.rows > 8 * busy;
+    const int64_t tile = l.wide ? kFewRows : 16, tiles = busy + (p.rows - busy) / tile;
+    const int64_t items = tiles * (p.n / (l.wide ? 32 : 64)), kt = p.k / 16;
+    l.splits = 1;
+    while (l.splits < 32 && items * l.splits < 8 * sms && kt / (l.splits * 2) >= 8) l.splits *= 2;
     l.scale = align128(p.rows * p.k * 2);
-    l.w = l.scale + align128(p.rows * 4);
-    l.bytes = l.w + p.experts * p.k * p.n * 2;
+    l.rest = l.scale + align128(p.rows * 4);
+    l.bytes = l.rest + (l.few ? (int64_t)l.splits * p.rows * p.n * 4 : p.experts * p.k * p.n * 2);
     return l;
 }
 
@@ -303,7 +265,9 @@ int rotate_in(const kq_trellis_product& p, __half* xr, float* scale, cudaStream_
 
 extern "C" size_t kq_trellis_linear_workspace_bytes(const kq_trellis_product* p) {
     if (!p || kq::check_trellis(*p, "kq_trellis_linear_workspace_bytes") || p->rows == 0) return 0;
-    return (size_t)kq::layout(*p).bytes;
+    int sms;
+    if (kq::sm_count(&sms)) return 0;
+    return (size_t)kq::plan(*p, sms).bytes;
 }
 
 extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, size_t workspace_bytes, void* stream) {
@@ -321,15 +285,36 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         set_error("%s: trellis and table need 16-byte alignment", what);
         return KQ_ERR_ALIGN;
     }
-    const Layout l = layout(p);
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    const Plan l = plan(p, sms);
     if (!workspace || workspace_bytes < (size_t)l.bytes) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    __half *xr = reinterpret_cast<__half*>(ws + l.xr), *w = reinterpret_cast<__half*>(ws + l.w);
+    __half* xr = reinterpret_cast<__half*>(ws + l.xr);
     float* scale = reinterpret_cast<float*>(ws + l.scale);
     const bool bf16 = p.dtype == KQ_BF16;
     if (int rc = bf16 ? rotate_in<__nv_bfloat16>(p, xr, scale, s) : rotate_in<__half>(p, xr, scale, s)) return rc;
+    if (l.few) {
+        float* partial = reinterpret_cast<float*>(ws + l.rest);
+        const FewTrellis f{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr), partial,
+                           (int)p.rows, (int)p.experts, (int)p.k, (int)p.n, l.splits};
+        const int dec = p.codebook == KQ_CB_MCG ? DEC_MCG : p.codebook == KQ_CB_SQG ? DEC_E4M3 : DEC_F16;
+        int rc = p.bits <= 2 ? few_trellis_k12(f, p.bits, dec, l.wide, s) : p.bits <= 4 ? few_trellis_k34(f, p.bits, dec, l.wide, s)
+               : p.bits <= 6 ? few_trellis_k56(f, p.bits, dec, l.wide, s) : few_trellis_k78(f, p.bits, dec, l.wide, s);
+        if (rc) return rc;
+        const dim3 grid((unsigned)p.rows, (unsigned)((p.n / kBlock + 7) / 8));
+        const __half* svh = reinterpret_cast<const __half*>(p.svh);
+        if (bf16)
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.splits, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+                                                   (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy, p.zero_rest != 0);
+        else
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.splits, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+                                                   (int)p.n, static_cast<__half*>(p.y), p.ldy, p.zero_rest != 0);
+        return check_launch("rotate_out_kernel");
+    }
+    __half* w = reinterpret_cast<__half*>(ws + l.rest);
     if (p.zero_rest && p.offsets) {
         const int grid = (int)(p.rows < 1024 ? p.rows : 1024);
         if (bf16) zero_rest_kernel<<<grid, 256, 0, s>>>(p.offsets, (int)p.experts, (int)p.rows, (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy);
