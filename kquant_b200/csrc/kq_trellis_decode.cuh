@@ -88,17 +88,28 @@ __device__ __forceinline__ void decode_tile(const TileWords<K>& t, int lane, con
     for (int i = 0; i < 4; ++i) frag[i] = label_pair<DEC>(s[2 * i], s[2 * i + 1], table);
 }
 
-// Rows product of few rows: partial sums [splits][rows][n] of x' What over ranges of k.
+// Rows product of few rows.  The work is row tiles x strips of columns x k tiles, in that order; CTA c takes the k tiles
+// c * per .. of it, so a strip's sums come in up to `parts` parts, counted from the CTA that holds its first k tile:
+// partial [parts][rows][n].
 struct FewTrellis {
     const uint32_t* trellis;
     const void* table;
     const int64_t* offsets;
     const uint16_t* xr;        // [rows][k] binary16
     float* partial;
-    int rows, experts, k, n, splits;
+    int rows, experts, k, n, parts;
 };
 
+// k tiles of a CTA: an even share of `work` for `ctas`, at least 32 (a step of every warp or more), and enough that no strip is in
+// more than `parts` parts.
+__host__ __device__ inline int64_t few_share(int64_t work, int ctas, int kt, int parts) {
+    const int64_t even = (work + ctas - 1) / ctas, least = (kt + parts - 2) / (parts - 1);
+    const int64_t m = even > least ? even : least;
+    return m > 32 ? m : 32;
+}
+
 constexpr int kFewRows = 64;   // rows of the larger row tile; the smaller one has 16
+constexpr int few_columns(bool wide) { return wide ? 32 : 64; }     // of a strip
 
 // Launches for the rates of one source file each; `wide`: 64 rows a tile, else 16.
 int few_trellis_k12(const FewTrellis& p, int bits, int dec, bool wide, cudaStream_t s);

@@ -7,18 +7,20 @@
 // products of 64 rows take half of its time even on mma.sync), at three bits:
 // label lookups in shared memory for the tables, integer arithmetic for MCG.
 //
-// An item is one row tile (16 or 64 rows of an expert), a strip of columns and
-// a range of k; a CTA's eight warps take the k tiles of the range in turn, each
-// with its words two steps ahead in registers, and add up in shared memory in
-// a fixed order.  Items are dealt to a persistent grid of two CTAs an SM, whose
-// ends hide each other.
+// The work is dealt to a persistent grid of two CTAs an SM in equal shares of
+// k tiles, wherever strips of columns end: with whole strips the last round
+// of CTAs left SMs idle, with short items each began with a wait for memory.
+// A CTA's warps take the k tiles of a share in turn, each with its words two
+// steps ahead in registers, and add up in shared memory in a fixed order; the
+// output transform adds up a strip's shares.
 #pragma once
 #include "kq_trellis_decode.cuh"
 
 namespace kq {
 namespace {
 
-constexpr int kFewWarps = 8;
+// Warps of a CTA: 24 an SM hide the lookups' latency where the registers allow it (16 rows), 16 with 64 rows' sums.
+template <int RT> constexpr int few_warps() { return RT == 1 ? 12 : 8; }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -27,32 +29,35 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 // RT: row tiles of 16.
-template <int RT> constexpr int few_strip() { return RT == 1 ? 4 : 2; }     // tiles of 16 columns a warp holds
+template <int RT> constexpr int few_strip() { return few_columns(RT > 1) / 16; }     // tiles of 16 columns a warp holds
 template <int RT> constexpr int few_part() { return RT * 16 * (few_strip<RT>() * 16 + 8); }   // floats of a warp's sums, padded rows
 template <int DEC, int RT> constexpr int few_smem() {
-    return table_bytes(DEC) + kFewWarps / 2 * few_part<RT>() * 4 + (kMaxExperts + 4) * 4;
+    return table_bytes(DEC) + few_warps<RT>() / 2 * few_part<RT>() * 4 + (kMaxExperts + 4) * 4;
 }
 
 template <int K, int DEC, int RT>
-__global__ void __launch_bounds__(kFewWarps * 32, DEC == DEC_F16 ? 1 : 2) few_trellis_kernel(const FewTrellis p) {
-    constexpr int NT = few_strip<RT>(), COLS = NT * 16, LD = COLS + 8;
+__global__ void __launch_bounds__(few_warps<RT>() * 32, DEC == DEC_F16 ? 1 : 2) few_trellis_kernel(const FewTrellis p) {
+    constexpr int NT = few_strip<RT>(), COLS = NT * 16, LD = COLS + 8, WARPS = few_warps<RT>();
     extern __shared__ __align__(16) uint8_t smem[];
     float* sums = reinterpret_cast<float*>(smem + table_bytes(DEC));
-    int* cum = reinterpret_cast<int*>(sums + kFewWarps / 2 * few_part<RT>());
-    static_assert(kFewWarps / 2 * few_part<RT>() >= 2 * kMaxExperts, "the scan borrows the sums");
+    int* cum = reinterpret_cast<int*>(sums + WARPS / 2 * few_part<RT>());
+    static_assert(WARPS / 2 * few_part<RT>() >= 2 * kMaxExperts, "the scan borrows the sums");
     int* first = reinterpret_cast<int*>(sums);
     load_table<DEC>(p.table, smem);
     scan_groups(p.offsets, p.experts, p.rows, RT * 16, first, first + kMaxExperts, cum);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3;
     const int kt = p.k / 16, nt = p.n / 16, strips = p.n / COLS;
-    const int64_t items = (int64_t)cum[p.experts] * p.splits * strips;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int strip = (int)(item % strips), rest = (int)(item / strips), split = rest % p.splits, t = rest / p.splits;
+    const int64_t work = (int64_t)cum[p.experts] * strips * kt, per = few_share(work, gridDim.x, kt, p.parts);
+    const int64_t stop = min((int64_t)(blockIdx.x + 1) * per, work);
+    for (int64_t at = blockIdx.x * per; at < stop;) {
+        const int64_t item = at / kt, first_cta = item * kt / per;
+        const int strip = (int)(item % strips), t = (int)(item / strips), part = (int)(blockIdx.x - first_cta);
         const int e = expert_of(cum, p.experts, t), r0 = (t - cum[e]) * RT * 16;
         int lo, n_e;
         group_of(p.offsets, e, p.rows, lo, n_e);
         const int row0 = lo + r0, count = min(n_e - r0, RT * 16);
-        const int ka = (int)((int64_t)kt * split / p.splits), kb = (int)((int64_t)kt * (split + 1) / p.splits);
+        const int ka = (int)(at - item * kt), kb = (int)min((int64_t)kt, stop - item * kt);
+        at += kb - ka;
         const uint32_t* base = p.trellis + ((int64_t)e * kt * nt + strip * NT) * 8 * K;
         float acc[RT][NT][2][4] = {};
         TileWords<K> ahead[2][NT];
@@ -62,7 +67,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, DEC == DEC_F16 ? 1 : 2) few_tr
             for (int j = 0; j < NT; ++j) w[j].load(base + ((int64_t)kk * nt + j) * 8 * K, lane);
         };
         fetch(ka + warp, ahead[0]);
-        fetch(ka + warp + kFewWarps, ahead[1]);
+        fetch(ka + warp + WARPS, ahead[1]);
         const uint16_t* xp = p.xr + (int64_t)(row0 + (lane >> 2)) * p.k + 2 * q;
         auto step = [&](int kk, TileWords<K> (&w)[NT]) {
             uint32_t a[RT][4];
@@ -85,14 +90,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, DEC == DEC_F16 ? 1 : 2) few_tr
                     mma16816(acc[r][j][1], a[r], f[2], f[3]);
                 }
             }
-            fetch(kk + 2 * kFewWarps, w);
+            fetch(kk + 2 * WARPS, w);
         };
-        for (int kk = ka + warp; kk < kb; kk += 2 * kFewWarps) {
+        for (int kk = ka + warp; kk < kb; kk += 2 * WARPS) {
             step(kk, ahead[0]);
-            if (kk + kFewWarps < kb) step(kk + kFewWarps, ahead[1]);
+            if (kk + WARPS < kb) step(kk + WARPS, ahead[1]);
         }
-        // Warps 4..7 hand over, warps 0..3 add theirs, and the block adds up the four.
-        float* mine = sums + (warp & 3) * few_part<RT>();
+        // The upper half of the warps hand over, the lower half add theirs, and the block adds up the rest.
+        float* mine = sums + (warp % (WARPS / 2)) * few_part<RT>();
         auto each = [&](auto f) {
 #pragma unroll
             for (int r = 0; r < RT; ++r)
@@ -106,16 +111,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, DEC == DEC_F16 ? 1 : 2) few_tr
                               acc[r][j][h][2 * v], acc[r][j][h][2 * v + 1]);
         };
         __syncthreads();                         // the last item's sums are read
-        if (warp >= 4) each([](float2* s, float x, float y) { *s = make_float2(x, y); });
+        if (warp >= WARPS / 2) each([](float2* s, float x, float y) { *s = make_float2(x, y); });
         __syncthreads();
-        if (warp < 4) each([](float2* s, float x, float y) { const float2 o = *s; *s = make_float2(x + o.x, y + o.y); });
+        if (warp < WARPS / 2) each([](float2* s, float x, float y) { const float2 o = *s; *s = make_float2(x + o.x, y + o.y); });
         __syncthreads();
-        for (int i = threadIdx.x; i < count * COLS; i += kFewWarps * 32) {
+        for (int i = threadIdx.x; i < count * COLS; i += WARPS * 32) {
             const int r = i / COLS, c = i % COLS;
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) v += sums[w * few_part<RT>() + r * LD + c];
-            p.partial[((int64_t)split * p.rows + row0 + r) * p.n + strip * COLS + c] = v;
+            for (int w = 0; w < WARPS / 2; ++w) v += sums[w * few_part<RT>() + r * LD + c];
+            p.partial[((int64_t)part * p.rows + row0 + r) * p.n + strip * COLS + c] = v;
         }
     }
 }
@@ -128,7 +133,7 @@ int launch_few(const FewTrellis& p, cudaStream_t s) {
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    kernel<<<sms * (DEC == DEC_F16 ? 1 : 2), kFewWarps * 32, smem, s>>>(p);
+    kernel<<<sms * (DEC == DEC_F16 ? 1 : 2), few_warps<RT>() * 32, smem, s>>>(p);
     return check_launch("few_trellis_kernel");
 }
 

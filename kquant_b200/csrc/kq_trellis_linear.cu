@@ -23,17 +23,29 @@
 namespace kq {
 namespace {
 
-// Expert of one row, or -1: the block looks at all offsets at once.
-__device__ __forceinline__ int expert_of_row(const int64_t* offsets, int experts, int rows, int row, int* slot) {
-    if (threadIdx.x == 0) *slot = -1;
+// Place of one row: its expert or -1, and, counting row tiles of `tile` rows, its own and all of them.  The whole block looks
+// at all offsets at once.
+struct Place { int e, tile, tiles; };
+
+__device__ __forceinline__ Place place_of_row(const int64_t* offsets, int experts, int rows, int row, int tile) {
+    __shared__ int e_of, lo_of, before, all;
+    if (threadIdx.x == 0) { e_of = -1; lo_of = 0; before = 0; all = 0; }
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += blockDim.x) {
         int lo, n;
         group_of(offsets, e, rows, lo, n);
-        if (row >= lo && row < lo + n) *slot = e;
+        if (!n) continue;
+        const int t = (n + tile - 1) / tile;
+        atomicAdd(&all, t);
+        if (row >= lo && row < lo + n) {
+            e_of = e;
+            lo_of = lo;
+        } else if (lo + n <= row) {
+            atomicAdd(&before, t);
+        }
     }
     __syncthreads();
-    return *slot;
+    return Place{e_of, before + (row - lo_of) / tile, all};
 }
 
 __device__ __forceinline__ void had128_warp(float (&v)[4], int lane) {
@@ -48,26 +60,77 @@ __device__ __forceinline__ void had128_warp(float (&v)[4], int lane) {
         }
 }
 
-// x' = had(x * suh) * 2^s in binary16 and 2^-s; one block a row, a warp a Hadamard block.
+// 4 consecutive 16-bit values, 8 bytes at once where the address allows it.
 template <typename T>
-__global__ void __launch_bounds__(256) rotate_in_kernel(const T* __restrict__ x, int64_t ldx, const __half* __restrict__ suh,
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+    if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+        const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+        const T* h = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_f<T>(h[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_f<T>(p[i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+    if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+        uint2 q;
+        T* h = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = from_f<T>(v[i]);
+        *reinterpret_cast<uint2*>(p) = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = from_f<T>(v[i]);
+    }
+}
+
+// x' = had(x * suh) * 2^s in binary16 and 2^-s; one block a row, a warp a Hadamard block of 128 channels.  The row's
+// largest product decides s, so it is held in registers between the two (up to HELD blocks a warp; longer rows are read
+// twice).
+template <typename T>
+__global__ void __launch_bounds__(512) rotate_in_kernel(const T* __restrict__ x, int64_t ldx, const __half* __restrict__ suh,
                                                         int64_t suh_stride, const int64_t* __restrict__ offsets, int rows,
                                                         int experts, int k, __half* __restrict__ xr, float* __restrict__ scale) {
-    __shared__ int slot;
-    __shared__ float most[8];
-    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int e = expert_of_row(offsets, experts, rows, row, &slot);
+    constexpr int WARPS = 16, HELD = 4;
+    __shared__ float most[WARPS];
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = k / kBlock;
+    const int e = place_of_row(offsets, experts, rows, row, 1).e;
     if (e < 0) return;
     const T* xp = x + (int64_t)row * ldx;
     const __half* sp = suh + e * suh_stride;
+    auto fetch = [&](int blk, float (&v)[4]) {
+        float s[4];
+        load4(xp + blk * kBlock + lane * 4, v);
+        load4(sp + blk * kBlock + lane * 4, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= s[i];
+    };
+    float held[HELD][4];
     float m = 0.f;
-    for (int i = threadIdx.x; i < k; i += 256) m = fmaxf(m, fabsf(to_f<T>(xp[i]) * __half2float(sp[i])));
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        if (warp + h * WARPS < blocks) {
+            fetch(warp + h * WARPS, held[h]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(held[h][i]));
+        }
+    }
+    for (int blk = warp + HELD * WARPS; blk < blocks; blk += WARPS) {
+        float v[4];
+        fetch(blk, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     if (lane == 0) most[warp] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, most[i]);
+    for (int i = 0; i < WARPS; ++i) m = fmaxf(m, most[i]);
     // |had(v)| <= sqrt(128) max |v| < 2^4 max |v|: the exponent that brings it to at most 2^14.
     int ex = 0;
     if (m > 0.f && m < 1e38f) {
@@ -75,14 +138,18 @@ __global__ void __launch_bounds__(256) rotate_in_kernel(const T* __restrict__ x,
         ex = min(max(10 - ex, -120), 120);
     }
     const float up = ldexpf(0.08838834764831845f, ex);
-    for (int blk = warp; blk < k / kBlock; blk += 8) {
-        float v[4];
-        const int j = blk * kBlock + lane * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_f<T>(xp[j + i]) * __half2float(sp[j + i]);
+    auto emit = [&](int blk, float (&v)[4]) {
         had128_warp(v, lane);
         __half2 o[2] = {__floats2half2_rn(v[0] * up, v[1] * up), __floats2half2_rn(v[2] * up, v[3] * up)};
-        *reinterpret_cast<uint2*>(xr + (int64_t)row * k + j) = *reinterpret_cast<const uint2*>(o);
+        *reinterpret_cast<uint2*>(xr + (int64_t)row * k + blk * kBlock + lane * 4) = *reinterpret_cast<const uint2*>(o);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (warp + h * WARPS < blocks) emit(warp + h * WARPS, held[h]);
+    for (int blk = warp + HELD * WARPS; blk < blocks; blk += WARPS) {
+        float v[4];
+        fetch(blk, v);
+        emit(blk, v);
     }
     if (threadIdx.x == 0) scale[row] = ldexpf(1.f, -ex);
 }
@@ -90,13 +157,14 @@ __global__ void __launch_bounds__(256) rotate_in_kernel(const T* __restrict__ x,
 // y = had(sum of the partial sums) * svh * 2^-s; a warp a Hadamard block of one row.  Rows of no expert: zeros in a fresh
 // output.
 template <typename T>
-__global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict__ partial, int splits, const float* __restrict__ scale,
+__global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict__ partial, int parts, int ctas, int kt, bool wide,
+                                                         const float* __restrict__ scale,
                                                          const __half* __restrict__ svh, int64_t svh_stride,
                                                          const int64_t* __restrict__ offsets, int rows, int experts, int n,
                                                          T* __restrict__ y, int64_t ldy, bool zero_rest) {
-    __shared__ int slot;
     const int row = blockIdx.x, lane = threadIdx.x & 31, blk = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int e = expert_of_row(offsets, experts, rows, row, &slot);
+    const Place at = place_of_row(offsets, experts, rows, row, wide ? kFewRows : 16);
+    const int e = at.e;
     if (blk >= n / kBlock || (e < 0 && !zero_rest)) return;
     const int j = blk * kBlock + lane * 4;
     T* o = y + (int64_t)row * ldy + j;
@@ -106,15 +174,23 @@ __global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict
         return;
     }
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
+    // The parts of this lane's strip: from the CTA of its first k tile to that of its last.
+    const int strips = n / few_columns(wide);
+    const int64_t per = few_share((int64_t)at.tiles * strips * kt, ctas, kt, parts);
+    const int64_t first = ((int64_t)at.tile * strips + j / few_columns(wide)) * kt;
+    const int mine = (int)((first + kt - 1) / per - first / per) + 1;
+#pragma unroll 4
+    for (int s = 0; s < mine; ++s) {
         const float4 q = __ldcs(reinterpret_cast<const float4*>(partial + ((int64_t)s * rows + row) * n + j));
         v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
     }
     had128_warp(v, lane);
     const float f = scale[row] * 0.08838834764831845f;      // 1 / sqrt(128)
-    const __half* sv = svh + e * svh_stride + j;
+    float sv[4];
+    load4(svh + e * svh_stride + j, sv);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = from_f<T>(v[i] * f * __half2float(sv[i]));
+    for (int i = 0; i < 4; ++i) v[i] *= f * sv[i];
+    store4(o, v);
 }
 
 // What_e as binary16 [n][k].  A block decodes 128 columns x 64 rows at a time through shared memory, so that it
@@ -183,21 +259,22 @@ constexpr int kFewMean = 64;
 
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
-// Few rows: k is split until every SM has several items (64 or 32 columns of one row tile and range of k).
-struct Plan { bool few, wide; int splits; int64_t xr, scale, rest, bytes; };
+struct Plan { bool few, wide; int parts, ctas; int64_t scale, rest, bytes; };
 
 Plan plan(const kq_trellis_product& p, int sms) {
     Plan l{};
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
     l.few = p.rows <= kFewMean * busy;
     l.wide = p.rows > 8 * busy;
-    const int64_t tile = l.wide ? kFewRows : 16, tiles = busy + (p.rows - busy) / tile;
-    const int64_t items = tiles * (p.n / (l.wide ? 32 : 64)), kt = p.k / 16;
-    l.splits = 1;
-    while (l.splits < 32 && items * l.splits < 8 * sms && kt / (l.splits * 2) >= 8) l.splits *= 2;
+    l.ctas = sms * (p.codebook == KQ_CB_LABELS ? 1 : 2);      // a table of 128 KB leaves room for one
+    // Parts of a strip: what an even share of a single row tile makes, within 256 MB (two at least).
+    const int64_t kt = p.k / 16, strips = p.n / few_columns(l.wide), one = p.rows * p.n * 4;
+    const int64_t share = strips * kt / l.ctas > 32 ? strips * kt / l.ctas : 32, fit = ((int64_t)1 << 28) / one;
+    const int64_t most = kt / share + 2;
+    l.parts = (int)(most < fit ? most : fit < 2 ? 2 : fit);
     l.scale = align128(p.rows * p.k * 2);
     l.rest = l.scale + align128(p.rows * 4);
-    l.bytes = l.rest + (l.few ? (int64_t)l.splits * p.rows * p.n * 4 : p.experts * p.k * p.n * 2);
+    l.bytes = l.rest + (l.few ? (int64_t)l.parts * one : p.experts * p.k * p.n * 2);
     return l;
 }
 
@@ -255,7 +332,7 @@ int decode_all(const kq_trellis_product& p, __half* out, cudaStream_t s) {
 
 template <typename T>
 int rotate_in(const kq_trellis_product& p, __half* xr, float* scale, cudaStream_t s) {
-    rotate_in_kernel<T><<<(unsigned)p.rows, 256, 0, s>>>(static_cast<const T*>(p.x), p.ldx, reinterpret_cast<const __half*>(p.suh),
+    rotate_in_kernel<T><<<(unsigned)p.rows, 512, 0, s>>>(static_cast<const T*>(p.x), p.ldx, reinterpret_cast<const __half*>(p.suh),
                                                          p.suh_stride_e, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, xr, scale);
     return check_launch("rotate_in_kernel");
 }
@@ -292,14 +369,14 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    __half* xr = reinterpret_cast<__half*>(ws + l.xr);
+    __half* xr = reinterpret_cast<__half*>(ws);
     float* scale = reinterpret_cast<float*>(ws + l.scale);
     const bool bf16 = p.dtype == KQ_BF16;
     if (int rc = bf16 ? rotate_in<__nv_bfloat16>(p, xr, scale, s) : rotate_in<__half>(p, xr, scale, s)) return rc;
     if (l.few) {
         float* partial = reinterpret_cast<float*>(ws + l.rest);
         const FewTrellis f{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr), partial,
-                           (int)p.rows, (int)p.experts, (int)p.k, (int)p.n, l.splits};
+                           (int)p.rows, (int)p.experts, (int)p.k, (int)p.n, l.parts};
         const int dec = p.codebook == KQ_CB_MCG ? DEC_MCG : p.codebook == KQ_CB_SQG ? DEC_E4M3 : DEC_F16;
         int rc = p.bits <= 2 ? few_trellis_k12(f, p.bits, dec, l.wide, s) : p.bits <= 4 ? few_trellis_k34(f, p.bits, dec, l.wide, s)
                : p.bits <= 6 ? few_trellis_k56(f, p.bits, dec, l.wide, s) : few_trellis_k78(f, p.bits, dec, l.wide, s);
@@ -307,10 +384,10 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         const dim3 grid((unsigned)p.rows, (unsigned)((p.n / kBlock + 7) / 8));
         const __half* svh = reinterpret_cast<const __half*>(p.svh);
         if (bf16)
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.splits, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, l.ctas, (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
                                                    (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy, p.zero_rest != 0);
         else
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.splits, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, l.ctas, (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
                                                    (int)p.n, static_cast<__half*>(p.y), p.ldy, p.zero_rest != 0);
         return check_launch("rotate_out_kernel");
     }
