@@ -34,8 +34,8 @@ __device__ __forceinline__ uint32_t label_pair(uint32_t s0, uint32_t s1, const u
     if constexpr (DEC == DEC_MCG) {
         const uint32_t y0 = ((s0 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
         const uint32_t y1 = ((s1 * 0xCBAC1FEDu) & 0x8fff8fffu) ^ 0x3b603b60u;
-        const uint32_t lo = __byte_perm(y0, y1, 0x5410), hi = __byte_perm(y0, y1, 0x7632);
-        const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&hi));
+        const __half2 h0 = *reinterpret_cast<const __half2*>(&y0), h1 = *reinterpret_cast<const __half2*>(&y1);
+        const __half2 v = __halves2half2(__hadd(__low2half(h0), __high2half(h0)), __hadd(__low2half(h1), __high2half(h1)));
         return *reinterpret_cast<const uint32_t*>(&v);
     } else if constexpr (DEC == DEC_E4M3) {
         const uint16_t b = (uint16_t)(table[s0] | (table[s1] << 8));
@@ -77,12 +77,16 @@ __device__ __forceinline__ void decode_tile(const TileWords<K>& t, int lane, con
     const uint32_t w0 = __funnelshift_l(c, b, off), w1 = __funnelshift_l(b, a, off);
     uint32_t w2 = 0;
     if constexpr (K > 6) w2 = __funnelshift_l(a, t.at(wi - 3), off);
+    // A window inside one word is shifted to its top and down again: the first shift runs as a multiply beside the ALU,
+    // which is the busy pipe (a mask would be a second ALU operation).
     uint32_t s[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int sh = (7 - i) * K;
-        s[i] = (sh + 16 <= 32 ? w0 >> sh : sh < 32 ? __funnelshift_r(w0, w1, sh) : sh + 16 <= 64 ? w1 >> (sh - 32)
-                                                                                               : __funnelshift_r(w1, w2, sh - 32)) & 0xFFFFu;
+        if (sh <= 16) s[i] = (w0 << (16 - sh)) >> 16;
+        else if (sh < 32) s[i] = __funnelshift_r(w0, w1, sh) & 0xFFFFu;
+        else if (sh <= 48) s[i] = (w1 << (48 - sh)) >> 16;
+        else s[i] = __funnelshift_r(w1, w2, sh - 32) & 0xFFFFu;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) frag[i] = label_pair<DEC>(s[2 * i], s[2 * i + 1], table);

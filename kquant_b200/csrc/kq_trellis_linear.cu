@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict
     store4(o, v);
 }
 
-// What_e as binary16 [n][k].  A block decodes 128 columns x 64 rows at a time through shared memory, so that it
-// reads 8 tiles' words in a row and writes whole 128-byte lines.
+// What_e as binary16 [n][k].  A block decodes 128 columns x 64 rows at a time, a warp 16 of the columns: the block reads
+// 8 tiles' words in a row, and a warp turns its 64 x 16 part in shared memory and writes whole 128-byte lines.
 constexpr int DN = 128, DK = 64, DPAD = 72;            // row stride of the staged tile in halves
 template <int K, int DEC>
 __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict__ trellis, const void* __restrict__ table,
@@ -204,26 +204,37 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
     __half* stage = reinterpret_cast<__half*>(smem + table_bytes(DEC));
     load_table<DEC>(table, smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nb = n / DN, kb = (k + DK - 1) / DK, per = nb * kb;
-    int last = -1, busy = 0;
-    for (int64_t i = blockIdx.x; i < (int64_t)per * experts; i += gridDim.x) {
-        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per);
-        if (e != last) {
-            int lo;
-            group_of(offsets, e, rows, lo, busy);
-            last = e;
+    const int nb = n / DN, kb = k / DK, per = nb * kb;
+    const int64_t tiles_n = n / 16, all = (int64_t)per * experts;
+    // The next block of a busy expert from `i` on (an expert without rows is not decoded), and its words.
+    int busy_e = -1, busy = 0;
+    auto seek = [&](int64_t i) {
+        for (; i < all; i += gridDim.x) {
+            const int e = (int)(i / per);
+            if (e != busy_e) {
+                int lo;
+                group_of(offsets, e, rows, lo, busy);
+                busy_e = e;
+            }
+            if (busy) break;
         }
-        if (!busy) continue;                           // an expert without rows is not decoded
-        const int n0 = (l % nb) * DN, k0 = (l / nb) * DK, kts = min(DK, k - k0) / 16;
-        __syncthreads();
-        TileWords<K> w[4];
-        const int64_t tiles_n = n / 16;
+        return i;
+    };
+    TileWords<K> w[4];
+    auto fetch = [&](int64_t i) {
+        if (i >= all) return;
+        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per), n0 = (l % nb) * DN, k0 = (l / nb) * DK;
 #pragma unroll
         for (int a = 0; a < 4; ++a)
-            if (a < kts) w[a].load(trellis + (((int64_t)e * (k / 16) + k0 / 16 + a) * tiles_n + n0 / 16 + warp) * 8 * K, lane);
+            w[a].load(trellis + (((int64_t)e * (k / 16) + k0 / 16 + a) * tiles_n + n0 / 16 + warp) * 8 * K, lane);
+    };
+    int64_t i = seek(blockIdx.x);
+    fetch(i);
+    __syncthreads();
+    while (i < all) {
+        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per), n0 = (l % nb) * DN, k0 = (l / nb) * DK;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            if (a >= kts) break;
             uint32_t f[4];
             decode_tile<K, DEC>(w[a], lane, smem, f);
             uint32_t* o = reinterpret_cast<uint32_t*>(stage + (warp * 16 + (lane >> 2)) * DPAD + a * 16 + 2 * (lane & 3));
@@ -232,13 +243,17 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
             o[8 * DPAD / 2] = f[2];
             o[8 * DPAD / 2 + 4] = f[3];
         }
-        __syncthreads();
-        const int lines = kts * 2;                     // 16-byte pieces of a row
-        for (int p = threadIdx.x; p < DN * lines; p += 256) {
-            const int r = p / lines, c = p % lines;
-            *reinterpret_cast<uint4*>(out + ((int64_t)e * n + n0 + r) * k + k0 + c * 8) =
-                *reinterpret_cast<const uint4*>(stage + r * DPAD + c * 8);
+        const int64_t next = seek(i + gridDim.x);
+        fetch(next);                                    // under the other warps' decoding and the stores
+        // Each warp's 16 columns are its own: they leave without the rest of the block.
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int r = warp * 16 + p * 4 + (lane >> 3), c = (lane & 7) * 8;
+            *reinterpret_cast<uint4*>(out + ((int64_t)e * n + n0 + r) * k + k0 + c) = *reinterpret_cast<const uint4*>(stage + r * DPAD + c);
         }
+        __syncwarp();
+        i = next;
     }
 }
 
@@ -302,7 +317,7 @@ int launch_decode(const kq_trellis_product& p, __half* out, cudaStream_t s) {
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    const int64_t items = (p.n / DN) * ((p.k + DK - 1) / DK) * p.experts;
+    const int64_t items = (p.n / DN) * (p.k / DK) * p.experts;
     const int per_sm = DEC == DEC_F16 ? 1 : DEC == DEC_E4M3 ? 2 : 8;
     const int grid = (int)(items < (int64_t)sms * per_sm ? items : (int64_t)sms * per_sm);
     decode_kernel<K, DEC><<<grid, 256, smem, s>>>(reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, (int)p.rows,
