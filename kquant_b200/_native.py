@@ -100,6 +100,8 @@ class KQError(RuntimeError):
 def load() -> ctypes.CDLL:
     """Load the library (no device work).  Raises if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -517,67 +519,66 @@ def reconstruct_rotated(wq: torch.Tensor, su: torch.Tensor, sv: torch.Tensor) ->
     return out
 
 
-def scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    """Workspace of one call, from torch's allocator: ordered with the call's stream, and inside a captured graph
-    the graph's own, so that graphs replayed side by side share none."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _call(device: torch.device, what: str, need: int, fn, *args) -> None:
+    """One entry point on ``device``'s current stream with ``need`` bytes of workspace: fn(*args, ws, need, stream).
+
+    The workspace comes from torch's allocator: ordered with the stream, and inside a captured graph the graph's own,
+    so that graphs replayed side by side share none.
+    """
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(device, what, need, fn, *args)
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    rc = fn(*args, ws.data_ptr() if need else None, need, stream)
+    if rc:
+        _check(rc, what)
 
 
 def expert_linear(p: ExpertProduct, device: torch.device) -> None:
-    with torch.cuda.device(device):
-        n = load().kq_expert_linear_workspace_bytes(p)
-        ws = scratch(n, device)
-        _check(load().kq_expert_linear(p, None if ws is None else ws.data_ptr(), n, _stream(device)), "kq_expert_linear")
+    L = load()
+    _call(device, "kq_expert_linear", L.kq_expert_linear_workspace_bytes(p), L.kq_expert_linear, p)
     stats.launches += 1
 
 
 def expert_linear_grad_z(p: ExpertProduct, dy: torch.Tensor, device: torch.device) -> None:
-    with torch.cuda.device(device):
-        n = load().kq_expert_linear_workspace_bytes(p)
-        ws = scratch(n, device)
-        _check(load().kq_expert_linear_grad_z(p, dy.data_ptr(), dy.stride(0), None if ws is None else ws.data_ptr(), n,
-                                              _stream(device)), "kq_expert_linear_grad_z")
+    L = load()
+    _call(device, "kq_expert_linear_grad_z", L.kq_expert_linear_workspace_bytes(p), L.kq_expert_linear_grad_z, p,
+          dy.data_ptr(), dy.stride(0))
     stats.launches += 1
 
 
 def expert_weight_grad(p: ExpertProduct, dz: torch.Tensor, dw: torch.Tensor, device: torch.device) -> None:
-    with torch.cuda.device(device):
-        n = load().kq_expert_weight_grad_workspace_bytes(p, dz.data_ptr(), dz.stride(0))
-        ws = scratch(n, device)
-        _check(load().kq_expert_weight_grad(p, dz.data_ptr(), dz.stride(0), dw.data_ptr(),
-                                            None if ws is None else ws.data_ptr(), n, _stream(device)),
-               "kq_expert_weight_grad")
+    L, at, ld = load(), dz.data_ptr(), dz.stride(0)
+    _call(device, "kq_expert_weight_grad", L.kq_expert_weight_grad_workspace_bytes(p, at, ld), L.kq_expert_weight_grad, p, at, ld,
+          dw.data_ptr())
     stats.launches += 1
 
 
 def expert_bias_grad(dz: torch.Tensor, offsets: torch.Tensor | None, db: torch.Tensor, dtype: int) -> None:
-    device = dz.device
-    with torch.cuda.device(device):
-        _check(load().kq_expert_bias_grad(dz.data_ptr(), dz.stride(0), None if offsets is None else offsets.data_ptr(),
-                                          dz.shape[0], dz.shape[1], db.shape[0], dtype, db.data_ptr(), db.stride(0),
-                                          _stream(device)), "kq_expert_bias_grad")
+    def fn(ws, need, stream):
+        return load().kq_expert_bias_grad(dz.data_ptr(), dz.stride(0), None if offsets is None else offsets.data_ptr(), dz.shape[0],
+                                          dz.shape[1], db.shape[0], dtype, db.data_ptr(), db.stride(0), stream)
+    _call(dz.device, "kq_expert_bias_grad", 0, fn)
     stats.launches += 1
 
 
 def accumulate_expert_hessians(x: torch.Tensor, dtype: int, index: torch.Tensor | None, w: torch.Tensor | None,
                                offsets: torch.Tensor, rows: int, H: torch.Tensor, add: bool, den: torch.Tensor) -> None:
-    device, E = H.device, H.shape[0]
-    with torch.cuda.device(device):
-        n = load().kq_expert_hessian_workspace_bytes(rows, x.shape[1], E, dtype, int(w is not None))
-        ws = scratch(n, device)
-        _check(load().kq_accumulate_expert_hessians(
-            x.data_ptr(), x.shape[0], x.shape[1], x.stride(0), dtype, None if index is None else index.data_ptr(),
-            None if w is None else w.data_ptr(), offsets.data_ptr(), rows, E, H.data_ptr(), H.stride(0), H.stride(1),
-            int(add), den.data_ptr(), None if ws is None else ws.data_ptr(), n, _stream(device)),
-            "kq_accumulate_expert_hessians")
+    L, E, (tokens, d) = load(), H.shape[0], x.shape
+    _call(H.device, "kq_accumulate_expert_hessians", L.kq_expert_hessian_workspace_bytes(rows, d, E, dtype, w is not None),
+          L.kq_accumulate_expert_hessians, x.data_ptr(), tokens, d, x.stride(0), dtype, None if index is None else index.data_ptr(),
+          None if w is None else w.data_ptr(), offsets.data_ptr(), rows, E, H.data_ptr(), H.stride(0), H.stride(1), add, den.data_ptr())
     stats.launches += 2
 
 
 def trellis_linear(p: TrellisProduct, device: torch.device) -> None:
-    with torch.cuda.device(device):
-        n = load().kq_trellis_linear_workspace_bytes(p)
-        ws = scratch(n, device)
-        _check(load().kq_trellis_linear(p, None if ws is None else ws.data_ptr(), n, _stream(device)), "kq_trellis_linear")
+    L = load()
+    _call(device, "kq_trellis_linear", L.kq_trellis_linear_workspace_bytes(p), L.kq_trellis_linear, p)
     stats.launches += 3
 
 

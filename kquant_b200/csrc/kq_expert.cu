@@ -187,6 +187,9 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t stages = 12 / (a_parts + 1), stage_bytes = (a_parts + 1) * SIDE_BYTES, b_at = a_parts * SIDE_BYTES;
 
     if (threadIdx.x == 0) {
+        tma_prefetch(&map_a);
+        tma_prefetch(&map_b);
+        tma_prefetch(&map_b_full);
         for (int s = 0; s < MAX_STAGES; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
@@ -445,13 +448,31 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 // 16-bit rows [batch][r][c] -> [batch][r][cols_out]: an operand whose base or
 // strides are not the multiples of 16 bytes that TMA needs is laid out once
 // more.  Columns c .. cols_out are not written (no tile map reaches them, or
-// only as output columns that are not stored).
-__global__ void relayout_kernel(const uint16_t* __restrict__ src, int64_t sb, int64_t sr, int64_t r, int64_t c,
-                                uint16_t* __restrict__ dst, int64_t db, int64_t cols_out, int64_t total) {
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t j = i % c, row = i / c;
-        const int64_t b = row / r, y = row - b * r;
-        dst[b * db + y * cols_out + j] = src[b * sb + y * sr + j];
+// only as output columns that are not stored).  Up to three copies in one
+// launch (blockIdx.y); a warp a row at a time.
+struct Copy {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t sb, sr, db, rows, r;       // rows = batch * r
+    int c, cols_out;
+};
+
+struct Copies {
+    Copy job[3];
+    int n = 0;
+};
+
+__global__ void __launch_bounds__(256) relayout_kernel(const Copies copies) {
+    const Copy& j = copies.job[blockIdx.y];
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < j.rows; row += (int64_t)gridDim.x * 8) {
+        const int64_t b = j.r == j.rows ? 0 : row / j.r, y = row - b * j.r;
+        const uint16_t* s = j.src + b * j.sb + y * j.sr;
+        uint16_t* d = j.dst + b * j.db + y * j.cols_out;       // rows start on 16 bytes
+        int c = lane * 2;
+#pragma unroll 4
+        for (; c + 1 < j.c; c += 64) *reinterpret_cast<uint32_t*>(d + c) = (uint32_t)s[c] | ((uint32_t)s[c + 1] << 16);
+        if (c < j.c) d[c] = s[c];
     }
 }
 
@@ -483,24 +504,28 @@ size_t relayout_bytes(const Operand& o) {
     return o.direct ? 0 : (size_t)(o.batch * o.r * round8(o.c)) * 2;
 }
 
-// `halves` = 2: the columns are two halves (gate and up) that each start on a 16-byte boundary in the copy.
-int relayout(Operand& o, uint16_t*& ws, int halves, cudaStream_t s) {
-    if (o.direct) return KQ_OK;
+// Adds the copies that `o` needs to `jobs` and points it at them.  `halves` = 2: the columns are two halves (gate and up)
+// that each start on a 16-byte boundary in the copy.
+void relayout(Operand& o, uint16_t*& ws, int halves, Copies& jobs) {
+    if (o.direct) return;
     const int64_t part = o.c / halves, pad = round8(part), cols = pad * halves;
-    for (int h = 0; h < halves; ++h) {
-        const int64_t total = o.batch * o.r * part;
-        const int64_t blocks = (total + 1023) / 1024;
-        relayout_kernel<<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(o.base + h * part, o.sb, o.sr, o.r, part, ws + h * pad,
-                                                                           o.r * cols, cols, total);
-        if (int rc = check_launch("relayout_kernel")) return rc;
-    }
+    for (int h = 0; h < halves; ++h)
+        jobs.job[jobs.n++] = Copy{o.base + h * part, ws + h * pad, o.sb, o.sr, o.r * cols, o.batch * o.r, o.r, (int)part, (int)cols};
     o.base = ws;
     o.sr = cols;
     o.sb = o.r * cols;
     o.c = cols == pad ? o.c : cols;
     ws += (o.batch * o.r * cols + 7) & ~(int64_t)7;
     o.direct = true;
-    return KQ_OK;
+}
+
+int run_copies(const Copies& jobs, cudaStream_t s) {
+    if (!jobs.n) return KQ_OK;
+    int64_t most = 0;
+    for (int i = 0; i < jobs.n; ++i) most = jobs.job[i].rows > most ? jobs.job[i].rows : most;
+    const int64_t blocks = (most + 7) / 8;
+    relayout_kernel<<<dim3((unsigned)(blocks < 2368 ? blocks : 2368), (unsigned)jobs.n), 256, 0, s>>>(jobs);
+    return check_launch("relayout_kernel");
 }
 
 // Pairs of CTAs that run at once (every instance needs a whole SM); asked once for each device.
@@ -664,8 +689,10 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     const bool bf16 = p.dtype == KQ_BF16, mn = n_contiguous(p);
     Operand x = operand(p.x, 1, p.rows, p.k, 0, p.ldx), w = w_operand(p, mn);
     const bool gated_copy = mn && p.gated && !w.direct;
-    if (int rc = relayout(x, ws, 1, s)) return rc;
-    if (int rc = relayout(w, ws, gated_copy ? 2 : 1, s)) return rc;
+    Copies jobs;
+    relayout(x, ws, 1, jobs);
+    relayout(w, ws, gated_copy ? 2 : 1, jobs);
+    if (int rc = run_copies(jobs, s)) return rc;
     RowsProduct r{};
     r.x = x;
     r.w = w;
@@ -775,8 +802,10 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     if ((uintptr_t)workspace & 15) { set_error("%s: workspace must be 16-byte aligned", what); return KQ_ERR_ALIGN; }
     uint16_t* ws = static_cast<uint16_t*>(workspace);
     SumsSides o = sums_sides(p, dz, ld_dz);
-    if (int rc = relayout(o.a, ws, 1, s)) return rc;
-    if (int rc = relayout(o.b, ws, 1, s)) return rc;
+    Copies jobs;
+    relayout(o.a, ws, 1, jobs);
+    relayout(o.b, ws, 1, jobs);
+    if (int rc = run_copies(jobs, s)) return rc;
     CUtensorMap ma, mb;
     if (int rc = map_rows_2d(&ma, o.a, bf16, 64, BK, what)) return rc;
     if (int rc = map_rows_2d(&mb, o.b, bf16, 64, BK, what)) return rc;

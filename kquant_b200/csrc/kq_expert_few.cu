@@ -11,8 +11,8 @@
 // memory, and each CTA of the cluster adds up (in rank order: the same bits
 // every time) and finishes its share of the features.
 //
-// Up to 32 rows, two CTAs share an SM with 100 KB of loads in flight each: the
-// epilogue of one runs under the loads of the other.
+// Two CTAs share an SM with 100 KB of loads in flight each where that is at
+// least three stages: the epilogue of one runs under the loads of the other.
 #include "kq_expert_rows.cuh"
 
 namespace kq {
@@ -74,6 +74,10 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        tma_prefetch(&map_w);
+        tma_prefetch(&map_x);
+    }
     const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
     const int m0 = (int)(blockIdx.x / p.splits) * 128;
 
@@ -163,6 +167,26 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     }
     if (!ok) report_wait_error(p.err);
     __syncwarp();
+    // What the epilogue reads from memory comes in under the products: the bias and the first rows of aux.
+    const int width = 128 / p.splits, f0 = rank * width;
+    auto load_aux = [&](float (&a)[4], int r, int step) {
+        const int f = m0 + f0 + (threadIdx.x & (width - 1));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t row = row0 + min(r + u * step, count - 1);
+            a[u] = p.aux && f < p.m_out ? to_f<T>(static_cast<const T*>(p.aux)[row * p.ld_aux + f]) : 0.f;
+        }
+    };
+    float early[4], add = 0.f, add_up = 0.f;
+    {
+        const int shift = 31 - __clz(width), f = m0 + f0 + (threadIdx.x & (width - 1));
+        load_aux(early, threadIdx.x >> shift, THREADS >> shift);
+        if (p.bias && f < p.m_out) {
+            const T* bias = static_cast<const T*>(p.bias) + e * p.bias_stride + f;
+            add = to_f<T>(bias[0]);
+            if constexpr (GATED) add_up = to_f<T>(bias[p.m_out]);
+        }
+    }
     if (!mbar_wait(&done_bar, 0)) {
         if (lane == 0) report_wait_error(p.err);
     }
@@ -172,8 +196,6 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     // Partial sums [rows][128 features] (gate, then up) meet in shared memory, 32 rows at a time.
     float* part = reinterpret_cast<float*>(smem);
     const uint32_t part_addr = smem_addr(part);
-    const int width = 128 / p.splits, f0 = rank * width;
-    const T* bias = static_cast<const T*>(p.bias) + e * p.bias_stride;
     for (int c0 = 0; c0 < count; c0 += PART) {
         const int n = min(PART, count - c0);
         const uint32_t base = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c0;
@@ -190,30 +212,40 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         }
         if (p.splits > 1) cluster_sync();
         else __syncthreads();
-        for (int i = threadIdx.x; i < width * n; i += THREADS) {
-            const int f = f0 + i % width, r = i / width;
-            if (m0 + f >= p.m_out) continue;
-            const int64_t row = row0 + c0 + r;
-            const float a = p.aux ? to_f<T>(static_cast<const T*>(p.aux)[row * p.ld_aux + m0 + f]) : 0.f;
-            float z = p.bias ? to_f<T>(bias[m0 + f]) : 0.f, w = 0.f;
-            if (GATED && p.bias) w = to_f<T>(bias[p.m_out + m0 + f]);
-            float sum = 0.f, sum_up = 0.f;
-            for (int s = 0; s < p.splits; ++s) {
-                const uint32_t at = part_addr + (uint32_t)(r * 128 + f) * 4;
-                const uint32_t from = p.splits > 1 ? rank_addr(at, s) : at;
-                sum += load_cluster(from);
-                if constexpr (GATED) sum_up += load_cluster(from + PART * 128 * 4);
-            }
-            z += sum;
-            w += sum_up;
-            T* o = static_cast<T*>(p.out) + row * p.ld_out + m0 + f;
-            if (!p.grad) {
-                o[0] = from_f<T>(act_of(p.act, z) * (GATED ? w : 1.f) + a);
-            } else if constexpr (GATED) {
-                o[0] = from_f<T>(a * w * slope_of(p.act, z));
-                o[p.m_out] = from_f<T>(a * act_of(p.act, z));
-            } else {
-                o[0] = from_f<T>(a * slope_of(p.act, z));
+        // A thread keeps its feature (128 threads are whole rows of `width` features) and takes four rows at a time.
+        const int shift = 31 - __clz(width), f = f0 + (threadIdx.x & (width - 1)), step = THREADS >> shift;
+        if (m0 + f < p.m_out) {
+            for (int r = threadIdx.x >> shift; r < n; r += 4 * step) {
+                float a[4], z[4], w[4];
+                if (c0 > 0 || r >= 4 * step) load_aux(a, c0 + r, step);
+                else
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) a[u] = early[u];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) { z[u] = 0.f; w[u] = 0.f; }
+                for (int s = 0; s < p.splits; ++s) {
+                    const uint32_t at = p.splits > 1 ? rank_addr(part_addr, s) : part_addr;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t from = at + (uint32_t)(min(r + u * step, PART - 1) * 128 + f) * 4;
+                        z[u] += load_cluster(from);
+                        if constexpr (GATED) w[u] += load_cluster(from + PART * 128 * 4);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (r + u * step >= n) break;
+                    T* o = static_cast<T*>(p.out) + (int64_t)(row0 + c0 + r + u * step) * p.ld_out + m0 + f;
+                    const float zz = z[u] + add, ww = w[u] + add_up;
+                    if (!p.grad) {
+                        o[0] = from_f<T>(act_of(p.act, zz) * (GATED ? ww : 1.f) + a[u]);
+                    } else if constexpr (GATED) {
+                        o[0] = from_f<T>(a[u] * ww * slope_of(p.act, zz));
+                        o[p.m_out] = from_f<T>(a[u] * act_of(p.act, zz));
+                    } else {
+                        o[0] = from_f<T>(a[u] * slope_of(p.act, zz));
+                    }
+                }
             }
         }
         if (p.splits > 1) cluster_sync();                 // the others are done with this CTA's part
@@ -246,9 +278,12 @@ int launch(const CUtensorMap& w, const CUtensorMap& x, const Params& p, int smem
 
 }  // namespace
 
+// Up to 16 rows an expert always; up to 48 where W's rows are long enough for its reading to be what counts (8 experts of
+// 7168 -> 4096 gated: 74 us against 82 us at 16 rows, 80 and 83 at 48; 1024 -> 1024: 17 and 14 us at 24); and up to 64 where
+// the other kernel's tiles would leave most SMs without work (7168 -> 2048: 21 us against 55 us).
 bool few_rows(const RowsProduct& p) {
-    const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
-    return p.rows <= 64 * busy;
+    const int64_t busy = p.experts < p.rows ? p.experts : p.rows, tiles = (p.n_out * (p.gated ? 2 : 1) + 255) / 256 * busy;
+    return p.rows <= 16 * busy || (p.k >= 2048 && p.rows <= (tiles <= 18 ? 64 : 48) * busy);
 }
 
 int few_rows_product(const RowsProduct& p, cudaStream_t s) {
@@ -273,8 +308,8 @@ int few_rows_product(const RowsProduct& p, cudaStream_t s) {
     q.grad = p.grad;
     q.zero_rest = p.zero_rest;
     const int stage = (p.gated ? 2 : 1) * SIDE + q.nt * 128;
-    // Two short rings on an SM hide each other's ends; tiles of many rows need the stages in one.
-    const int ring = q.nt <= 32 ? RING_TWO : RING_ONE;
+    // Two short rings on an SM hide each other's ends; where they would hold two stages only, one long ring is better.
+    const int ring = RING_TWO / stage >= 3 ? RING_TWO : RING_ONE;
     q.stages = ring / stage < MAX_STAGES ? ring / stage : MAX_STAGES;
     q.box = q.nt < X_BOX ? q.nt : X_BOX;
     q.idesc = idesc_f16(p.bf16, p.mn, false, 128, 0);

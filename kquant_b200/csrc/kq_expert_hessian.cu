@@ -106,6 +106,8 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
+        tma_prefetch(&maps.a[0]);
+        tma_prefetch(&maps.b[0]);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
@@ -382,8 +384,8 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     if (warp == DRAINS) tmem_free(tmem, 2 * BN);
 }
 
-// Operand rows.  Block (t, c): slots 32 t .. of the padded rows, columns
-// 1024 c ..; the blocks behind the last row tile sum the weights of one
+// Operand rows.  Block (t, c): slots 32 t .. of the padded rows, `block_cols`
+// columns from block_cols c; the blocks behind the last row tile sum the weights of one
 // expert each, in an order that depends on nothing.
 struct OperandParams {
     const void* x;
@@ -393,7 +395,7 @@ struct OperandParams {
     uint16_t* terms;           // a terms, then b terms, each [slots][ld]
     double* den;
     int64_t ldx, tokens, term_stride;
-    int rows, experts, d, ld, row_tiles;
+    int rows, experts, d, ld, row_tiles, block_shift;   // 8 << block_shift columns a block
     bool vec;
 };
 
@@ -437,8 +439,9 @@ __global__ void __launch_bounds__(256) operand_kernel(const OperandParams p) {
     const int t = blockIdx.x;
     if (t >= cum[p.experts]) return;
     const int e = expert_of(cum, p.experts, t), first = (t - cum[e]) * SLOT;
-    for (int i = threadIdx.x; i < SLOT * 128; i += 256) {        // 8 columns of one row at a time
-        const int r = i >> 7, c = blockIdx.y * 1024 + (i & 127) * 8;
+    const int per_row = 1 << p.block_shift;
+    for (int i = threadIdx.x; i < SLOT * per_row; i += 256) {    // 8 columns of one row at a time
+        const int r = i >> p.block_shift, c = (blockIdx.y * per_row + (i & (per_row - 1))) * 8;
         if (c >= p.ld) continue;
         float v[8];
 #pragma unroll
@@ -571,7 +574,10 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     o.ld = ld;
     o.row_tiles = (int)(n_slots / SLOT);
     o.vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
-    const dim3 grid((unsigned)(o.row_tiles + experts), (unsigned)((ld + 1023) / 1024));
+    // Few blocks: shorter ones, for their latency.
+    o.block_shift = (int64_t)o.row_tiles * ((ld + 1023) / 1024) < 296 ? 4 : 7;
+    const int block_cols = 8 << o.block_shift;
+    const dim3 grid((unsigned)(o.row_tiles + experts), (unsigned)((ld + block_cols - 1) / block_cols));
     if (dtype == KQ_FP32) operand_kernel<float, 3, 3><<<grid, 256, 0, s>>>(o);
     else if (dtype == KQ_BF16 && weighted) operand_kernel<__nv_bfloat16, 1, 3><<<grid, 256, 0, s>>>(o);
     else if (dtype == KQ_BF16) operand_kernel<__nv_bfloat16, 0, 0><<<grid, 256, 0, s>>>(o);

@@ -24,7 +24,7 @@ struct Params {
     int64_t svh_stride, ld_out;
     int rows, experts, k_steps, n_tiles, n_out;
     int* err;
-    bool vec_svh, vec_out;
+    bool vec_svh, vec_out, zero_rest;
 };
 
 struct Tile { int e, row0, count, n0; };
@@ -166,6 +166,17 @@ rotated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (lane == 0) mbar_arrive(&acc_empty[b]);
         }
         if (!ok && lane == 0) report_wait_error(p.err);
+        if (p.zero_rest && p.offsets) {
+            int begin, end, n;
+            group_of(p.offsets, 0, p.rows, begin, n);
+            group_of(p.offsets, p.experts - 1, p.rows, end, n);
+            end += n;
+            for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+                if (row >= begin && row < end) continue;
+                T* o = static_cast<T*>(p.out) + (int64_t)row * p.ld_out;
+                for (int j = threadIdx.x - 64; j < p.n_out; j += 32 * DRAIN_WARPS) o[j] = from_f<T>(0.f);
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -185,7 +196,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid
 
 int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
                          int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
-                         bool bf16_out, cudaStream_t s) {
+                         bool bf16_out, bool zero_rest, cudaStream_t s) {
     const char* what = "rows_product_rotated";
     CUtensorMap ma, mb;
     const int64_t xd[2] = {k, rows}, xs[1] = {k * 2}, wd[3] = {k, n, experts}, wst[2] = {k * 2, n * k * 2};
@@ -205,6 +216,7 @@ int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* of
     q.k_steps = (int)((k + BK - 1) / BK);
     q.n_tiles = (int)((n + BN - 1) / BN);
     q.n_out = (int)n;
+    q.zero_rest = zero_rest;
     q.vec_svh = ((uintptr_t)svh & 15) == 0 && svh_stride % 8 == 0;
     q.vec_out = ((uintptr_t)y & 15) == 0 && ldy % 8 == 0;
     int sms;

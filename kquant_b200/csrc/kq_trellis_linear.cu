@@ -91,11 +91,11 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
 // x' = had(x * suh) * 2^s in binary16 and 2^-s; one block a row, a warp a Hadamard block of 128 channels.  The row's
 // largest product decides s, so it is held in registers between the two (up to HELD blocks a warp; longer rows are read
 // twice).
-template <typename T>
-__global__ void __launch_bounds__(512) rotate_in_kernel(const T* __restrict__ x, int64_t ldx, const __half* __restrict__ suh,
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) rotate_in_kernel(const T* __restrict__ x, int64_t ldx, const __half* __restrict__ suh,
                                                         int64_t suh_stride, const int64_t* __restrict__ offsets, int rows,
                                                         int experts, int k, __half* __restrict__ xr, float* __restrict__ scale) {
-    constexpr int WARPS = 16, HELD = 4;
+    constexpr int HELD = 4;
     __shared__ float most[WARPS];
     const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = k / kBlock;
     const int e = place_of_row(offsets, experts, rows, row, 1).e;
@@ -204,35 +204,37 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
     __half* stage = reinterpret_cast<__half*>(smem + table_bytes(DEC));
     load_table<DEC>(table, smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nb = n / DN, kb = k / DK, per = nb * kb;
-    const int64_t tiles_n = n / 16, all = (int64_t)per * experts;
-    // The next block of a busy expert from `i` on (an expert without rows is not decoded), and its words.
-    int busy_e = -1, busy = 0;
-    auto seek = [&](int64_t i) {
-        for (; i < all; i += gridDim.x) {
-            const int e = (int)(i / per);
-            if (e != busy_e) {
+    const int nb = n / DN, kb = k / DK, per = nb * kb, tiles_n = n / 16;
+    // Block l of expert e; seek() moves on to a busy expert's (one without rows is not decoded).
+    struct At { int e, l; };
+    int known_e = -1, known_n = 0;
+    auto seek = [&](At& at) {
+        for (;; ++at.e, at.l -= per) {
+            while (at.l >= per) { at.l -= per; ++at.e; }
+            if (at.e >= experts) return;
+            if (at.e != known_e) {
                 int lo;
-                group_of(offsets, e, rows, lo, busy);
-                busy_e = e;
+                group_of(offsets, at.e, rows, lo, known_n);
+                known_e = at.e;
             }
-            if (busy) break;
+            if (known_n) return;
+            at.l += (per - at.l + (int)gridDim.x - 1) / (int)gridDim.x * (int)gridDim.x;   // this CTA's first one beyond it
         }
-        return i;
     };
     TileWords<K> w[4];
-    auto fetch = [&](int64_t i) {
-        if (i >= all) return;
-        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per), n0 = (l % nb) * DN, k0 = (l / nb) * DK;
+    auto fetch = [&](const At& at) {
+        if (at.e >= experts) return;
+        const int n0 = at.l % nb, k0 = at.l / nb;
+        const uint32_t* t = trellis + (((int64_t)at.e * (k / 16) + k0 * (DK / 16)) * tiles_n + n0 * (DN / 16) + warp) * 8 * K;
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-            w[a].load(trellis + (((int64_t)e * (k / 16) + k0 / 16 + a) * tiles_n + n0 / 16 + warp) * 8 * K, lane);
+        for (int a = 0; a < 4; ++a) w[a].load(t + (int64_t)a * tiles_n * 8 * K, lane);
     };
-    int64_t i = seek(blockIdx.x);
-    fetch(i);
+    At at{0, (int)blockIdx.x};
+    seek(at);
+    fetch(at);
     __syncthreads();
-    while (i < all) {
-        const int e = (int)(i / per), l = (int)(i - (int64_t)e * per), n0 = (l % nb) * DN, k0 = (l / nb) * DK;
+    while (at.e < experts) {
+        const int e = at.e, n0 = at.l % nb * DN, k0 = at.l / nb * DK;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             uint32_t f[4];
@@ -243,8 +245,9 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
             o[8 * DPAD / 2] = f[2];
             o[8 * DPAD / 2 + 4] = f[3];
         }
-        const int64_t next = seek(i + gridDim.x);
-        fetch(next);                                    // under the other warps' decoding and the stores
+        at.l += gridDim.x;
+        seek(at);
+        fetch(at);                                      // under the other warps' decoding and the stores
         // Each warp's 16 columns are its own: they leave without the rest of the block.
         __syncwarp();
 #pragma unroll
@@ -253,20 +256,6 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
             *reinterpret_cast<uint4*>(out + ((int64_t)e * n + n0 + r) * k + k0 + c) = *reinterpret_cast<const uint4*>(stage + r * DPAD + c);
         }
         __syncwarp();
-        i = next;
-    }
-}
-
-// Rows of no expert, zeroed in a fresh output.
-template <typename T>
-__global__ void zero_rest_kernel(const int64_t* offsets, int experts, int rows, int n, T* y, int64_t ldy) {
-    int first, last, c;
-    group_of(offsets, 0, rows, first, c);
-    group_of(offsets, experts - 1, rows, last, c);
-    last += c;
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-        if (row >= first && row < last) continue;
-        for (int j = threadIdx.x; j < n; j += blockDim.x) y[(int64_t)row * ldy + j] = from_f<T>(0.f);
     }
 }
 
@@ -274,17 +263,18 @@ constexpr int kFewMean = 64;
 
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
-struct Plan { bool few, wide; int parts, ctas; int64_t scale, rest, bytes; };
+struct Plan { bool few, wide; int parts; int64_t scale, rest, bytes; };
 
-Plan plan(const kq_trellis_product& p, int sms) {
+int few_ctas(const kq_trellis_product& p, int sms) { return sms * (p.codebook == KQ_CB_LABELS ? 1 : 2); }   // a table of 128 KB leaves room for one
+
+Plan plan(const kq_trellis_product& p) {
     Plan l{};
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
     l.few = p.rows <= kFewMean * busy;
     l.wide = p.rows > 8 * busy;
-    l.ctas = sms * (p.codebook == KQ_CB_LABELS ? 1 : 2);      // a table of 128 KB leaves room for one
-    // Parts of a strip: what an even share of a single row tile makes, within 256 MB (two at least).
+    // Parts of a strip: what an even share of a single row tile makes on 148 SMs, within 256 MB (two at least).
     const int64_t kt = p.k / 16, strips = p.n / few_columns(l.wide), one = p.rows * p.n * 4;
-    const int64_t share = strips * kt / l.ctas > 32 ? strips * kt / l.ctas : 32, fit = ((int64_t)1 << 28) / one;
+    const int64_t even = strips * kt / few_ctas(p, 148), share = even > 32 ? even : 32, fit = ((int64_t)1 << 28) / one;
     const int64_t most = kt / share + 2;
     l.parts = (int)(most < fit ? most : fit < 2 ? 2 : fit);
     l.scale = align128(p.rows * p.k * 2);
@@ -345,10 +335,15 @@ int decode_all(const kq_trellis_product& p, __half* out, cudaStream_t s) {
     }
 }
 
+// Few rows: more warps a row, for its latency; many: enough rows an SM as it is.
 template <typename T>
 int rotate_in(const kq_trellis_product& p, __half* xr, float* scale, cudaStream_t s) {
-    rotate_in_kernel<T><<<(unsigned)p.rows, 512, 0, s>>>(static_cast<const T*>(p.x), p.ldx, reinterpret_cast<const __half*>(p.suh),
-                                                         p.suh_stride_e, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, xr, scale);
+    auto run = [&](auto kernel, int threads) {
+        kernel<<<(unsigned)p.rows, threads, 0, s>>>(static_cast<const T*>(p.x), p.ldx, reinterpret_cast<const __half*>(p.suh),
+                                                    p.suh_stride_e, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, xr, scale);
+    };
+    if (p.rows <= 256) run(rotate_in_kernel<T, 16>, 512);
+    else run(rotate_in_kernel<T, 4>, 128);
     return check_launch("rotate_in_kernel");
 }
 
@@ -357,9 +352,7 @@ int rotate_in(const kq_trellis_product& p, __half* xr, float* scale, cudaStream_
 
 extern "C" size_t kq_trellis_linear_workspace_bytes(const kq_trellis_product* p) {
     if (!p || kq::check_trellis(*p, "kq_trellis_linear_workspace_bytes") || p->rows == 0) return 0;
-    int sms;
-    if (kq::sm_count(&sms)) return 0;
-    return (size_t)kq::plan(*p, sms).bytes;
+    return (size_t)kq::plan(*p).bytes;
 }
 
 extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, size_t workspace_bytes, void* stream) {
@@ -377,9 +370,7 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         set_error("%s: trellis and table need 16-byte alignment", what);
         return KQ_ERR_ALIGN;
     }
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
-    const Plan l = plan(p, sms);
+    const Plan l = plan(p);
     if (!workspace || workspace_bytes < (size_t)l.bytes) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -389,6 +380,8 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
     const bool bf16 = p.dtype == KQ_BF16;
     if (int rc = bf16 ? rotate_in<__nv_bfloat16>(p, xr, scale, s) : rotate_in<__half>(p, xr, scale, s)) return rc;
     if (l.few) {
+        int sms;
+        if (int rc = sm_count(&sms)) return rc;
         float* partial = reinterpret_cast<float*>(ws + l.rest);
         const FewTrellis f{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr), partial,
                            (int)p.rows, (int)p.experts, (int)p.k, (int)p.n, l.parts};
@@ -399,21 +392,15 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         const dim3 grid((unsigned)p.rows, (unsigned)((p.n / kBlock + 7) / 8));
         const __half* svh = reinterpret_cast<const __half*>(p.svh);
         if (bf16)
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, l.ctas, (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
                                                    (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy, p.zero_rest != 0);
         else
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, l.ctas, (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
+            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
                                                    (int)p.n, static_cast<__half*>(p.y), p.ldy, p.zero_rest != 0);
         return check_launch("rotate_out_kernel");
     }
     __half* w = reinterpret_cast<__half*>(ws + l.rest);
-    if (p.zero_rest && p.offsets) {
-        const int grid = (int)(p.rows < 1024 ? p.rows : 1024);
-        if (bf16) zero_rest_kernel<<<grid, 256, 0, s>>>(p.offsets, (int)p.experts, (int)p.rows, (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy);
-        else zero_rest_kernel<<<grid, 256, 0, s>>>(p.offsets, (int)p.experts, (int)p.rows, (int)p.n, static_cast<__half*>(p.y), p.ldy);
-        if (int rc = check_launch("zero_rest_kernel")) return rc;
-    }
     if (int rc = decode_all(p, w, s)) return rc;
     return rows_product_rotated(reinterpret_cast<const uint16_t*>(xr), reinterpret_cast<const uint16_t*>(w), p.offsets, p.rows, p.k, p.n,
-                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, s);
+                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, p.zero_rest != 0, s);
 }

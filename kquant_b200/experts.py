@@ -24,22 +24,26 @@ _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def _operand(t: torch.Tensor, name: str, dims: int, dtype: torch.dtype, device: torch.device) -> None:
+    if t.is_cuda and t.dtype is dtype and t.ndim == dims and t.device == device:
+        return
     if not t.is_cuda:
         raise _native.KQError(f"{name} must be a CUDA tensor (kquant_b200 has no CPU path)")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.ndim != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, got {t.ndim}")
+    raise ValueError(f"{name} must have {dims} dimensions, got {t.ndim}")
 
 
-def _rows_operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, device: torch.device) -> None:
+def _rows_operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, device: torch.device) -> int:
+    """The row stride of a [rows, width] operand."""
     _operand(t, name, 2, dtype, device)
     if t.shape != (rows, width):
         raise ValueError(f"{name} must be [{rows}, {width}], got {list(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
+    ld, unit = t.stride()
+    if unit != 1 and width > 1:
         raise ValueError(f"{name} needs unit stride along its last dimension")
+    return ld
 
 
 def _check_offsets(offsets: torch.Tensor | None, experts: int, device: torch.device) -> None:
@@ -56,20 +60,29 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _product(x, w, offsets, bias, activation, gated) -> _native.ExpertProduct:
-    """The checked operands that every product of these shares."""
+def _product(x, w, offsets, bias, activation, gated, dense=False) -> _native.ExpertProduct:
+    """The checked operands that every product of these shares; ``dense``: one matrix [k, n] and its bias [n]."""
     if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor):
         raise TypeError("x and w must be tensors")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    dev = x.device
-    _operand(x, "x", 2, x.dtype, dev)
-    _operand(w, "w", 3, x.dtype, dev)
-    E, k, n = w.shape
-    if min(E, k, n) < 1:
+    dt, dev = x.dtype, x.device
+    if dt not in _DTYPES:
+        raise TypeError(f"x must be torch.bfloat16 or torch.float16, got {dt}")
+    _operand(x, "x", 2, dt, dev)
+    p = _native.ExpertProduct()
+    if dense:
+        _operand(w, "w", 2, dt, dev)
+        E, (k, n) = 1, w.shape
+        p.w_stride_k, p.w_stride_n = sk, sn = w.stride()
+    else:
+        _operand(w, "w", 3, dt, dev)
+        E, k, n = w.shape
+        p.w_stride_e, p.w_stride_k, p.w_stride_n = _, sk, sn = w.stride()
+    if E < 1 or k < 1 or n < 1:
         raise ValueError(f"w must not be empty, got {list(w.shape)}")
-    _rows_operand(x, "x", x.shape[0], k, x.dtype, dev)
-    if w.stride(1) != 1 and w.stride(2) != 1 and k > 1 and n > 1:
+    rows = x.shape[0]
+    p.rows, p.k, p.n, p.experts = rows, k, n, E
+    p.ldx = _rows_operand(x, "x", rows, k, dt, dev)
+    if sk != 1 and sn != 1 and k > 1 and n > 1:
         raise ValueError("w needs unit stride along its in or its out dimension")
     _check_offsets(offsets, E, dev)
     if activation not in _ACTIVATIONS:
@@ -77,17 +90,34 @@ def _product(x, w, offsets, bias, activation, gated) -> _native.ExpertProduct:
     if gated and n % 2:
         raise ValueError("a gated product needs an even out dimension (gate, then up)")
     if bias is not None:
-        _operand(bias, "bias", 2, x.dtype, dev)
-        if bias.shape != (E, n) or (n > 1 and bias.stride(1) != 1):
-            raise ValueError(f"bias must be [{E}, {n}] with unit stride along its last dimension, got {list(bias.shape)}")
-    p = _native.ExpertProduct()
-    p.x, p.w, p.offsets, p.bias = x.data_ptr(), w.data_ptr(), _ptr(offsets), _ptr(bias)
-    p.rows, p.k, p.n, p.experts = x.shape[0], k, n, E
-    p.ldx = x.stride(0)
-    p.w_stride_e, p.w_stride_k, p.w_stride_n = w.stride()
-    p.bias_stride_e = 0 if bias is None else bias.stride(0)
-    p.dtype, p.activation, p.gated = _DTYPES[x.dtype], _ACTIVATIONS[activation], int(bool(gated))
+        _operand(bias, "bias", 1 if dense else 2, dt, dev)
+        if bias.shape != ((n,) if dense else (E, n)) or (n > 1 and bias.stride(-1) != 1):
+            raise ValueError(f"bias must be [{'' if dense else f'{E}, '}{n}] with unit stride along its last dimension, got {list(bias.shape)}")
+        p.bias = bias.data_ptr()
+        if not dense:
+            p.bias_stride_e = bias.stride(0)
+    p.x, p.w = x.data_ptr(), w.data_ptr()
+    if offsets is not None:
+        p.offsets = offsets.data_ptr()
+    p.dtype, p.activation, p.gated = _DTYPES[dt], _ACTIVATIONS[activation], 1 if gated else 0
     return p
+
+
+def _linear(p: _native.ExpertProduct, x, residual, out) -> torch.Tensor:
+    """The forward product behind checked operands."""
+    n_out, rows, dt, dev = p.n // 2 if p.gated else p.n, p.rows, x.dtype, x.device
+    if residual is not None:
+        p.ld_residual = _rows_operand(residual, "residual", rows, n_out, dt, dev)
+        p.residual = residual.data_ptr()
+    if out is None:
+        out = torch.empty((rows, n_out), dtype=dt, device=dev)
+        p.ldy, p.zero_rest = n_out, 1
+    else:
+        p.ldy = _rows_operand(out, "out", rows, n_out, dt, dev)
+    if rows:
+        p.y = out.data_ptr()
+        _native.expert_linear(p, dev)
+    return out
 
 
 def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *, bias: torch.Tensor | None = None,
@@ -99,31 +129,13 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None
     columns and then the up projection's, y = act(gate) * up + residual has n / 2 columns.  ``activation``: None,
     "relu", "silu" or "gelu" (the error-function form).  ``out`` may be the residual itself.
     """
-    p = _product(x, w, offsets, bias, activation, gated)
-    n_out = p.n // 2 if gated else p.n
-    if residual is not None:
-        _rows_operand(residual, "residual", p.rows, n_out, x.dtype, x.device)
-        p.residual, p.ld_residual = residual.data_ptr(), residual.stride(0)
-    if out is None:
-        out = torch.empty((p.rows, n_out), dtype=x.dtype, device=x.device)
-        p.zero_rest = 1
-    else:
-        _rows_operand(out, "out", p.rows, n_out, x.dtype, x.device)
-    if p.rows:
-        p.y, p.ldy = out.data_ptr(), out.stride(0)
-        _native.expert_linear(p, x.device)
-    return out
+    return _linear(_product(x, w, offsets, bias, activation, gated), x, residual, out)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
            gated: bool = False, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """act(x w + bias) + residual with one matrix w [k, n] and bias [n]; see :func:`expert_linear`."""
-    if isinstance(w, torch.Tensor) and w.ndim != 2:
-        raise ValueError(f"w must have 2 dimensions, got {w.ndim}")
-    if bias is not None and bias.ndim != 1:
-        raise ValueError(f"bias must have 1 dimension, got {bias.ndim}")
-    return expert_linear(x, w[None], None, bias=None if bias is None else bias[None], activation=activation, gated=gated,
-                         residual=residual, out=out)
+    return _linear(_product(x, w, None, bias, activation, gated, dense=True), x, residual, out)
 
 
 def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *,
@@ -185,7 +197,8 @@ def trellis_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, sv
         raise ValueError("trellis must be contiguous [experts, k/16, n/16, 16 K] words with K in 1..8")
     if E < 1 or k < 1 or n < 1 or k % 128 or n % 128:
         raise ValueError(f"trellis must hold at least one matrix with k and n multiples of 128, got {E} of [{k}, {n}]")
-    _rows_operand(x, "x", x.shape[0], k, x.dtype, dev)
+    rows = x.shape[0]
+    ldx = _rows_operand(x, "x", rows, k, x.dtype, dev)
     _check_offsets(offsets, E, dev)
     for name, t, size in (("suh", suh, k), ("svh", svh, n)):
         _operand(t, name, 2, torch.float16, dev)
@@ -202,15 +215,15 @@ def trellis_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, sv
         p.codebook = _native.KQ_CB_SQG if codebook.dtype == torch.uint8 else _native.KQ_CB_LABELS
         p.table = codebook.data_ptr()
     if out is None:
-        out = torch.empty((x.shape[0], n), dtype=x.dtype, device=dev)
-        p.zero_rest = 1
+        out = torch.empty((rows, n), dtype=x.dtype, device=dev)
+        p.ldy, p.zero_rest = n, 1
     else:
-        _rows_operand(out, "out", x.shape[0], n, x.dtype, dev)
+        p.ldy = _rows_operand(out, "out", rows, n, x.dtype, dev)
     p.x, p.trellis, p.suh, p.svh, p.offsets, p.y = (x.data_ptr(), trellis.data_ptr(), suh.data_ptr(), svh.data_ptr(),
                                                     _ptr(offsets), out.data_ptr())
-    p.rows, p.k, p.n, p.experts = x.shape[0], k, n, E
-    p.ldx, p.ldy, p.suh_stride_e, p.svh_stride_e = x.stride(0), out.stride(0), suh.stride(0), svh.stride(0)
+    p.rows, p.k, p.n, p.experts = rows, k, n, E
+    p.ldx, p.suh_stride_e, p.svh_stride_e = ldx, suh.stride(0), svh.stride(0)
     p.bits, p.dtype = K, _DTYPES[x.dtype]
-    if p.rows:
+    if rows:
         _native.trellis_linear(p, dev)
     return out
