@@ -304,7 +304,7 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 tc_fence_after();
                 return got;
             };
-            if (!(ok = mbar_wait_cluster(&acc_empty[h0], ((turn >> 1) & 1) ^ 1))) break;
+            if (!(ok = mbar_wait(&acc_empty[h0], ((turn >> 1) & 1) ^ 1))) break;
             tc_fence_after();
             int done0 = 0;                      // k steps issued into the first accumulator, at `lead` in the ring
             Ring lead = at;
@@ -316,7 +316,7 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if ((ok = loaded(done0, lead))) products(0, done0++, lead.s);
                     lead.next(stages);
                 }
-                if (!(ok = ok && mbar_wait_cluster(&acc_empty[h1], parity))) break;
+                if (!(ok = ok && mbar_wait(&acc_empty[h1], parity))) break;
                 tc_fence_after();
             }
             for (int ks = 0; ks < t.k_steps; ++ks, at.next(stages)) {
