@@ -123,11 +123,10 @@ struct Ring {
 // Zeroes rows valid .. 63 of a sums stage in this CTA once its loads have landed.  Whole warp.
 __device__ __forceinline__ bool zero_tail(uint8_t* stage, int slabs, int valid, uint64_t* tail_bar, uint32_t parity, int lane) {
     const bool ok = mbar_wait(tail_bar, parity);
-    const int missing = BK - valid, pieces = slabs * missing * 8;
-    for (int i = lane; i < pieces; i += 32) {
-        const int line = i >> 3, c = line / missing, r = valid + line % missing;
-        *reinterpret_cast<uint4*>(stage + c * CHUNK + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-    }
+    // Eight lanes a 128-byte row.
+    for (int c = 0; c < slabs; ++c)
+        for (int r = valid + (lane >> 3); r < BK; r += 4)
+            *reinterpret_cast<uint4*>(stage + c * CHUNK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     return ok;
