@@ -55,7 +55,8 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
     ``rows`` [tokens, d] bf16, fp16 or fp32 on the GPU.  ``index`` (int64) names the row of each slot, as routing
     gives it (a row may serve several experts, and an index outside the rows counts for nothing); without it slot t
     is row t.  ``weights`` fp32, one per slot.  Returns (H [experts, d, d] fp32, denominators [experts] fp64, the
-    sums of the weights), both on the GPU: nothing waits for the device.  With ``out`` the sums are added to it,
+    sums of the weights), both on the GPU: nothing waits for the device.  A fresh H whose d is not a multiple of 32 is a
+    view with rows padded to one.  With ``out`` the sums are added to it,
     which is how samples stream in; the denominators are this call's alone.  fp32 accuracy for every type.
     """
     if not isinstance(rows, torch.Tensor) or rows.dtype not in _ROW_DTYPES:
@@ -85,7 +86,8 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
             raise ValueError(f"out must be [{E}, {d}, {d}] with unit stride along its last dimension")
     if tokens > 1 and rows.stride(0) < d:
         rows = rows.contiguous()
-    H = out if out is not None else torch.empty((E, d, d), dtype=torch.float32, device=dev)
+    # Rows of a fresh H start on 128-byte lines: with d floats a row, an odd d splits every line that is written.
+    H = out if out is not None else torch.empty((E, d, -(-d // 32) * 32), dtype=torch.float32, device=dev)[:, :, :d]
     den = torch.empty(E, dtype=torch.float64, device=dev)
     _native.accumulate_expert_hessians(rows, _ROW_DTYPES[rows.dtype], index, weights, offsets, slots, H, out is not None, den)
     return H, den

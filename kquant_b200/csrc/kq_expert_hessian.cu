@@ -219,8 +219,11 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                     __syncwarp();
                     const int j = j0 + c + lane;
                     float* dst = p.H + e * p.h_stride + (int64_t)i0 * p.ldh + j;
-                    for (int k = 0; k < min(32, p.d - i0) && j < p.d; ++k, dst += p.ldh) {
+                    const int n = j < p.d ? p.d - i0 : 0;
+#pragma unroll 16
+                    for (int k = 0; k < 32; ++k, dst += p.ldh) {
                         const float x = reinterpret_cast<const float*>(unit(k, lane >> 2))[lane & 3];
+                        if (k >= n) continue;
                         if (add) atomicAdd(dst, x);
                         else *dst = x;
                     }
@@ -295,16 +298,14 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                     }
                 }
                 __syncwarp();
-                if (p.vec) {
+                if (p.vec && max(i0, j) + 32 <= p.d) {
                     // 16 bytes a lane, four rows an access.
                     for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
                         const int row0 = (side ? j : i0) + (lane >> 3), col = (side ? i0 : j) + (lane & 7) * 4;
                         uint8_t* block = side ? mirror : piece;
-                        if (col >= p.d) continue;
                         float* dst = H + (int64_t)row0 * p.ldh + col;
 #pragma unroll
                         for (int k = 0; k < 32; k += 4, dst += 4 * p.ldh) {
-                            if (row0 + k >= p.d) break;
                             const float4 x = *reinterpret_cast<const float4*>(at(block, (lane >> 3) + k, (lane & 7) * 4));
                             if (p.add) atomicAdd(reinterpret_cast<float4*>(dst), x);
                             else __stcs(reinterpret_cast<float4*>(dst), x);
@@ -315,11 +316,14 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                     for (int side = 0; side < (diagonal ? 1 : 2); ++side) {
                         const int row0 = side ? j : i0, col = (side ? i0 : j) + lane;
                         uint8_t* block = side ? mirror : piece;
-                        if (col >= p.d) continue;
                         float* dst = H + (int64_t)row0 * p.ldh + col;
-                        for (int k = 0; k < min(32, p.d - row0); ++k, dst += p.ldh) {
-                            if (p.add) atomicAdd(dst, *at(block, k, lane));
-                            else *dst = *at(block, k, lane);
+                        const int n = col < p.d ? p.d - row0 : 0;
+#pragma unroll 16
+                        for (int k = 0; k < 32; ++k, dst += p.ldh) {
+                            const float x = *at(block, k, lane);
+                            if (k >= n) continue;
+                            if (p.add) atomicAdd(dst, x);
+                            else *dst = x;
                         }
                     }
                     __syncwarp();
@@ -614,7 +618,7 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     q.idesc = idesc_f16(!fp16, true, true, BM, BN);
     q.add = add != 0;
     const bool vec = ((uintptr_t)H & 15) == 0 && ldh % 4 == 0 && h_stride % 4 == 0;
-    q.vec = vec && dim % 4 == 0 && ldh < ((int64_t)1 << 36) && h_stride < ((int64_t)1 << 36);
+    q.vec = vec && ldh < ((int64_t)1 << 36) && h_stride < ((int64_t)1 << 36);
     CUtensorMap map_h{};
     if (q.vec && whole) {
         const int64_t hd[3] = {dim, dim, experts}, hs[2] = {ldh * 4, (experts > 1 ? h_stride : ldh * dim) * 4};
