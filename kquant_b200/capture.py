@@ -93,5 +93,27 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
     return H, den
 
 
+def expert_layer_hessians(tokens: torch.Tensor, index: torch.Tensor, offsets: torch.Tensor, w13: torch.Tensor, *,
+                          weights: torch.Tensor | None = None, activation: str | None = "silu",
+                          bias: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Both calibration Hessians of every expert of a layer from its routed tokens, on the GPU throughout.
+
+    tokens [T, k] bf16 or fp16; ``index`` (int64) the token of each routed slot, slots sorted by expert behind
+    ``offsets``; w13 [experts, k, 2 I] the gate's columns and then the up projection's (``weights``, ``activation`` and
+    ``bias`` as in :func:`accumulate_expert_hessians` and ``experts.expert_linear``).  Returns (H13 [experts, k, k] of
+    the inputs of gate and up, H2 [experts, I, I] of act(gate) * up, the inputs of the down projection, and the
+    denominators): the (x13, x2) pair of kquant/capture.py:1268-1273 for a whole layer.  Slots whose index is outside
+    the tokens count for nothing in either.
+    """
+    H13, den = accumulate_expert_hessians(tokens, offsets, index=index, weights=weights)
+    valid = (index >= 0) & (index < tokens.shape[0])
+    rows = tokens.index_select(0, index.clamp(0, max(tokens.shape[0] - 1, 0))) if tokens.shape[0] else \
+        tokens.new_zeros((index.numel(), tokens.shape[1]))
+    hidden = experts.expert_linear(rows, w13, offsets, bias=bias, activation=activation, gated=True)
+    slot = torch.where(valid, torch.arange(index.numel(), device=index.device), -1)
+    H2, _ = accumulate_expert_hessians(hidden, offsets, index=slot, weights=weights)
+    return H13, H2, den
+
+
 # the reference's private name, for callers that import it directly
 _accumulate_hessian = accumulate_hessian
