@@ -105,6 +105,8 @@ def expert_layer_hessians(tokens: torch.Tensor, index: torch.Tensor, offsets: to
     denominators): the (x13, x2) pair of kquant/capture.py:1268-1273 for a whole layer.  Slots whose index is outside
     the tokens count for nothing in either.
     """
+    if index is None:
+        raise ValueError("index must name the token of each slot")
     H13, den = accumulate_expert_hessians(tokens, offsets, index=index, weights=weights)
     valid = (index >= 0) & (index < tokens.shape[0])
     rows = tokens.index_select(0, index.clamp(0, max(tokens.shape[0] - 1, 0))) if tokens.shape[0] else \

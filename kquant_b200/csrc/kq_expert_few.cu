@@ -281,7 +281,7 @@ int launch(const CUtensorMap& w, const CUtensorMap& x, const Params& p, int smem
 // Up to 16 rows an expert always; up to 48 where W's rows are long enough for its reading to be what counts (8 experts of
 // 7168 -> 4096 gated: 74 us against 82 us at 16 rows, 80 and 83 at 48; 1024 -> 1024: 17 and 14 us at 24).  And however many
 // where the other kernel's tiles of 256 x 256 would leave most SMs without work and k is worth splitting (7168 -> 2048, 64
-// rows: 21 us against 55 us; 5388 -> 39, 174 rows: SPLIT_US against 65 us).
+// rows: 21 us against 55 us; 5388 -> 39, 174 rows: 40 us against 65 us).
 bool few_rows(const RowsProduct& p) {
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
     const int64_t tiles = (p.n_out * (p.gated ? 2 : 1) + 255) / 256 * ((p.rows + 255) / 256 + busy - 1);

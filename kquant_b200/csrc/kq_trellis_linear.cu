@@ -12,7 +12,7 @@
 // bits of x and y.  Products are summed in fp32, the output transform runs in
 // fp32, and y is rounded once.
 //
-// Up to a mean of MEAN rows an expert, the payload is decoded in registers next
+// With few rows an expert (rows_are_few), the payload is decoded in registers next
 // to the product (kq_trellis_few.cuh) and partial sums over ranges of k are
 // added up by the output transform.  With more rows it is decoded once, to
 // binary16 in the workspace, and the tensor-core product with the rotation in
@@ -133,14 +133,17 @@ __global__ void __launch_bounds__(WARPS * 32) rotate_in_kernel(const T* __restri
     for (int i = 0; i < WARPS; ++i) m = fmaxf(m, most[i]);
     // |had(v)| <= sqrt(128) max |v| < 2^4 max |v|: the exponent that brings it to at most 2^14.
     int ex = 0;
-    if (m > 0.f && m < 1e38f) {
+    if (m > 0.f && m < 3.3e38f) {
         frexpf(m, &ex);                                // m < 2^ex
         ex = min(max(10 - ex, -120), 120);
     }
-    const float up = ldexpf(0.08838834764831845f, ex);
+    // The power of two goes in first: the transform of values near the end of the fp32 range stays in it.
+    const float up = ldexpf(1.f, ex), norm = 0.08838834764831845f;      // 1 / sqrt(128)
     auto emit = [&](int blk, float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= up;
         had128_warp(v, lane);
-        __half2 o[2] = {__floats2half2_rn(v[0] * up, v[1] * up), __floats2half2_rn(v[2] * up, v[3] * up)};
+        __half2 o[2] = {__floats2half2_rn(v[0] * norm, v[1] * norm), __floats2half2_rn(v[2] * norm, v[3] * norm)};
         *reinterpret_cast<uint2*>(xr + (int64_t)row * k + blk * kBlock + lane * 4) = *reinterpret_cast<const uint2*>(o);
     };
 #pragma unroll
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict
     float sv[4];
     load4(svh + e * svh_stride + j, sv);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= f * sv[i];
+    for (int i = 0; i < 4; ++i) v[i] = v[i] * sv[i] * f;      // f last: f * sv may be below the normal numbers
     store4(o, v);
 }
 
@@ -259,7 +262,15 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
     }
 }
 
-constexpr int kFewMean = 64;
+// Decoding next to the product costs time per 16 rows of every expert; decoding once costs the same for any number of them,
+// and its product leaves most SMs idle when it has few tiles of 128 columns.  8 experts of 7168 x 4096 at 4 bits, a mean of
+// 16 / 32 / 48 / 64 rows: 196 / 205 / 226 / 272 us against 232 to 243 (MCG), 220 / 260 / 318 / 369 against 278 to 291 (E4M3
+// labels), 295 / 307 / 334 / 375 against 347 to 359 (a table of labels).  One of 7168 x 2048 (16 tiles), 16 / 64 / 96 rows:
+// 25 / 31 / 44 against 56 to 58 us.
+bool rows_are_few(const kq_trellis_product& p) {
+    const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
+    return p.rows <= (p.n / 128 * busy <= 64 ? 96 : 40) * busy;
+}
 
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
@@ -270,7 +281,7 @@ int few_ctas(const kq_trellis_product& p, int sms) { return sms * (p.codebook ==
 Plan plan(const kq_trellis_product& p) {
     Plan l{};
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
-    l.few = p.rows <= kFewMean * busy;
+    l.few = rows_are_few(p);
     l.wide = p.rows > 8 * busy;
     // Parts of a strip: what an even share of a single row tile makes on 148 SMs, within 256 MB (two at least).
     const int64_t kt = p.k / 16, strips = p.n / few_columns(l.wide), one = p.rows * p.n * 4;
@@ -290,6 +301,7 @@ int check_trellis(const kq_trellis_product& p, const char* what) {
                   (long long)p.rows, (long long)p.k, (long long)p.n, (long long)p.experts, p.bits);
         return KQ_ERR_ARG;
     }
+    if (p.k > (int64_t(1) << 41) / p.n) { set_error("%s: one expert's matrix has more than 2^41 elements", what); return KQ_ERR_ARG; }
     if (p.experts > 1 && !p.offsets) { set_error("%s: several experts need offsets", what); return KQ_ERR_ARG; }
     if (p.dtype != KQ_BF16 && p.dtype != KQ_FP16) { set_error("%s: dtype must be KQ_BF16 or KQ_FP16", what); return KQ_ERR_ARG; }
     if (p.codebook != KQ_CB_MCG && p.codebook != KQ_CB_SQG && p.codebook != KQ_CB_LABELS) {

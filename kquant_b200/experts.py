@@ -56,6 +56,25 @@ def _check_offsets(offsets: torch.Tensor | None, experts: int, device: torch.dev
         raise ValueError(f"offsets must be {experts + 1} contiguous values for {experts} experts")
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte and end of what a tensor's elements lie in."""
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _refuse_overlap(out: torch.Tensor, t: torch.Tensor | None, name: str) -> None:
+    """The kernels read operands while others write results; columns of one buffer beside each other are apart."""
+    if t is None or not t.numel() or not out.numel() or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
+        return
+    (a, a_end), (b, b_end) = _span(out), _span(t)
+    if a_end <= b or b_end <= a:
+        return
+    if t.ndim == 2 and t.stride(0) == out.stride(0) > 0 and name != "bias":
+        ld, by = out.stride(0), (b - a) // out.element_size() % out.stride(0)      # where t's rows begin among out's
+        if by >= out.shape[1] and by + t.shape[1] <= ld:
+            return
+    raise ValueError(f"out must not overlap {name}")
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
@@ -103,7 +122,7 @@ def _product(x, w, offsets, bias, activation, gated, dense=False) -> _native.Exp
     return p
 
 
-def _linear(p: _native.ExpertProduct, x, residual, out) -> torch.Tensor:
+def _linear(p: _native.ExpertProduct, x, w, bias, residual, out) -> torch.Tensor:
     """The forward product behind checked operands."""
     n_out, rows, dt, dev = p.n // 2 if p.gated else p.n, p.rows, x.dtype, x.device
     if residual is not None:
@@ -114,6 +133,11 @@ def _linear(p: _native.ExpertProduct, x, residual, out) -> torch.Tensor:
         p.ldy, p.zero_rest = n_out, 1
     else:
         p.ldy = _rows_operand(out, "out", rows, n_out, dt, dev)
+        _refuse_overlap(out, x, "x")
+        _refuse_overlap(out, w, "w")
+        _refuse_overlap(out, bias, "bias")
+        if residual is not None and (residual.data_ptr(), residual.stride()) != (out.data_ptr(), out.stride()):
+            _refuse_overlap(out, residual, "residual other than as the same view")
     if rows:
         p.y = out.data_ptr()
         _native.expert_linear(p, dev)
@@ -127,15 +151,15 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None
 
     x [rows, k], w [experts, k, n], bias [experts, n], residual and y [rows, n].  ``gated``: w holds the gate's
     columns and then the up projection's, y = act(gate) * up + residual has n / 2 columns.  ``activation``: None,
-    "relu", "silu" or "gelu" (the error-function form).  ``out`` may be the residual itself.
+    "relu", "silu" or "gelu" (the error-function form).  ``out`` may be the residual itself, and overlaps no operand otherwise.
     """
-    return _linear(_product(x, w, offsets, bias, activation, gated), x, residual, out)
+    return _linear(_product(x, w, offsets, bias, activation, gated), x, w, bias, residual, out)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
            gated: bool = False, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """act(x w + bias) + residual with one matrix w [k, n] and bias [n]; see :func:`expert_linear`."""
-    return _linear(_product(x, w, None, bias, activation, gated, dense=True), x, residual, out)
+    return _linear(_product(x, w, None, bias, activation, gated, dense=True), x, w, bias, residual, out)
 
 
 def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *,

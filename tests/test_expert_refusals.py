@@ -54,6 +54,27 @@ def test_linear_and_gradient_refuse():
         experts.expert_linear_grad(fake(4, 5), fake(4, 8), fake(1, 8, 6), None)
 
 
+def test_overlapping_results_are_refused():
+    buf = fake(64)
+    wide = fake(6, 24)
+    w = fake(8, 8)
+    for x, residual, out in ((buf[:32].view(4, 8), None, buf[8:40].view(4, 8)), (wide[:4, :8], None, wide[:4, 4:12]),
+                             (wide[:4, :8], None, wide[1:5, :8]), (buf[:32].view(4, 8), None, buf[:32].view(4, 8)),
+                             (fake(4, 8), buf[:32].view(4, 8), buf[8:40].view(4, 8)), (w[:4], None, w[4:]),
+                             (fake(4, 8), None, w[:4])):
+        with pytest.raises(ValueError, match="overlap"):
+            experts.linear(x, w, residual=residual, out=out)
+    with pytest.raises(ValueError, match="overlap bias"):
+        experts.linear(fake(4, 8), w, bias=buf[20:28], out=buf[:32].view(4, 8))
+    for x, residual, out in ((wide[:4, :8], None, wide[:4, 8:16]), (wide[:4, 16:], None, wide[:4, 8:16]),
+                             (buf[:32].view(4, 8), None, buf[32:].view(4, 8)), (wide[:1, :8], None, wide[1:2, 2:10]),
+                             (wide[:4, :8], wide[:4, 8:16], wide[:4, 8:16]), (wide[:4, 8:16], None, wide[1:5, 16:])):
+        experts._refuse_overlap(out, x, "x")
+        if residual is not None:
+            with pytest.raises(ValueError, match="overlap"):
+                experts._refuse_overlap(out, residual, "residual")
+
+
 def _product(**kw):
     p = _native.ExpertProduct(x=64, w=64, y=64, rows=4, k=8, n=6, experts=1, ldx=8, w_stride_e=48, w_stride_k=6, w_stride_n=1,
                               ldy=6)

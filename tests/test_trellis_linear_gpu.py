@@ -127,6 +127,9 @@ def test_scales_of_rows(cuda_device):
     x, t, suh, svh, off = make([8, 30], 256, 256, 4, torch.bfloat16, cuda_device, seed=6)
     x[0], x[1], x[2], x[3] = 0, x[1] * 2.0 ** -60, x[2] * 2.0 ** 60, x[3] * 2.0 ** 20
     x[4, 17], x[9, 200] = 3e4, -2e5
+    x[5] = torch.sign(x[5]) * 1e38                     # the transform of these would leave the fp32 range
+    suh[0] *= 0.5
+    svh[0] *= 2.0 ** -10
     y = experts.trellis_linear(x, t, suh, svh, off)
     want, bound = expect(x, t, suh, svh, off, None)
     check(y, want, bound)
