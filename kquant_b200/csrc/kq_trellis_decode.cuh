@@ -121,4 +121,25 @@ int few_trellis_k34(const FewTrellis& p, int bits, int dec, bool wide, cudaStrea
 int few_trellis_k56(const FewTrellis& p, int bits, int dec, bool wide, cudaStream_t s);
 int few_trellis_k78(const FewTrellis& p, int bits, int dec, bool wide, cudaStream_t s);
 
+// Rows product of many rows; y bf16 or fp16.
+struct TrellisRows {
+    const uint32_t* trellis;
+    const void* table;
+    const int64_t* offsets;
+    const uint16_t* xr;        // [rows][k] binary16
+    const __half* svh;
+    const float* row_scale;
+    void* y;
+    int64_t svh_stride, ldy;
+    int rows, experts, k, n;
+    int* err;
+    bool bf16, vec_svh, vec_y, zero_rest;
+};
+
+// DEC_MCG and DEC_E4M3: a binary16 table and the stages do not fit in shared memory together.
+int rows_trellis_k12(const TrellisRows& p, int bits, int dec, cudaStream_t s);
+int rows_trellis_k34(const TrellisRows& p, int bits, int dec, cudaStream_t s);
+int rows_trellis_k56(const TrellisRows& p, int bits, int dec, cudaStream_t s);
+int rows_trellis_k78(const TrellisRows& p, int bits, int dec, cudaStream_t s);
+
 }  // namespace kq

@@ -12,11 +12,12 @@
 // bits of x and y.  Products are summed in fp32, the output transform runs in
 // fp32, and y is rounded once.
 //
-// With few rows an expert (rows_are_few), the payload is decoded in registers next
-// to the product (kq_trellis_few.cuh) and partial sums over ranges of k are
-// added up by the output transform.  With more rows it is decoded once, to
-// binary16 in the workspace, and the tensor-core product with the rotation in
-// its epilogue reads that (kq_expert_rotated.cu).
+// With few rows an expert, the payload is decoded in registers next to the
+// product (kq_trellis_few.cuh) and partial sums over ranges of k are added up
+// by the output transform.  With more it is decoded into the tensor core's
+// tiles (kq_trellis_rows.cuh); with many it is decoded once, to binary16 in
+// the workspace, and the tensor-core product with the rotation in its epilogue
+// reads that (kq_expert_rotated.cu).
 #include "kq_expert_rows.cuh"
 #include "kq_trellis_decode.cuh"
 
@@ -262,26 +263,37 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
     }
 }
 
-// Decoding next to the product costs time per 16 rows of every expert; decoding once costs the same for any number of them,
-// and its product leaves most SMs idle when it has few tiles of 128 columns.  8 experts of 7168 x 4096 at 4 bits, a mean of
-// 16 / 32 / 48 / 64 rows: 196 / 205 / 226 / 272 us against 232 to 243 (MCG), 220 / 260 / 318 / 369 against 278 to 291 (E4M3
-// labels), 295 / 307 / 334 / 375 against 347 to 359 (a table of labels).  One of 7168 x 2048 (16 tiles), 16 / 64 / 96 rows:
-// 25 / 31 / 44 against 56 to 58 us.
-bool rows_are_few(const kq_trellis_product& p) {
-    const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
-    return p.rows <= (p.n / 128 * busy <= 64 ? 96 : 40) * busy;
+// Three ways, for MCG (and E4M3) at 4 bits, us by the mean of rows an expert:
+//   few: in registers for mma.sync, k split over CTAs; costs what the weights' decoding costs, once per 16 or 64 rows.
+//   fused: in shared memory for the tensor core, once per 256 rows; a tile of 256 rows x 128 columns takes all of k, so 64
+//     tiles leave more than half of the SMs idle.
+//   decoded once to the workspace, then the product; reading and writing binary16, whatever the rows.
+// 8 experts of 7168 x 4096:    8 rows 113 (144) / 152 (189) / 233 (277);  16 rows 207 (220) / 152 (189) / 233 (278);
+//   256 rows  - / 222 (240) / 290 (336);  384 rows  - / 405 (438) / 345 (388).
+// 8 of 2048 x 7168: 8 rows 64 (81) / 92 (112) / 124 (150);  256 rows  - / 135 (149) / 158 (181).
+// One of 7168 x 2048 (16 tiles): 64 rows 31 (37) / 80 (98) / 58 (62);  128 rows 46 (58) / 80 (98) / 59 (63).
+// Uneven experts have more row tiles than their mean says, so the fused way ends before 256.  A binary16 table leaves no room
+// for its stages; 8 of 7168 x 4096 from such a table: few 295 / 307 / 334 / 375 us at 16 / 32 / 48 / 64 rows, decoded once
+// 347 to 359.
+enum Way { FEW, FUSED, ONCE };
+
+Way way_of(const kq_trellis_product& p) {
+    const int64_t busy = p.experts < p.rows ? p.experts : p.rows, tiles = p.n / 128 * busy;
+    if (tiles <= 64) return p.rows <= 96 * busy ? FEW : ONCE;
+    if (p.codebook == KQ_CB_LABELS) return p.rows <= 40 * busy ? FEW : ONCE;
+    return p.rows <= 8 * busy ? FEW : p.rows <= 192 * busy ? FUSED : ONCE;
 }
 
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
-struct Plan { bool few, wide; int parts; int64_t scale, rest, bytes; };
+struct Plan { Way way; bool wide; int parts; int64_t scale, rest, bytes; };
 
 int few_ctas(const kq_trellis_product& p, int sms) { return sms * (p.codebook == KQ_CB_LABELS ? 1 : 2); }   // a table of 128 KB leaves room for one
 
 Plan plan(const kq_trellis_product& p) {
     Plan l{};
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
-    l.few = rows_are_few(p);
+    l.way = way_of(p);
     l.wide = p.rows > 8 * busy;
     // Parts of a strip: what an even share of a single row tile makes on 148 SMs, within 256 MB (two at least).
     const int64_t kt = p.k / 16, strips = p.n / few_columns(l.wide), one = p.rows * p.n * 4;
@@ -290,7 +302,7 @@ Plan plan(const kq_trellis_product& p) {
     l.parts = (int)(most < fit ? most : fit < 2 ? 2 : fit);
     l.scale = align128(p.rows * p.k * 2);
     l.rest = l.scale + align128(p.rows * 4);
-    l.bytes = l.rest + (l.few ? (int64_t)l.parts * one : p.experts * p.k * p.n * 2);
+    l.bytes = l.rest + (l.way == FEW ? (int64_t)l.parts * one : l.way == FUSED ? 0 : p.experts * p.k * p.n * 2);
     return l;
 }
 
@@ -391,7 +403,7 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
     float* scale = reinterpret_cast<float*>(ws + l.scale);
     const bool bf16 = p.dtype == KQ_BF16;
     if (int rc = bf16 ? rotate_in<__nv_bfloat16>(p, xr, scale, s) : rotate_in<__half>(p, xr, scale, s)) return rc;
-    if (l.few) {
+    if (l.way == FEW) {
         int sms;
         if (int rc = sm_count(&sms)) return rc;
         float* partial = reinterpret_cast<float*>(ws + l.rest);
@@ -410,6 +422,16 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
             rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
                                                    (int)p.n, static_cast<__half*>(p.y), p.ldy, p.zero_rest != 0);
         return check_launch("rotate_out_kernel");
+    }
+    if (l.way == FUSED) {
+        TrellisRows r{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr),
+                      reinterpret_cast<const __half*>(p.svh), scale, p.y, p.svh_stride_e, p.ldy, (int)p.rows, (int)p.experts, (int)p.k,
+                      (int)p.n, nullptr, bf16, ((uintptr_t)p.svh & 15) == 0 && p.svh_stride_e % 8 == 0,
+                      ((uintptr_t)p.y & 15) == 0 && p.ldy % 8 == 0, p.zero_rest != 0};
+        if (int rc = wait_error_word(&r.err)) return rc;
+        const int dec = p.codebook == KQ_CB_MCG ? DEC_MCG : DEC_E4M3;
+        return p.bits <= 2 ? rows_trellis_k12(r, p.bits, dec, s) : p.bits <= 4 ? rows_trellis_k34(r, p.bits, dec, s)
+             : p.bits <= 6 ? rows_trellis_k56(r, p.bits, dec, s) : rows_trellis_k78(r, p.bits, dec, s);
     }
     __half* w = reinterpret_cast<__half*>(ws + l.rest);
     if (int rc = decode_all(p, w, s)) return rc;

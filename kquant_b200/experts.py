@@ -185,7 +185,12 @@ def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offse
         dz = dy.new_empty((0, n))
     dx = dw = db = None
     if need_dx:
-        dx = expert_linear(dz, w.transpose(1, 2), offsets)
+        dx = torch.empty((p.rows, k), dtype=dt, device=dev)
+        if p.rows:                                  # dz w^T: the product with in and out exchanged
+            q = _native.ExpertProduct(x=dz.data_ptr(), w=p.w, offsets=p.offsets, y=dx.data_ptr(), rows=p.rows, k=n, n=k, experts=E,
+                                      ldx=dz.stride(0), w_stride_e=p.w_stride_e, w_stride_k=p.w_stride_n, w_stride_n=p.w_stride_k,
+                                      ldy=k, dtype=p.dtype, zero_rest=1)
+            _native.expert_linear(q, dev)
     if need_dw:
         n_major = not (w.stride(2) != 1 and w.stride(1) == 1)
         dw = torch.empty((E, k, n), dtype=dt, device=dev) if n_major else \

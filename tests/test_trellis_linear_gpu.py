@@ -184,3 +184,73 @@ def test_no_rows(cuda_device):
     assert experts.trellis_linear(x, t, suh, svh, off).shape == (0, 128)
     x = torch.randn((4, 128), device=cuda_device).bfloat16()
     assert not experts.trellis_linear(x, t, suh, svh, off).any()
+
+
+@pytest.mark.parametrize("K", RATES)
+@pytest.mark.parametrize("book", ["mcg", "e4m3"])
+@pytest.mark.parametrize("counts,k,n", [([300, 0, 1, 70, 129, 256], 256, 1920), ([9, 17, 1] * 11, 384, 256), ([12], 128, 8320)])
+def test_middling_rows(cuda_device, K, book, counts, k, n):
+    """More than a few rows an expert and enough columns: decoded into the tensor core's tiles."""
+    for dtype in (torch.bfloat16, torch.float16):
+        x, t, suh, svh, off = make(counts, k, n, K, dtype, cuda_device, seed=10 + K)
+        cb = tables(cuda_device)[book]
+        y = experts.trellis_linear(x, t, suh, svh, off, codebook=cb)
+        want, bound = expect(x, t, suh, svh, off, cb)
+        check(y, want, bound)
+        near(y, want)
+    _native.check_wait_errors(cuda_device)
+
+
+def test_middling_rows_views_replay_and_nan(cuda_device):
+    """Rows of no expert kept or zeroed, odd strides and bases, NaN confined to its row, new offsets at replay."""
+    counts, k, n = [40, 0, 33, 260, 5], 384, 1792
+    x, t, suh, svh, off = make(counts, k, n, 4, torch.float16, cuda_device, seed=3, spare=5, first=3)
+    wide = torch.full((x.shape[0], k + 7), float("nan"), dtype=x.dtype, device=cuda_device)
+    wide[:, 3:3 + k].copy_(x)
+    x = wide[:, 3:3 + k]
+    x[off[1] - 2, 5] = float("nan")
+    x[-2, 7] = float("inf")                                # behind the last expert
+    buf = torch.full((x.shape[0], n + 9), 7.0, dtype=x.dtype, device=cuda_device)
+    out = buf[:, 1:1 + n]
+    assert experts.trellis_linear(x, t, suh, svh, off, out=out) is out
+    fresh = experts.trellis_linear(x, t, suh, svh, off)
+    a, b = int(off[0]), int(off[-1])
+    keep = torch.ones(x.shape[0], dtype=torch.bool, device=cuda_device)
+    keep[off[1] - 2] = False
+    assert torch.isnan(fresh[~keep]).all()
+    clean = x.clone()
+    clean[~keep] = 0
+    want, bound = expect(clean, t, suh, svh, off, None)
+    want[a:b][~keep[a:b]] = float("nan")
+    inside = keep.clone()
+    inside[:a], inside[b:] = False, False
+    check(fresh[inside], want[inside], bound[inside])
+    assert torch.equal(out[inside], fresh[inside])
+    assert not fresh[:a].any() and not fresh[b:].any()
+    assert (buf[:, 0] == 7).all() and (buf[:, 1 + n:] == 7).all() and (out[:a] == 7).all() and (out[b:] == 7).all()
+
+    x = torch.randn((64, k), device=cuda_device).half()
+    off = offsets_of([20, 14, 10, 12, 8], cuda_device)
+    run = lambda: experts.trellis_linear(x, t, suh, svh, off)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for new in ([64, 0, 0, 0, 0], [0, 0, 0, 0, 0], [1, 1, 1, 1, 1], [0, 30, 0, 34, 0]):
+        off.copy_(offsets_of(new, cuda_device))
+        graph.replay()
+        assert torch.equal(got, run())
+        want, bound = expect(x, t, suh, svh, off, None)
+        check(got[:sum(new)], want[:sum(new)], bound[:sum(new)])
+    _native.check_wait_errors(cuda_device)
+
+
+def test_every_way_gives_the_same_sums(cuda_device):
+    """Row counts on both sides of each choice of kernel."""
+    for book, counts, n in (("mcg", [8, 8], 4224), ("mcg", [9, 9], 4224), ("e4m3", [192, 192], 4224), ("e4m3", [193, 193], 4224),
+                            ("mcg", [96], 8192), ("mcg", [97], 8192), ("labels", [40, 40], 4224), ("labels", [41, 41], 4224)):
+        x, t, suh, svh, off = make(counts, 256, n, 3, torch.bfloat16, cuda_device, seed=5)
+        cb = tables(cuda_device)[book]
+        y = experts.trellis_linear(x, t, suh, svh, off, codebook=cb)
+        check(y, *expect(x, t, suh, svh, off, cb))
