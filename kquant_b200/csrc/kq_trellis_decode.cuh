@@ -14,6 +14,29 @@
 
 namespace kq {
 
+// The kernels of one call follow one another by programmatic launch: a kernel lets the next one start (its tables, its words of
+// the payload, its first tiles), which waits for everything before it where it needs it, and at its end at the latest, so that
+// a kernel's end is the end of all before it.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+int launch_next(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, const char* what, const A&... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = (size_t)smem;
+    c.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+    if (e != cudaSuccess) { set_error("%s: %s", what, cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+    return check_launch(what);
+}
+
 enum { DEC_MCG, DEC_E4M3, DEC_F16 };
 constexpr int kBlock = 128;    // channels of a Hadamard block
 

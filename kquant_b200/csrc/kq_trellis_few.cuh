@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(few_warps<RT>() * 32, DEC == DEC_F16 ? 1 : 2) 
     int* cum = reinterpret_cast<int*>(sums + WARPS / 2 * few_part<RT>());
     static_assert(WARPS / 2 * few_part<RT>() >= 2 * kMaxExperts, "the scan borrows the sums");
     int* first = reinterpret_cast<int*>(sums);
+    let_next_start();
     load_table<DEC>(p.table, smem);
     scan_groups(p.offsets, p.experts, p.rows, RT * 16, first, first + kMaxExperts, cum);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3;
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(few_warps<RT>() * 32, DEC == DEC_F16 ? 1 : 2) 
         };
         fetch(ka + warp, ahead[0]);
         fetch(ka + warp + WARPS, ahead[1]);
+        wait_for_last();                         // x' is there; plain loads of it, which stay behind this
         const uint16_t* xp = p.xr + (int64_t)(row0 + (lane >> 2)) * p.k + 2 * q;
         auto step = [&](int kk, TileWords<K> (&w)[NT]) {
             uint32_t a[RT][4];
@@ -75,10 +77,10 @@ __global__ void __launch_bounds__(few_warps<RT>() * 32, DEC == DEC_F16 ? 1 : 2) 
             for (int r = 0; r < RT; ++r) {
                 const uint16_t* x = xp + (int64_t)r * 16 * p.k + kk * 16;
                 const bool top = r * 16 + (lane >> 2) < count, low = r * 16 + 8 + (lane >> 2) < count;
-                a[r][0] = top ? __ldg(reinterpret_cast<const uint32_t*>(x)) : 0u;
-                a[r][1] = low ? __ldg(reinterpret_cast<const uint32_t*>(x + 8 * (int64_t)p.k)) : 0u;
-                a[r][2] = top ? __ldg(reinterpret_cast<const uint32_t*>(x + 8)) : 0u;
-                a[r][3] = low ? __ldg(reinterpret_cast<const uint32_t*>(x + 8 * (int64_t)p.k + 8)) : 0u;
+                a[r][0] = top ? *reinterpret_cast<const uint32_t*>(x) : 0u;
+                a[r][1] = low ? *reinterpret_cast<const uint32_t*>(x + 8 * (int64_t)p.k) : 0u;
+                a[r][2] = top ? *reinterpret_cast<const uint32_t*>(x + 8) : 0u;
+                a[r][3] = low ? *reinterpret_cast<const uint32_t*>(x + 8 * (int64_t)p.k + 8) : 0u;
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -123,6 +125,7 @@ __global__ void __launch_bounds__(few_warps<RT>() * 32, DEC == DEC_F16 ? 1 : 2) 
             p.partial[((int64_t)part * p.rows + row0 + r) * p.n + strip * COLS + c] = v;
         }
     }
+    wait_for_last();
 }
 
 template <int K, int DEC, int RT>
@@ -133,8 +136,7 @@ int launch_few(const FewTrellis& p, cudaStream_t s) {
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    kernel<<<sms * (DEC == DEC_F16 ? 1 : 2), few_warps<RT>() * 32, smem, s>>>(p);
-    return check_launch("few_trellis_kernel");
+    return launch_next(kernel, sms * (DEC == DEC_F16 ? 1 : 2), few_warps<RT>() * 32, smem, s, "few_trellis_kernel", p);
 }
 
 template <int K>

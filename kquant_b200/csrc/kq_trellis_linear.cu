@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(WARPS * 32) rotate_in_kernel(const T* __restri
                                                         int experts, int k, __half* __restrict__ xr, float* __restrict__ scale) {
     constexpr int HELD = 4;
     __shared__ float most[WARPS];
+    let_next_start();
     const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = k / kBlock;
     const int e = place_of_row(offsets, experts, rows, row, 1).e;
     if (e < 0) return;
@@ -158,17 +159,25 @@ __global__ void __launch_bounds__(WARPS * 32) rotate_in_kernel(const T* __restri
     if (threadIdx.x == 0) scale[row] = ldexpf(1.f, -ex);
 }
 
+// Four floats that are read once; not before wait_for_last.
+__device__ __forceinline__ float4 load_once(const float* p) {
+    float4 v;
+    asm volatile("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // y = had(sum of the partial sums) * svh * 2^-s; a warp a Hadamard block of one row.  Rows of no expert: zeros in a fresh
 // output.
 template <typename T>
-__global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict__ partial, int parts, int ctas, int kt, bool wide,
-                                                         const float* __restrict__ scale,
+__global__ void __launch_bounds__(256) rotate_out_kernel(const float* partial, int parts, int ctas, int kt, bool wide,
+                                                         const float* scale,
                                                          const __half* __restrict__ svh, int64_t svh_stride,
                                                          const int64_t* __restrict__ offsets, int rows, int experts, int n,
                                                          T* __restrict__ y, int64_t ldy, bool zero_rest) {
     const int row = blockIdx.x, lane = threadIdx.x & 31, blk = blockIdx.y * 8 + (threadIdx.x >> 5);
     const Place at = place_of_row(offsets, experts, rows, row, wide ? kFewRows : 16);
     const int e = at.e;
+    wait_for_last();
     if (blk >= n / kBlock || (e < 0 && !zero_rest)) return;
     const int j = blk * kBlock + lane * 4;
     T* o = y + (int64_t)row * ldy + j;
@@ -185,7 +194,7 @@ __global__ void __launch_bounds__(256) rotate_out_kernel(const float* __restrict
     const int mine = (int)((first + kt - 1) / per - first / per) + 1;
 #pragma unroll 4
     for (int s = 0; s < mine; ++s) {
-        const float4 q = __ldcs(reinterpret_cast<const float4*>(partial + ((int64_t)s * rows + row) * n + j));
+        const float4 q = load_once(partial + ((int64_t)s * rows + row) * n + j);
         v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
     }
     had128_warp(v, lane);
@@ -261,6 +270,7 @@ __global__ void __launch_bounds__(256) decode_kernel(const uint32_t* __restrict_
         }
         __syncwarp();
     }
+    wait_for_last();
 }
 
 // Three ways, for MCG (and E4M3) at 4 bits, us by the mean of rows an expert:
@@ -334,9 +344,9 @@ int launch_decode(const kq_trellis_product& p, __half* out, cudaStream_t s) {
     const int64_t items = (p.n / DN) * (p.k / DK) * p.experts;
     const int per_sm = DEC == DEC_F16 ? 1 : DEC == DEC_E4M3 ? 2 : 8;
     const int grid = (int)(items < (int64_t)sms * per_sm ? items : (int64_t)sms * per_sm);
-    decode_kernel<K, DEC><<<grid, 256, smem, s>>>(reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, (int)p.rows,
-                                                  (int)p.experts, (int)p.k, (int)p.n, out);
-    return check_launch("decode_kernel");
+    return launch_next(decode_kernel<K, DEC>, dim3((unsigned)grid), 256, smem, s, "decode_kernel",
+                       reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, (int)p.n,
+                       out);
 }
 
 template <int K>
@@ -415,13 +425,12 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         if (rc) return rc;
         const dim3 grid((unsigned)p.rows, (unsigned)((p.n / kBlock + 7) / 8));
         const __half* svh = reinterpret_cast<const __half*>(p.svh);
-        if (bf16)
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
-                                                   (int)p.n, static_cast<__nv_bfloat16*>(p.y), p.ldy, p.zero_rest != 0);
-        else
-            rotate_out_kernel<<<grid, 256, 0, s>>>(partial, l.parts, few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows, (int)p.experts,
-                                                   (int)p.n, static_cast<__half*>(p.y), p.ldy, p.zero_rest != 0);
-        return check_launch("rotate_out_kernel");
+        auto out = [&](auto* y) {
+            return launch_next(rotate_out_kernel<std::remove_pointer_t<decltype(y)>>, grid, 256, 0, s, "rotate_out_kernel", partial, l.parts,
+                               few_ctas(p, sms), (int)(p.k / 16), l.wide, scale, svh, p.svh_stride_e, p.offsets, (int)p.rows,
+                               (int)p.experts, (int)p.n, y, p.ldy, p.zero_rest != 0);
+        };
+        return bf16 ? out(static_cast<__nv_bfloat16*>(p.y)) : out(static_cast<__half*>(p.y));
     }
     if (l.way == FUSED) {
         TrellisRows r{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr),

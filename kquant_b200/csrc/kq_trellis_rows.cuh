@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(R_THREADS, 1) rows_trellis_kernel(const __grid
 
     if (warp == 0) {
         if (lane == 0) {
+            wait_for_last();                     // x' is there
             uint32_t it = 0;
             for (int64_t i = blockIdx.x; ok && rows_tile(p, lo, cnt, cum, i, t); i += gridDim.x) {
                 const bool two = t.count > RM;
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(R_THREADS, 1) rows_trellis_kernel(const __grid
             const int b = tile_no & 1;
             if (!(ok = __all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[b], (tile_no >> 1) & 1)))) break;
             tc_fence_after();
+            wait_for_last();                     // row_scale, as this thread sees it
             const __half* svh = p.svh + t.e * p.svh_stride + t.n0;
             for (int m = 0; m < (t.count > RM ? 2 : 1); ++m) {
                 const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * 2 * RN + m * RN);
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(R_THREADS, 1) rows_trellis_kernel(const __grid
         }
     }
     tc_fence_before();
+    wait_for_last();
     __syncthreads();
     if (warp == 1) tmem_free(tmem, 512);
 }
@@ -275,8 +278,7 @@ int launch_rows(const TrellisRows& p, cudaStream_t s) {
     if (int rc = sm_count(&sms)) return rc;
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows;
     const int64_t most = (busy + (p.rows - busy) / (2 * RM)) * (p.n / RN);
-    kernel<<<(unsigned)(most < sms ? most : sms), R_THREADS, smem, s>>>(map, p);
-    return check_launch(what);
+    return launch_next(kernel, dim3((unsigned)(most < sms ? most : sms)), R_THREADS, smem, s, what, map, p);
 }
 
 template <int K>
