@@ -838,7 +838,7 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     if ((uintptr_t)workspace & 15) { set_error("%s: workspace must be 16-byte aligned", what); return KQ_ERR_ALIGN; }
     uint16_t* ws = static_cast<uint16_t*>(workspace);
     // A lane takes a line of dW (and stores 32 bytes at a time) where lines start on 16 bytes, else a column (2 bytes, 64 a warp):
-    // dW of 7168 x 4096, 8 experts, 4096 rows: LINES_US against 362 us.
+    // dW of 7168 x 4096, 8 experts, 4096 uneven rows: 313 us against 362.
     SumsSides o = sums_sides(p, dz, ld_dz);
     const bool by_line = (((uintptr_t)dw | (uintptr_t)(ld * 2) | (uintptr_t)(p.experts > 1 ? p.w_stride_e * 2 : 0)) & 15) == 0;
     const bool wide = (((uintptr_t)dw | (uintptr_t)(ld * 2) | (uintptr_t)(p.experts > 1 ? p.w_stride_e * 2 : 0)) & 31) == 0;
