@@ -296,10 +296,12 @@ int kq_reconstruct_rotated(const float* wq, const float* su, const float* sv, in
  *                               z; y receives dz [rows x n]
  *     kq_expert_weight_grad:    dW_e = x_e^T dz_e, in W's strides (every
  *                               expert is written, zeros where it has no rows)
- *     kq_expert_bias_grad:      db_e = the column sums of dz_e
+ *     kq_expert_bias_grad:      db_e = the column sums of dz_e + dz_low_e (dz_low may be NULL)
  *
  * The gradient in x is kq_expert_linear on dz with W's strides exchanged.
  * Rows of no expert are left as they were, or zeroed with zero_rest.
+ * The calls after kq_expert_linear_grad_z take dz as rounded; db alone takes it
+ * with what the rounding left out.
  * bias and residual may be NULL.  At most 1024 experts.
  */
 typedef struct {
@@ -314,6 +316,7 @@ typedef struct {
     int64_t w_stride_e, w_stride_k, w_stride_n;
     int64_t bias_stride_e, ld_residual, ldy;
     int32_t dtype, activation, gated, zero_rest;
+    void* y_low;                 /* kq_expert_linear_grad_z: dz - its rounding, row stride ldy; may be NULL */
 } kq_expert_product;
 
 size_t kq_expert_linear_workspace_bytes(const kq_expert_product* p);
@@ -323,8 +326,8 @@ int kq_expert_linear_grad_z(const kq_expert_product* p, const void* dy, int64_t 
 size_t kq_expert_weight_grad_workspace_bytes(const kq_expert_product* p, const void* dz, int64_t ld_dz);
 int kq_expert_weight_grad(const kq_expert_product* p, const void* dz, int64_t ld_dz, void* dw, void* workspace,
                           size_t workspace_bytes, void* stream);
-int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n, int64_t experts,
-                        int dtype, void* db, int64_t db_stride_e, void* stream);
+int kq_expert_bias_grad(const void* dz, const void* dz_low, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n,
+                        int64_t experts, int dtype, void* db, int64_t db_stride_e, void* stream);
 
 /*
  * Calibration Hessians of all experts at once (kquant/capture.py:713-730,

@@ -76,7 +76,7 @@ class ExpertProduct(ctypes.Structure):
                 ("w_stride_e", ctypes.c_int64), ("w_stride_k", ctypes.c_int64), ("w_stride_n", ctypes.c_int64),
                 ("bias_stride_e", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ldy", ctypes.c_int64),
                 ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("gated", ctypes.c_int32),
-                ("zero_rest", ctypes.c_int32)]
+                ("zero_rest", ctypes.c_int32), ("y_low", ctypes.c_void_p)]
 
 
 class TrellisProduct(ctypes.Structure):
@@ -141,7 +141,7 @@ def load() -> ctypes.CDLL:
         L.kq_expert_weight_grad_workspace_bytes.argtypes = [EP, P, I64]
         L.kq_expert_weight_grad_workspace_bytes.restype = SZ
         L.kq_expert_weight_grad.argtypes = [EP, P, I64, P, P, SZ, P]
-        L.kq_expert_bias_grad.argtypes = [P, I64, P, I64, I64, I64, I, P, I64, P]
+        L.kq_expert_bias_grad.argtypes = [P, P, I64, P, I64, I64, I64, I, P, I64, P]
         L.kq_wait_errors.argtypes = [P, P]
         TP = ctypes.POINTER(TrellisProduct)
         L.kq_trellis_linear_workspace_bytes.argtypes = [TP]
@@ -559,9 +559,9 @@ def expert_weight_grad(p: ExpertProduct, dz: torch.Tensor, dw: torch.Tensor, dev
     stats.launches += 1
 
 
-def expert_bias_grad(dz: torch.Tensor, offsets: torch.Tensor | None, db: torch.Tensor, dtype: int) -> None:
+def expert_bias_grad(dz: torch.Tensor, low: torch.Tensor | None, offsets: torch.Tensor | None, db: torch.Tensor, dtype: int) -> None:
     def fn(ws, need, stream):
-        return load().kq_expert_bias_grad(dz.data_ptr(), dz.stride(0), None if offsets is None else offsets.data_ptr(), dz.shape[0],
+        return load().kq_expert_bias_grad(dz.data_ptr(), None if low is None else low.data_ptr(), dz.stride(0), None if offsets is None else offsets.data_ptr(), dz.shape[0],
                                           dz.shape[1], db.shape[0], dtype, db.data_ptr(), db.stride(0), stream)
     _call(dz.device, "kq_expert_bias_grad", 0, fn)
     stats.launches += 1

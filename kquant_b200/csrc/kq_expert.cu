@@ -61,7 +61,7 @@ struct Params {
     const int64_t* offsets;
     const void* bias;
     const void* aux;       // residual (forward) or dy (gradient)
-    void* out;
+    void *out, *low;       // low (gradient): what the rounding of dz leaves out, or null
     int64_t bias_stride, ld_aux, ld_out, out_stride;   // out_stride: per expert (sums)
     int rows, experts, k_steps, m_tiles, n_tiles;
     int m_out, n_out;      // output extents: features, and (sums) rows
@@ -448,6 +448,16 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     store_rows(out + (int64_t)c * p.ld_out, p.ld_out, live ? n - c : 0, z);
                     if constexpr (EPI == EPI_GRAD && GATED)
                         store_rows(out + (int64_t)c * p.ld_out + p.m_out, p.ld_out, live ? n - c : 0, u);
+                    if (EPI == EPI_GRAD && p.low) {
+                        T* low = static_cast<T*>(p.low) + (out - static_cast<T*>(p.out)) + (int64_t)c * p.ld_out;
+#pragma unroll
+                        for (int j = 0; j < TR; ++j) {
+                            z[j] = left_out<T>(z[j]);
+                            if constexpr (GATED) u[j] = left_out<T>(u[j]);
+                        }
+                        store_rows(low, p.ld_out, live ? n - c : 0, z);
+                        if constexpr (GATED) store_rows(low + p.m_out, p.ld_out, live ? n - c : 0, u);
+                    }
                     tmem_wait_ld();
                 }
             }
@@ -512,11 +522,11 @@ __global__ void __launch_bounds__(256) relayout_kernel(const Copies copies) {
     }
 }
 
-// Column sums of dz over every expert's rows, fp32 in row order within a
+// Column sums of dz (and of what its rounding left out) over every expert's rows, fp32 in row order within a
 // thread: one warp per 32 columns and expert, rows split over 8 warps.
 template <typename T>
 __global__ void __launch_bounds__(256)
-bias_grad_kernel(const T* __restrict__ dz, int64_t ld, const int64_t* __restrict__ offsets, int rows, int n, T* __restrict__ db,
+bias_grad_kernel(const T* __restrict__ dz, const T* __restrict__ low, int64_t ld, const int64_t* __restrict__ offsets, int rows, int n, T* __restrict__ db,
                  int64_t db_stride) {
     __shared__ float part[8][32];
     const int e = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -525,7 +535,10 @@ bias_grad_kernel(const T* __restrict__ dz, int64_t ld, const int64_t* __restrict
     group_of(offsets, e, rows, lo, count);
     float s = 0.f;
     if (j < n)
-        for (int r = w; r < count; r += 8) s += to_f<T>(dz[(int64_t)(lo + r) * ld + j]);
+        for (int r = w; r < count; r += 8) {
+            const int64_t at = (int64_t)(lo + r) * ld + j;
+            s += to_f<T>(dz[at]) + (low ? to_f<T>(low[at]) : 0.f);
+        }
     part[w][lane] = s;
     __syncthreads();
     if (w == 0 && j < n) {
@@ -688,6 +701,7 @@ int many_rows_product(const RowsProduct& p, cudaStream_t s) {
     q.bias = p.bias;
     q.aux = p.aux;
     q.out = p.out;
+    q.low = p.low;
     q.bias_stride = p.bias_stride;
     q.ld_aux = p.ld_aux;
     q.ld_out = p.ld_out;
@@ -736,6 +750,7 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     r.bias = p.bias;
     r.aux = grad ? dy : p.residual;
     r.out = p.y;
+    r.low = grad ? p.y_low : nullptr;
     r.bias_stride = p.bias_stride_e;
     r.ld_aux = grad ? ld_dy : p.ld_residual;
     r.ld_out = p.ldy;
@@ -876,7 +891,7 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     return launch<EPI_SUMS, false>(bf16, ma, mb, mb, q, (int64_t)q.m_tiles * q.n_tiles * p.experts, s);
 }
 
-extern "C" int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n,
+extern "C" int kq_expert_bias_grad(const void* dz, const void* dz_low, int64_t ld_dz, const int64_t* offsets, int64_t rows, int64_t n,
                                    int64_t experts, int dtype, void* db, int64_t db_stride_e, void* stream) {
     using namespace kq;
     const char* what = "kq_expert_bias_grad";
@@ -888,10 +903,10 @@ extern "C" int kq_expert_bias_grad(const void* dz, int64_t ld_dz, const int64_t*
     const dim3 grid((unsigned)((n + 31) / 32), (unsigned)experts);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == KQ_BF16)
-        bias_grad_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(dz), ld_dz, offsets, (int)rows, (int)n,
+        bias_grad_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(dz), static_cast<const __nv_bfloat16*>(dz_low), ld_dz, offsets, (int)rows, (int)n,
                                               static_cast<__nv_bfloat16*>(db), db_stride_e);
     else
-        bias_grad_kernel<<<grid, 256, 0, s>>>(static_cast<const __half*>(dz), ld_dz, offsets, (int)rows, (int)n,
+        bias_grad_kernel<<<grid, 256, 0, s>>>(static_cast<const __half*>(dz), static_cast<const __half*>(dz_low), ld_dz, offsets, (int)rows, (int)n,
                                               static_cast<__half*>(db), db_stride_e);
     return check_launch(what);
 }

@@ -84,6 +84,13 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// What rounding v to T leaves out, itself rounded (nothing of what is not finite).
+template <typename T>
+__device__ __forceinline__ float left_out(float v) {
+    const float r = v - to_f<T>(from_f<T>(v));
+    return fabsf(r) <= 3.4e38f ? r : 0.f;
+}
+
 // 8 consecutive elements: one 16-byte access when `vec`, else the first `nv` one by one.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool vec, int nv, float (&f)[8]) {

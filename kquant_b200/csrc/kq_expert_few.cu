@@ -28,7 +28,7 @@ constexpr int PART = 32;                        // rows that are finished at a t
 struct Params {
     const int64_t* offsets;
     const void *bias, *aux;
-    void* out;
+    void *out, *low;
     int64_t bias_stride, ld_aux, ld_out;
     int rows, experts, k_steps, m_out, up, nt, box, stages, splits, act;
     uint32_t idesc, tmem_cols;   // idesc without N
@@ -235,15 +235,23 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     if (r + u * step >= n) break;
-                    T* o = static_cast<T*>(p.out) + (int64_t)(row0 + c0 + r + u * step) * p.ld_out + m0 + f;
+                    const int64_t to = (int64_t)(row0 + c0 + r + u * step) * p.ld_out + m0 + f;
+                    T *o = static_cast<T*>(p.out) + to, *low = static_cast<T*>(p.low) + to;
                     const float zz = z[u] + add, ww = w[u] + add_up;
                     if (!p.grad) {
                         o[0] = from_f<T>(act_of(p.act, zz) * (GATED ? ww : 1.f) + a[u]);
                     } else if constexpr (GATED) {
-                        o[0] = from_f<T>(a[u] * ww * slope_of(p.act, zz));
-                        o[p.m_out] = from_f<T>(a[u] * act_of(p.act, zz));
+                        const float dg = a[u] * ww * slope_of(p.act, zz), du = a[u] * act_of(p.act, zz);
+                        o[0] = from_f<T>(dg);
+                        o[p.m_out] = from_f<T>(du);
+                        if (p.low) {
+                            low[0] = from_f<T>(left_out<T>(dg));
+                            low[p.m_out] = from_f<T>(left_out<T>(du));
+                        }
                     } else {
-                        o[0] = from_f<T>(a[u] * slope_of(p.act, zz));
+                        const float dz = a[u] * slope_of(p.act, zz);
+                        o[0] = from_f<T>(dz);
+                        if (p.low) low[0] = from_f<T>(left_out<T>(dz));
                     }
                 }
             }
@@ -297,6 +305,7 @@ int few_rows_product(const RowsProduct& p, cudaStream_t s) {
     q.bias = p.bias;
     q.aux = p.aux;
     q.out = p.out;
+    q.low = p.low;
     q.bias_stride = p.bias_stride;
     q.ld_aux = p.ld_aux;
     q.ld_out = p.ld_out;

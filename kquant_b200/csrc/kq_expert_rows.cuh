@@ -43,6 +43,7 @@ struct RowsProduct {
     const int64_t* offsets;
     const void *bias, *aux;    // aux: residual or dy
     void* out;
+    void* low;                 // grad: what the rounding of dz leaves out, laid out as `out`; may be null
     int64_t bias_stride, ld_aux, ld_out;
     int64_t rows, k, n_out, experts;
     int up;                    // gated: first coordinate of the up half in W

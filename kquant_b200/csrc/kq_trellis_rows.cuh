@@ -9,6 +9,11 @@
 // take turns, a stage each, so that one waits for its words while the other
 // decodes.  Rows on the M axis put a row of a Hadamard block in one thread of
 // the epilogue, 32 columns at a time.
+//
+// Bound by the decoding's integer arithmetic (8 experts of 7168 x 4096 at 4
+// bits, 32 rows each: 152 us, the ALU pipe 68% busy, HBM 9%); with more than
+// 128 rows a tile the products' operands join in shared memory (256 rows: 222
+// us), which E4M3 lookups already use (189 and 240 us).
 #pragma once
 #include "kq_expert_rows.cuh"
 #include "kq_trellis_decode.cuh"

@@ -168,7 +168,7 @@ def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offse
     """Gradients (dx, dw, dbias) of :func:`expert_linear` for dy, the gradient of its result.
 
     The pre-activation z = x w + bias is recomputed where the activation needs it; dz (one rounding to the operands'
-    type) then feeds dx = dz w^T, dw[e] = x_e^T dz_e and dbias[e] = sum dz_e.  dw has w's layout; an expert without
+    type) then feeds dx = dz w^T and dw[e] = x_e^T dz_e; dbias[e] = sum dz_e is taken of it unrounded.  dw has w's layout; an expert without
     rows gets zeros.  dbias is None without a bias, dx and dw where they are not asked for.  The residual's gradient
     is dy itself.
     """
@@ -176,10 +176,13 @@ def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offse
     dev, dt = x.device, x.dtype
     _rows_operand(dy, "dy", p.rows, p.n // 2 if gated else p.n, dt, dev)
     E, k, n = w.shape
-    dz = dy
+    dz, low = dy, None
     if p.rows and (gated or activation is not None):
         dz = torch.empty((p.rows, -(-n // 8) * 8), dtype=dt, device=dev)[:, :n]
         p.y, p.ldy = dz.data_ptr(), dz.stride(0)
+        if bias is not None:
+            low = torch.empty((p.rows, p.ldy), dtype=dt, device=dev)     # laid out as dz: the sums of db take dz as it was before its rounding
+            p.y_low = low.data_ptr()
         _native.expert_linear_grad_z(p, dy, dev)
     elif gated:
         dz = dy.new_empty((0, n))
@@ -200,7 +203,7 @@ def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offse
         _native.expert_weight_grad(p, dz, dw, dev)
     if bias is not None:
         db = torch.empty((E, n), dtype=dt, device=dev)
-        _native.expert_bias_grad(dz, offsets, db, p.dtype)
+        _native.expert_bias_grad(dz, low, offsets, db, p.dtype)
     return dx, dw, db
 
 

@@ -80,6 +80,7 @@ def grad64(dy, x, w, bias, act, gated):
     X, W, D = x.double(), w.double(), dy.double()
     if not gated and act is None:
         dz, e = D, torch.zeros_like(D)
+        e_sum = e
     else:
         z = X @ W + (0 if bias is None else bias.double())
         ez = (X.abs() @ W.abs()) * sum_slack(k) + z.abs() * 2.0 ** -23
@@ -100,6 +101,7 @@ def grad64(dy, x, w, bias, act, gated):
                 e[:, : n // 2] += near * full
             else:
                 e += near * full
+        e_sum = e + (dz.abs() + e) * HALF_STEP[dt] ** 2 + TINY[dt]     # db: of dz in two terms
         e = e + (dz.abs() + e) * HALF_STEP[dt] + TINY[dt]
 
     def rounded(v, b):
@@ -108,7 +110,7 @@ def grad64(dy, x, w, bias, act, gated):
     rows = x.shape[0]
     dx = rounded(dz @ W.T, e @ W.abs().T + (dz.abs() @ W.abs().T) * sum_slack(n))
     dw = rounded(X.T @ dz, X.abs().T @ e + (X.abs().T @ dz.abs()) * sum_slack(rows))
-    db = rounded(dz.sum(0), e.sum(0) + dz.abs().sum(0) * (rows + 8) * 2.0 ** -24)
+    db = rounded(dz.sum(0), e_sum.sum(0) + dz.abs().sum(0) * (rows + 8) * 2.0 ** -24)
     return dx, dw, db
 
 

@@ -102,7 +102,7 @@ def test_c_entries_refuse_null():
     assert L.kq_expert_linear_grad_z(None, None, 0, None, 0, None) == -1
     assert L.kq_expert_weight_grad(None, None, 0, None, None, 0, None) == -1
     assert L.kq_expert_weight_grad(ctypes.byref(_product()), None, 0, 64, None, 0, None) == -1
-    assert L.kq_expert_bias_grad(None, 0, None, 4, 8, 1, 0, None, 0, None) == -1
+    assert L.kq_expert_bias_grad(None, None, 0, None, 4, 8, 1, 0, None, 0, None) == -1
     assert L.kq_wait_errors(None, None) == -1
     assert L.kq_expert_linear_workspace_bytes(None) == 0
     # Nothing to do: no pointer is needed.
