@@ -535,6 +535,7 @@ bias_grad_kernel(const T* __restrict__ dz, const T* __restrict__ low, int64_t ld
     group_of(offsets, e, rows, lo, count);
     float s = 0.f;
     if (j < n)
+#pragma unroll 8
         for (int r = w; r < count; r += 8) {
             const int64_t at = (int64_t)(lo + r) * ld + j;
             s += to_f<T>(dz[at]) + (low ? to_f<T>(low[at]) : 0.f);
