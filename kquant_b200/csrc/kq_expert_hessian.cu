@@ -96,7 +96,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     constexpr int BK = stage_rows(NA, NB), PER_SLOT = SLOT / BK, CHUNK = chunk_bytes(NA, NB);
     constexpr int A_BYTES = BM / 64 * CHUNK, B_BYTES = BN / 64 * CHUNK;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], seg_full[2], seg_empty[2];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], seg_full[WHOLE ? 4 : 2], seg_empty[2];
     __shared__ uint32_t tmem_slot;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* out_smem = smem + STAGES * STAGE;
@@ -114,6 +114,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&seg_full[b], 1);
+            if (WHOLE) mbar_init(&seg_full[2 + b], 1);
             mbar_init(&seg_empty[b], 8);
         }
         mbar_init_fence();
@@ -152,10 +153,12 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
         }
     } else if (warp == DRAINS + 1) {
         if (lane == 0) {
-            uint32_t it = 0, seg = 0;
+            uint32_t it = 0, seg = 0, turn = 0;
             bool ok = true;
             for (int64_t i = blockIdx.x; i < all && ok; i += gridDim.x) {
                 const int e = (int)(i / p.tiles), ks_end = cum[e + 1] * PER_SLOT;
+                const int owner = WHOLE ? turn & 1 : 0;      // the group of drain warps that takes this tile
+                turn += ks_end > cum[e] * PER_SLOT;
                 for (int ks0 = cum[e] * PER_SLOT; ks0 < ks_end && ok; ks0 += SEG, ++seg) {
                     const int b = seg & 1;
                     if (!(ok = mbar_wait(&seg_empty[b], ((seg >> 1) & 1) ^ 1))) break;
@@ -179,7 +182,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                         }
                         mma_commit(&empty_bar[s]);
                     }
-                    if (ok) mma_commit(&seg_full[b]);
+                    if (ok) mma_commit(&seg_full[2 * owner + b]);
                 }
             }
             if (!ok) report_wait_error(p.err);
@@ -187,10 +190,11 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     } else if constexpr (WHOLE) {
         // Two groups of eight warps take tiles in turn (four quarters of the rows, two halves of the columns): one stores
         // while the other fills its buffers.  A tile's further segments (an expert of more rows) are added to what its
-        // first one wrote, by the same thread.
+        // first one wrote, by the same thread.  Each group has barriers of its own: it sees none of the other's segments, and
+        // a barrier that went through a phase unseen would be taken for the one before it.
         const int q = warp & 3, h = (warp >> 2) & 1, group = warp >> 3;
         uint8_t* stage = out_smem + warp * PIECE_BYTES;          // two 32 x 32 pieces under way
-        uint32_t seg = 0, piece_no = 0;
+        uint32_t seg = 0, turn = 0, piece_no = 0, seen = 0;                // seen: the phase of this group's two barriers
         bool ok = true;
         for (int64_t it = blockIdx.x; it < all && ok; it += gridDim.x) {
             const int e = (int)(it / p.tiles), ks_begin = cum[e] * PER_SLOT, ks_end = cum[e + 1] * PER_SLOT;
@@ -236,11 +240,12 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                 for (int c = 0; c < BN / 2; c += 32) put(zero, c, false);
                 continue;
             }
-            const int owner = seg & 1;
+            const int owner = turn++ & 1;
             for (int ks0 = ks_begin; ks0 < ks_end; ks0 += SEG, ++seg) {
                 if (owner != group) continue;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[seg & 1], (seg >> 1) & 1));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&seg_full[2 * group + (seg & 1)], (seen >> (seg & 1)) & 1));
                 if (!ok) break;
+                seen ^= 1u << (seg & 1);
                 tc_fence_after();
                 if (ks0 > ks_begin && lane == 0) bulk_wait_all();      // what this adds to is there
                 __syncwarp();

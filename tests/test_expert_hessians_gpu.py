@@ -132,3 +132,28 @@ def test_nothing_to_add(cuda_device):
     assert H.shape == (2, 40, 40) and not H.any() and not den.any()
     start = torch.ones((2, 40, 40), device=cuda_device)
     assert (accumulate_expert_hessians(x, off, out=start)[0] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[300, 5, 0, 140, 1, 130, 20, 129, 2, 257, 40, 0, 400, 64, 128, 3, 90, 131, 60, 33],
+                                    [129] * 3 + [1] * 17, [200] * 11 + [2] * 9, [1, 500, 1, 260, 1, 130] + [7] * 14])
+def test_uneven_experts(cuda_device, dtype, counts):
+    """Experts of one to several segments of rows in turn, every CTA with several tiles of each."""
+    E, d, tokens, rows = len(counts), 901, 333, sum(counts)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x = torch.randn((tokens, d), generator=g, device=cuda_device).to(dtype)
+    index = torch.randint(tokens, (rows,), generator=g, device=cuda_device)
+    off = offsets_of(counts, cuda_device)
+    first = None
+    for _ in range(10):
+        H, den = accumulate_expert_hessians(x, off, index=index)
+        first = H if first is None else first
+        assert torch.equal(H, first)
+    assert den.tolist() == counts
+    added, _ = accumulate_expert_hessians(x, off, index=index, out=H.clone())
+    for e, r in enumerate(groups(off)):
+        X = x[index[r]].double()
+        want, mass = X.T @ X, X.abs().T @ X.abs()
+        assert ((H[e].double() - want).abs() <= mass * slack(counts[e]) + 1e-38).all(), e
+        assert ((added[e].double() - 2 * want).abs() <= 2 * mass * slack(2 * counts[e]) + 1e-38).all(), e
+    _native.check_wait_errors(cuda_device)
