@@ -181,19 +181,21 @@ __device__ __forceinline__ void drain_lines(uint32_t tmem, T* line, bool live, i
         T* h = reinterpret_cast<T*>(o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) h[j] = from_f<T>(zero ? 0.f : __uint_as_float(v[j]));
-        if (!live) continue;
-        if (c + 16 <= n && wide) {
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(line + c), "r"(o[0]), "r"(o[1]), "r"(o[2]),
-                         "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
-                         : "memory");
-        } else if (c + 16 <= n) {
-            reinterpret_cast<uint4*>(line + c)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            reinterpret_cast<uint4*>(line + c)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        } else {
+        if (live) {
+            if (c + 16 <= n && wide) {
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(line + c), "r"(o[0]), "r"(o[1]),
+                             "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                             : "memory");
+            } else if (c + 16 <= n) {
+                reinterpret_cast<uint4*>(line + c)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                reinterpret_cast<uint4*>(line + c)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (c + j < n) line[c + j] = h[j];
+                for (int j = 0; j < 16; ++j)
+                    if (c + j < n) line[c + j] = h[j];
+            }
         }
+        __syncwarp();                            // the next tensor-memory load is the whole warp's
     }
 }
 
@@ -417,6 +419,7 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 T ahead[TR];
                 if (aux && begin < n) fetch_rows(ahead, aux + (int64_t)begin * p.ld_aux, p.ld_aux, n - begin);
                 uint32_t v[TR], w[TR];
+                __syncwarp();                           // tensor-memory loads are the whole warp's
                 if (begin < n) {
                     tmem_ld8(base + begin, v);
                     if constexpr (GATED) tmem_ld8(col[1] + begin, w);
@@ -458,6 +461,7 @@ expert_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         store_rows(low, p.ld_out, live ? n - c : 0, z);
                         if constexpr (GATED) store_rows(low + p.m_out, p.ld_out, live ? n - c : 0, u);
                     }
+                    __syncwarp();
                     tmem_wait_ld();
                 }
             }

@@ -114,6 +114,7 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         mbar_init(&done_bar, 1);
         mbar_init_fence();
     }
+    __syncwarp();                                         // lane 0 was apart; what is .aligned needs its whole warp
     if (warp == 0) tmem_alloc(&tmem_slot, p.tmem_cols);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
@@ -256,6 +257,7 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 }
             }
         }
+        __syncwarp();                                     // lanes without a row or feature left the loop early
         if (p.splits > 1) cluster_sync();                 // the others are done with this CTA's part
         else __syncthreads();
     }

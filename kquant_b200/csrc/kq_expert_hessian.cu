@@ -219,6 +219,7 @@ hessian_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
                         }
                         bulk_commit();
                     }
+                    __syncwarp();                                  // the next tensor-memory load is the whole warp's
                 } else {
                     __syncwarp();
                     const int j = j0 + c + lane;

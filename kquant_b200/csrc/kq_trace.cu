@@ -75,6 +75,7 @@ abt_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
         mbar_init(&done_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
                      "r"(kTmemCols));
