@@ -154,7 +154,7 @@ rotated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                             float a[8];
                             load8(svh + c, p.vec_svh, 8, a);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) a[e] *= z[c + e] * scale;
+                            for (int e = 0; e < 8; ++e) a[e] = z[c + e] * a[e] * scale;      // scale last: z * scale may be beyond fp32
                             store8(orow + c, p.vec_out, 8, a);
                         }
                     }

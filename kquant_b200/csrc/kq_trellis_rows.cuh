@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(R_THREADS, 1) rows_trellis_kernel(const __grid
                             float a[8];
                             load8(svh + o * 32 + c, p.vec_svh, 8, a);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) a[e] *= z[c + e] * scale;
+                            for (int e = 0; e < 8; ++e) a[e] = z[c + e] * a[e] * scale;      // scale last: z * scale may be beyond fp32
                             if (p.bf16) store8(static_cast<__nv_bfloat16*>(p.y) + at + o * 32 + c, p.vec_y, 8, a);
                             else store8(static_cast<__half*>(p.y) + at + o * 32 + c, p.vec_y, 8, a);
                         }
