@@ -269,7 +269,8 @@ few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
 template <typename T, bool GATED>
 int launch(const CUtensorMap& w, const CUtensorMap& x, const Params& p, int smem, dim3 grid, cudaStream_t s) {
     auto kernel = few_kernel<T, GATED>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // The attribute is the kernel's, for every thread of the process: always the most that a call can need.
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_ONE + 1024);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     cudaLaunchConfig_t c{};
     c.gridDim = grid;

@@ -1,4 +1,5 @@
 """Calls of the expert-layer operators as programs make them: from several threads, with results in given memory, repeated."""
+import ctypes
 import threading
 
 import pytest
@@ -14,7 +15,7 @@ def test_threads_with_calls_of_different_sizes(cuda_device):
     """Threads whose calls differ in the shared memory that they ask for do not disturb one another."""
     g = torch.Generator(device=cuda_device).manual_seed(31)
     w = (torch.randn((8, 64, 256), generator=g, device=cuda_device) / 8).bfloat16()
-    calls = []
+    L, calls = _native.load(), []
     for each in (1, 16):                                   # rows an expert
         x = torch.randn((8 * each, 64), generator=g, device=cuda_device).bfloat16()
         off = offsets_of([each] * 8, cuda_device)
@@ -24,16 +25,17 @@ def test_threads_with_calls_of_different_sizes(cuda_device):
 
     def work(i):
         x, off, want = calls[i % 2]
-        out = torch.empty_like(want)
-        try:
-            with torch.cuda.stream(torch.cuda.Stream(cuda_device)):
-                for _ in range(2000):
-                    experts.expert_linear(x, w, off, activation="silu", gated=True, out=out)
-                torch.cuda.current_stream().synchronize()
-                if not torch.equal(out, want):
-                    wrong.append("values")
-        except Exception as error:                         # noqa: BLE001
-            wrong.append(error)
+        out, stream = torch.empty_like(want), torch.cuda.Stream(cuda_device)
+        stream.wait_stream(torch.cuda.current_stream(cuda_device))
+        p = experts._product(x, w, off, None, "silu", True)
+        p.y, p.ldy = out.data_ptr(), out.stride(0)
+        for _ in range(5000):                              # the C entry itself: ctypes lets the other threads run meanwhile
+            if L.kq_expert_linear(ctypes.byref(p), None, 0, stream.cuda_stream):
+                wrong.append(L.kq_last_error())
+                break
+        stream.synchronize()
+        if not torch.equal(out, want):
+            wrong.append("values")
 
     threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
     for t in threads:
