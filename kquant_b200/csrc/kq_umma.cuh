@@ -8,7 +8,9 @@
 
 namespace kq {
 
-constexpr uint32_t kSpinLimit = 1u << 22;
+// Polls of a barrier before a wait gives up.  A poll returns at once or sleeps for a while, so this is some tenths of a second
+// at least: far above any wait of a kernel that makes progress, also on a GPU that is shared.
+constexpr uint32_t kSpinLimit = 1u << 24;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
