@@ -33,6 +33,7 @@ extern "C" {
 #define KQ_ERR_WORKSPACE (-2)  /* workspace too small */
 #define KQ_ERR_CUDA (-3)       /* CUDA runtime error (launch, attribute, device) */
 #define KQ_ERR_ALIGN (-4)      /* pointer not aligned as the kernel requires */
+#define KQ_ERR_TIMEOUT (-5)    /* an earlier kernel's internal wait ran out (kq_wait_errors) */
 
 /* Codebook kinds, numbered like the reference's `cb` template argument
  * (kquant/csrc/qsrt_quantize_tiles_kernel.cuh:21, exl3_compat/quant/codebook.cuh). */
@@ -381,10 +382,19 @@ size_t kq_trellis_linear_workspace_bytes(const kq_trellis_product* p);
 int kq_trellis_linear(const kq_trellis_product* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Writes 1 to *out (device int32) if an internal wait of an expert-layer
- * kernel ran out on this device since the last call, else 0, and clears it.
+ * The internal waits of the expert-layer kernels are bounded.  When one runs
+ * out the kernel ends with undefined results, and the expert-layer entry
+ * points refuse every call on that device with KQ_ERR_TIMEOUT until
+ * kq_wait_errors has been called.
+ *
+ * kq_wait_errors writes 1 to *out (device int32) if a wait ran out on this
+ * device since the last call, else 0, and clears it, in stream order.
+ * kq_wait_error_flag gives the address of the current device's flag in host
+ * memory, for programs that look at it themselves (replayed graphs make no
+ * calls): non-zero once a wait has run out.  The address stays valid.
  */
 int kq_wait_errors(int32_t* out, void* stream);
+int kq_wait_error_flag(int32_t** flag);
 
 /*
  * Roofline probe (no reference counterpart): launches blocks x threads

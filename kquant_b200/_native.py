@@ -49,6 +49,7 @@ EXPORTED = (
     "kq_expert_weight_grad",
     "kq_expert_bias_grad",
     "kq_wait_errors",
+    "kq_wait_error_flag",
     "kq_expert_hessian_workspace_bytes",
     "kq_accumulate_expert_hessians",
     "kq_trellis_linear_workspace_bytes",
@@ -143,6 +144,7 @@ def load() -> ctypes.CDLL:
         L.kq_expert_weight_grad.argtypes = [EP, P, I64, P, P, SZ, P]
         L.kq_expert_bias_grad.argtypes = [P, P, I64, P, I64, I64, I64, I, P, I64, P]
         L.kq_wait_errors.argtypes = [P, P]
+        L.kq_wait_error_flag.argtypes = [P]
         TP = ctypes.POINTER(TrellisProduct)
         L.kq_trellis_linear_workspace_bytes.argtypes = [TP]
         L.kq_trellis_linear_workspace_bytes.restype = SZ
@@ -583,9 +585,13 @@ def trellis_linear(p: TrellisProduct, device: torch.device) -> None:
 
 
 def check_wait_errors(device: torch.device) -> None:
-    """Raise if a bounded wait inside an expert-layer kernel ran out since the last call (one device sync)."""
-    out = torch.empty((), dtype=torch.int32, device=device)
+    """Raise if a bounded wait inside an expert-layer kernel ran out since the last call (waits for the device).
+
+    After such a wait every call of the expert-layer operators on that device raises, until this one has.
+    """
     with torch.cuda.device(device):
-        _check(load().kq_wait_errors(out.data_ptr(), _stream(device)), "kq_wait_errors")
-    if int(out.item()):
-        raise KQError("an internal wait of an expert-layer kernel timed out; results since the last check are invalid")
+        torch.cuda.synchronize()
+        out = torch.empty((), dtype=torch.int32, device=device)
+        _check(load().kq_wait_errors(out.data_ptr(), _stream(out.device)), "kq_wait_errors")
+        if int(out.item()):
+            raise KQError("an internal wait of an expert-layer kernel timed out; results since the last check are invalid")

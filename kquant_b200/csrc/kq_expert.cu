@@ -38,12 +38,12 @@
 // computes them and does not store them (a row meets only its own
 // accumulators); a sums tile zeroes the rows behind its expert's last in
 // shared memory before the product, because there they would be added in.
+#include <atomic>
+#include <cstring>
 #include "kq_expert_rows.cuh"
 
 namespace kq {
 namespace {
-
-__device__ int g_wait_error = 0;
 
 constexpr int BK = 64, MAX_STAGES = 6;
 constexpr int TILE = 256;                       // features of an accumulator pair, rows of a tile at most
@@ -701,7 +701,7 @@ int many_rows_product(const RowsProduct& p, cudaStream_t s) {
     if (int rc = map_rows_2d(&mb, p.x, p.bf16, BK, 32, p.what)) return rc;
     if (int rc = map_rows_2d(&mf, p.x, p.bf16, BK, 128, p.what)) return rc;
     Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
+    q.err = p.err;
     q.offsets = p.offsets;
     q.bias = p.bias;
     q.aux = p.aux;
@@ -741,6 +741,8 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     if (need && (workspace_bytes < need || !workspace)) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
     if ((uintptr_t)workspace & 15) { set_error("%s: workspace must be 16-byte aligned", what); return KQ_ERR_ALIGN; }
     uint16_t* ws = static_cast<uint16_t*>(workspace);
+    RowsProduct r{};
+    if (int rc = wait_error_word(&r.err, what)) return rc;
     const bool bf16 = p.dtype == KQ_BF16, mn = n_contiguous(p);
     Operand x = operand(p.x, 1, p.rows, p.k, 0, p.ldx), w = w_operand(p, mn);
     const bool gated_copy = mn && p.gated && !w.direct;
@@ -748,7 +750,6 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     relayout(x, ws, 1, jobs);
     relayout(w, ws, gated_copy ? 2 : 1, jobs);
     if (int rc = run_copies(jobs, s)) return rc;
-    RowsProduct r{};
     r.x = x;
     r.w = w;
     r.offsets = p.offsets;
@@ -774,15 +775,43 @@ int rows_product(const kq_expert_product& p, const void* dy, int64_t ld_dy, void
     return few_rows(r) ? few_rows_product(r, s) : many_rows_product(r, s);
 }
 
-__global__ void take_errors_kernel(int* out) { *out = atomicExch(&g_wait_error, 0); }
+__global__ void take_errors_kernel(volatile int* word, int* out) {
+    *out = *word;
+    *word = 0;
+}
 
 }  // namespace
 
-int wait_error_word(int** out) {
-    void* p = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&p, g_wait_error);
-    if (e != cudaSuccess) { set_error("cudaGetSymbolAddress: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
-    *out = static_cast<int*>(p);
+int wait_error_flag(int** out) {
+    constexpr int kDevices = 64, kApart = 32;           // a 128-byte line a device
+    static std::atomic<int*> words{nullptr};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) { set_error("cudaGetDevice: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+    if (dev >= kDevices) { set_error("device %d: at most %d devices", dev, kDevices); return KQ_ERR_ARG; }
+    int* w = words.load(std::memory_order_acquire);
+    if (!w) {
+        // Once in a process; the first call may be a captured one, into which this allocation does not go.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* fresh = nullptr;
+        e = cudaHostAlloc(&fresh, kDevices * kApart * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) { set_error("cudaHostAlloc: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
+        memset(fresh, 0, kDevices * kApart * sizeof(int));
+        if (words.compare_exchange_strong(w, static_cast<int*>(fresh), std::memory_order_acq_rel)) w = static_cast<int*>(fresh);
+        else cudaFreeHost(fresh);                       // another thread was first, w is its memory
+    }
+    *out = w + dev * kApart;
+    return KQ_OK;
+}
+
+int wait_error_word(int** out, const char* what) {
+    if (int rc = wait_error_flag(out)) return rc;
+    if (*static_cast<volatile int*>(*out)) {
+        set_error("%s: an internal wait of an earlier expert-layer kernel ran out; results since the last kq_wait_errors are invalid", what);
+        return KQ_ERR_TIMEOUT;
+    }
     return KQ_OK;
 }
 
@@ -857,6 +886,8 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     }
     if ((uintptr_t)workspace & 15) { set_error("%s: workspace must be 16-byte aligned", what); return KQ_ERR_ALIGN; }
     uint16_t* ws = static_cast<uint16_t*>(workspace);
+    Params q{};
+    if (int rc = wait_error_word(&q.err, what)) return rc;
     // A lane takes a line of dW (and stores 32 bytes at a time) where lines start on 16 bytes, else a column (2 bytes, 64 a warp):
     // dW of 7168 x 4096, 8 experts, 4096 uneven rows: 313 us against 362.
     SumsSides o = sums_sides(p, dz, ld_dz);
@@ -871,8 +902,6 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     CUtensorMap ma, mb;
     if (int rc = map_rows_2d(&ma, o.a, bf16, 64, BK, what)) return rc;
     if (int rc = map_rows_2d(&mb, o.b, bf16, 64, BK, what)) return rc;
-    Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
     q.offsets = p.offsets;
     q.out = dw;
     q.ld_out = ld;
@@ -905,6 +934,8 @@ extern "C" int kq_expert_bias_grad(const void* dz, const void* dz_low, int64_t l
         set_error("%s: bad arguments (rows=%lld n=%lld experts=%lld)", what, (long long)rows, (long long)n, (long long)experts);
         return KQ_ERR_ARG;
     }
+    int* flag;                                  // this kernel has no waits, but dz may come from one that had
+    if (int rc = wait_error_word(&flag, what)) return rc;
     const dim3 grid((unsigned)((n + 31) / 32), (unsigned)experts);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == KQ_BF16)
@@ -918,6 +949,13 @@ extern "C" int kq_expert_bias_grad(const void* dz, const void* dz_low, int64_t l
 
 extern "C" int kq_wait_errors(int32_t* out, void* stream) {
     if (!out) { kq::set_error("kq_wait_errors: null pointer"); return KQ_ERR_ARG; }
-    kq::take_errors_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(out);
+    int* word;
+    if (int rc = kq::wait_error_flag(&word)) return rc;
+    kq::take_errors_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(word, out);
     return kq::check_launch("kq_wait_errors");
+}
+
+extern "C" int kq_wait_error_flag(int32_t** flag) {
+    if (!flag) { kq::set_error("kq_wait_error_flag: null pointer"); return KQ_ERR_ARG; }
+    return kq::wait_error_flag(flag);
 }

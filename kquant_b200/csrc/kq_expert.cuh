@@ -8,9 +8,15 @@ namespace kq {
 
 constexpr int kMaxExperts = 1024;
 
-// Device word that a kernel sets when a bounded wait ran out (kq_wait_errors reads and clears it).
-int wait_error_word(int** out);
-__device__ __forceinline__ void report_wait_error(int* word) { atomicExch(word, 1); }
+// Word of the current device that a kernel sets when a bounded wait ran out.  It lies in host memory that the kernels can
+// write, so that the next call sees it without waiting for the GPU: wait_error_flag gives it, wait_error_word does unless it is
+// set (KQ_ERR_TIMEOUT; kq_wait_errors clears it).
+int wait_error_flag(int** out);
+int wait_error_word(int** out, const char* what);
+__device__ __forceinline__ void report_wait_error(int* word) {
+    *reinterpret_cast<volatile int*>(word) = 1;
+    __threadfence_system();
+}
 
 // Rows offsets[e] .. offsets[e+1] belong to expert e.  The offsets live on the
 // device, so every value is clamped into 0 .. rows before it is used as an

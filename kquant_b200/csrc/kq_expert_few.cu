@@ -302,7 +302,7 @@ bool few_rows(const RowsProduct& p) {
 int few_rows_product(const RowsProduct& p, cudaStream_t s) {
     const int64_t busy = p.experts < p.rows ? p.experts : p.rows, mean = (p.rows + busy - 1) / busy;
     Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
+    q.err = p.err;
     q.nt = mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 32 ? 64 : 128;     // twice the mean: uneven experts mostly fit one tile
     q.offsets = p.offsets;
     q.bias = p.bias;

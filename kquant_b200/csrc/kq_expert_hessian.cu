@@ -562,7 +562,7 @@ extern "C" int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int6
     if (need && (workspace_bytes < need || !workspace)) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
     Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
+    if (int rc = wait_error_word(&q.err, what)) return rc;
     const int ld = (int)pad_width(dim);
     const int64_t n_slots = slots(rows, experts);
     int na, nb;

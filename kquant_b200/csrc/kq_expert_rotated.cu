@@ -196,7 +196,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid
 
 int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
                          int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
-                         bool bf16_out, bool zero_rest, cudaStream_t s) {
+                         bool bf16_out, bool zero_rest, int* err, cudaStream_t s) {
     const char* what = "rows_product_rotated";
     CUtensorMap ma, mb;
     const int64_t xd[2] = {k, rows}, xs[1] = {k * 2}, wd[3] = {k, n, experts}, wst[2] = {k * 2, n * k * 2};
@@ -204,7 +204,7 @@ int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* of
     if (int rc = encode_tiles(&ma, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, xd, xs, xb, what)) return rc;
     if (int rc = encode_tiles(&mb, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, w, wd, wst, wb, what)) return rc;
     Params q{};
-    if (int rc = wait_error_word(&q.err)) return rc;
+    q.err = err;
     q.offsets = offsets;
     q.svh = reinterpret_cast<const __half*>(svh);
     q.svh_stride = svh_stride;

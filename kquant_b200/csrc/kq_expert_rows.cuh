@@ -49,6 +49,7 @@ struct RowsProduct {
     int up;                    // gated: first coordinate of the up half in W
     int act;
     bool bf16, mn, gated, grad, zero_rest;
+    int* err;                  // wait_error_word
     const char* what;
 };
 
@@ -61,6 +62,6 @@ int few_rows_product(const RowsProduct& p, cudaStream_t s);
 // fp16 with row stride ldy; rows of no expert are zeroed with zero_rest.
 int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
                          int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
-                         bool bf16_out, bool zero_rest, cudaStream_t s);
+                         bool bf16_out, bool zero_rest, int* err, cudaStream_t s);
 
 }  // namespace kq

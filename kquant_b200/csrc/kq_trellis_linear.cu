@@ -404,9 +404,11 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
         set_error("%s: trellis and table need 16-byte alignment", what);
         return KQ_ERR_ALIGN;
     }
+    int* err;
     const Plan l = plan(p);
     if (!workspace || workspace_bytes < (size_t)l.bytes) { set_error("%s: workspace too small", what); return KQ_ERR_WORKSPACE; }
     if ((uintptr_t)workspace & 127) { set_error("%s: workspace must be 128-byte aligned", what); return KQ_ERR_ALIGN; }
+    if (int rc = wait_error_word(&err, what)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     __half* xr = reinterpret_cast<__half*>(ws);
@@ -435,9 +437,8 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
     if (l.way == FUSED) {
         TrellisRows r{reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, reinterpret_cast<const uint16_t*>(xr),
                       reinterpret_cast<const __half*>(p.svh), scale, p.y, p.svh_stride_e, p.ldy, (int)p.rows, (int)p.experts, (int)p.k,
-                      (int)p.n, nullptr, bf16, ((uintptr_t)p.svh & 15) == 0 && p.svh_stride_e % 8 == 0,
+                      (int)p.n, err, bf16, ((uintptr_t)p.svh & 15) == 0 && p.svh_stride_e % 8 == 0,
                       ((uintptr_t)p.y & 15) == 0 && p.ldy % 8 == 0, p.zero_rest != 0};
-        if (int rc = wait_error_word(&r.err)) return rc;
         const int dec = p.codebook == KQ_CB_MCG ? DEC_MCG : DEC_E4M3;
         return p.bits <= 2 ? rows_trellis_k12(r, p.bits, dec, s) : p.bits <= 4 ? rows_trellis_k34(r, p.bits, dec, s)
              : p.bits <= 6 ? rows_trellis_k56(r, p.bits, dec, s) : rows_trellis_k78(r, p.bits, dec, s);
@@ -445,5 +446,5 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
     __half* w = reinterpret_cast<__half*>(ws + l.rest);
     if (int rc = decode_all(p, w, s)) return rc;
     return rows_product_rotated(reinterpret_cast<const uint16_t*>(xr), reinterpret_cast<const uint16_t*>(w), p.offsets, p.rows, p.k, p.n,
-                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, p.zero_rest != 0, s);
+                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, p.zero_rest != 0, err, s);
 }

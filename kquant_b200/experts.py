@@ -19,6 +19,9 @@ import torch
 
 from . import _native
 
+# Every wait inside the kernels is bounded.  Should one run out, later calls on that device raise until this has been called.
+check_wait_errors = _native.check_wait_errors
+
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 

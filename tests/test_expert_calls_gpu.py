@@ -5,7 +5,7 @@ import threading
 import pytest
 import torch
 
-from kquant_b200 import _native, experts
+from kquant_b200 import _native, capture, experts
 from tests.expert_cases import offsets_of
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +44,37 @@ def test_threads_with_calls_of_different_sizes(cuda_device):
         t.join()
     assert not wrong, wrong
     _native.check_wait_errors(cuda_device)
+
+
+def test_a_wait_that_ran_out_is_not_silent(cuda_device):
+    """A kernel reports it in a flag that the next call sees; here the flag is set by hand."""
+    bf16 = lambda *s: torch.ones(s, device=cuda_device).bfloat16()  # noqa: E731
+    half = lambda *s: torch.ones(s, device=cuda_device).half()  # noqa: E731
+    off = offsets_of([1, 2], cuda_device)
+    t = torch.zeros((2, 8, 8, 48), dtype=torch.int16, device=cuda_device)
+    calls = [lambda: experts.expert_linear(bf16(3, 128), bf16(2, 128, 64), off),
+             lambda: experts.linear(bf16(3, 128), bf16(128, 64)),
+             lambda: experts.expert_linear_grad(bf16(3, 64), bf16(3, 128), bf16(2, 128, 64), off),
+             lambda: experts.expert_linear_grad(bf16(3, 64), bf16(3, 128), bf16(2, 128, 64), off, bias=bf16(2, 64), need_dx=False,
+                                                need_dw=False),
+             lambda: experts.trellis_linear(bf16(3, 128), t, half(2, 128), half(2, 128), off),
+             lambda: experts.trellis_linear(bf16(900, 128), t, half(2, 128), half(2, 128), offsets_of([400, 500], cuda_device)),
+             lambda: capture.accumulate_expert_hessians(bf16(3, 128), off)]
+    want = [c() for c in calls]
+    experts.check_wait_errors(cuda_device)
+    torch.cuda.synchronize()
+    flag = ctypes.POINTER(ctypes.c_int32)()
+    with torch.cuda.device(cuda_device):
+        assert _native.load().kq_wait_error_flag(ctypes.byref(flag)) == 0
+    assert flag[0] == 0
+    flag[0] = 1
+    for c in calls:
+        with pytest.raises(_native.KQError, match="ran out"):
+            c()
+    with pytest.raises(_native.KQError, match="timed out"):
+        experts.check_wait_errors(cuda_device)
+    assert flag[0] == 0
+    experts.check_wait_errors(cuda_device)
+    for c, w in zip(calls, want):
+        for a, b in zip(*((r if isinstance(r, tuple) else (r,)) for r in (c(), w))):
+            assert a is b or torch.equal(a, b)
