@@ -57,7 +57,7 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
     is row t.  ``weights`` fp32, one per slot.  Returns (H [experts, d, d] fp32, denominators [experts] fp64, the
     sums of the weights), both on the GPU: nothing waits for the device.  A fresh H whose d is not a multiple of 32 is a
     view with rows padded to one.  With ``out`` the sums are added to it,
-    which is how samples stream in; the denominators are this call's alone.  fp32 accuracy for every type.
+    which is how samples stream in (it overlaps no operand); the denominators are this call's alone.  fp32 accuracy for every type.
     """
     if not isinstance(rows, torch.Tensor) or rows.dtype not in _ROW_DTYPES:
         raise TypeError("rows must be a torch.bfloat16, torch.float16 or torch.float32 tensor")
@@ -84,6 +84,8 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
         experts._operand(out, "out", 3, torch.float32, dev)
         if out.shape != (E, d, d) or (d > 1 and out.stride(2) != 1):
             raise ValueError(f"out must be [{E}, {d}, {d}] with unit stride along its last dimension")
+        for name, t in (("rows", rows), ("offsets", offsets), ("index", index), ("weights", weights)):
+            experts._refuse_overlap(out, t, name)
     if tokens > 1 and rows.stride(0) < d:
         rows = rows.contiguous()
     # Rows of a fresh H start on 128-byte lines: with d floats a row, an odd d splits every line that is written.

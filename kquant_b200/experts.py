@@ -66,12 +66,12 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 def _refuse_overlap(out: torch.Tensor, t: torch.Tensor | None, name: str) -> None:
     """The kernels read operands while others write results; columns of one buffer beside each other are apart."""
-    if t is None or not t.numel() or not out.numel() or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
+    if t is None or not t.numel() or not out.numel():
         return
     (a, a_end), (b, b_end) = _span(out), _span(t)
     if a_end <= b or b_end <= a:
         return
-    if t.ndim == 2 and t.stride(0) == out.stride(0) > 0 and name != "bias":
+    if t.ndim == out.ndim == 2 and t.element_size() == out.element_size() and t.stride(0) == out.stride(0) > 0 and name != "bias":
         ld, by = out.stride(0), (b - a) // out.element_size() % out.stride(0)      # where t's rows begin among out's
         if by >= out.shape[1] and by + t.shape[1] <= ld:
             return
@@ -125,7 +125,7 @@ def _product(x, w, offsets, bias, activation, gated, dense=False) -> _native.Exp
     return p
 
 
-def _linear(p: _native.ExpertProduct, x, w, bias, residual, out) -> torch.Tensor:
+def _linear(p: _native.ExpertProduct, x, w, offsets, bias, residual, out) -> torch.Tensor:
     """The forward product behind checked operands."""
     n_out, rows, dt, dev = p.n // 2 if p.gated else p.n, p.rows, x.dtype, x.device
     if residual is not None:
@@ -139,6 +139,7 @@ def _linear(p: _native.ExpertProduct, x, w, bias, residual, out) -> torch.Tensor
         _refuse_overlap(out, x, "x")
         _refuse_overlap(out, w, "w")
         _refuse_overlap(out, bias, "bias")
+        _refuse_overlap(out, offsets, "offsets")
         if residual is not None and (residual.data_ptr(), residual.stride()) != (out.data_ptr(), out.stride()):
             _refuse_overlap(out, residual, "residual other than as the same view")
     if rows:
@@ -156,13 +157,13 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None
     columns and then the up projection's, y = act(gate) * up + residual has n / 2 columns.  ``activation``: None,
     "relu", "silu" or "gelu" (the error-function form).  ``out`` may be the residual itself, and overlaps no operand otherwise.
     """
-    return _linear(_product(x, w, offsets, bias, activation, gated), x, w, bias, residual, out)
+    return _linear(_product(x, w, offsets, bias, activation, gated), x, w, offsets, bias, residual, out)
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
            gated: bool = False, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """act(x w + bias) + residual with one matrix w [k, n] and bias [n]; see :func:`expert_linear`."""
-    return _linear(_product(x, w, None, bias, activation, gated, dense=True), x, w, bias, residual, out)
+    return _linear(_product(x, w, None, bias, activation, gated, dense=True), x, w, None, bias, residual, out)
 
 
 def expert_linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *,
@@ -219,6 +220,7 @@ def trellis_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, sv
     svh [experts, n] fp16: ``{"suh", "svh", "trellis"}`` of the encoder's results, stacked over the experts of one
     rate K.  One encoded matrix goes without the experts dimension and without offsets.  ``codebook``: None for MCG,
     the 65,536 E4M3 bytes of an SQG table, or 65,536 binary16 labels (int16 bits, ``_native.build_labels``).
+    ``out`` may lie over x, which is read before the first result is written; it overlaps no other operand.
     """
     if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES:
         raise TypeError("x must be a torch.bfloat16 or torch.float16 tensor")
@@ -254,6 +256,8 @@ def trellis_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, sv
         p.ldy, p.zero_rest = n, 1
     else:
         p.ldy = _rows_operand(out, "out", rows, n, x.dtype, dev)
+        for name, t in (("trellis", trellis), ("suh", suh), ("svh", svh), ("offsets", offsets), ("codebook", codebook)):
+            _refuse_overlap(out, t, name)
     p.x, p.trellis, p.suh, p.svh, p.offsets, p.y = (x.data_ptr(), trellis.data_ptr(), suh.data_ptr(), svh.data_ptr(),
                                                     _ptr(offsets), out.data_ptr())
     p.rows, p.k, p.n, p.experts = rows, k, n, E

@@ -27,3 +27,14 @@ def test_scales_of_rows_in_every_kernel(cuda_device, book, counts, n):
     check(y, want, bound)
     assert not y[0].any()
     _native.check_wait_errors(cuda_device)
+
+
+@pytest.mark.parametrize("counts,n", [([8, 30], 256), ([8, 100], 4224), ([300, 100], 4224)])
+def test_result_over_its_own_rows(cuda_device, counts, n):
+    """x is read before the first result is written, in every kernel."""
+    x, t, suh, svh, off = make(counts, n, n, 3, torch.bfloat16, cuda_device, seed=42, spare=2)
+    want = experts.trellis_linear(x, t, suh, svh, off)
+    rows = x.clone()
+    assert experts.trellis_linear(rows, t, suh, svh, off, out=rows) is rows
+    assert torch.equal(rows[: sum(counts)], want[: sum(counts)]) and torch.equal(rows[sum(counts):], x[sum(counts):])
+    _native.check_wait_errors(cuda_device)
