@@ -362,7 +362,9 @@ int kq_accumulate_expert_hessians(const void* x, int64_t tokens, int64_t dim, in
  * 65,536 E4M3 bytes by state) or KQ_CB_LABELS (table: 65,536 binary16 labels
  * by state, kq_build_labels).  The rotated row enters the tensor cores as
  * binary16 with a power of two of its own; sums are fp32, y is rounded once.
- * Rows of no expert as in kq_expert_linear.
+ * Rows of no expert as in kq_expert_linear.  The workspace holds the rotated
+ * rows and partial sums or decoded matrices, of the latter at most 1 GiB (or
+ * one expert's, if that is more).
  */
 #define KQ_CB_LABELS 5
 typedef struct {

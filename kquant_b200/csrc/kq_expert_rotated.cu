@@ -17,12 +17,12 @@ constexpr int GROUP_BYTES = (3 * kMaxExperts + 4) * 4;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + GROUP_BYTES + 1024;
 
 struct Params {
-    const int64_t* offsets;
+    const int64_t *offsets, *all;   // of this call's experts, and of all experts of the rows
     const __half* svh;
     const float* row_scale;
     void* out;
     int64_t svh_stride, ld_out;
-    int rows, experts, k_steps, n_tiles, n_out;
+    int rows, experts, all_experts, k_steps, n_tiles, n_out;
     int* err;
     bool vec_svh, vec_out, zero_rest;
 };
@@ -168,8 +168,8 @@ rotated_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (!ok && lane == 0) report_wait_error(p.err);
         if (p.zero_rest && p.offsets) {
             int begin, end, n;
-            group_of(p.offsets, 0, p.rows, begin, n);
-            group_of(p.offsets, p.experts - 1, p.rows, end, n);
+            group_of(p.all, 0, p.rows, begin, n);
+            group_of(p.all, p.all_experts - 1, p.rows, end, n);
             end += n;
             for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
                 if (row >= begin && row < end) continue;
@@ -195,7 +195,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid
 }  // namespace
 
 int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
-                         int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
+                         int64_t all_experts, int64_t first, int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
                          bool bf16_out, bool zero_rest, int* err, cudaStream_t s) {
     const char* what = "rows_product_rotated";
     CUtensorMap ma, mb;
@@ -205,8 +205,10 @@ int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* of
     if (int rc = encode_tiles(&mb, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, w, wd, wst, wb, what)) return rc;
     Params q{};
     q.err = err;
-    q.offsets = offsets;
-    q.svh = reinterpret_cast<const __half*>(svh);
+    q.offsets = offsets ? offsets + first : nullptr;
+    q.all = offsets;
+    q.all_experts = (int)all_experts;
+    q.svh = reinterpret_cast<const __half*>(svh) + first * svh_stride;
     q.svh_stride = svh_stride;
     q.row_scale = row_scale;
     q.out = y;
@@ -216,7 +218,7 @@ int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* of
     q.k_steps = (int)((k + BK - 1) / BK);
     q.n_tiles = (int)((n + BN - 1) / BN);
     q.n_out = (int)n;
-    q.zero_rest = zero_rest;
+    q.zero_rest = zero_rest && first == 0;
     q.vec_svh = ((uintptr_t)svh & 15) == 0 && svh_stride % 8 == 0;
     q.vec_out = ((uintptr_t)y & 15) == 0 && ldy % 8 == 0;
     int sms;

@@ -57,11 +57,11 @@ struct RowsProduct {
 bool few_rows(const RowsProduct& p);
 int few_rows_product(const RowsProduct& p, cudaStream_t s);
 
-// y[r] = had128(x[r] W_e^T) * svh[e] * row_scale[r] for the rows of experts 0 .. experts-1 behind `offsets`:
-// x [rows x k] and W [experts][n][k] binary16 (k a multiple of 8, n of 128), svh binary16 [experts][n], y bf16 or
-// fp16 with row stride ldy; rows of no expert are zeroed with zero_rest.
+// y[r] = had128(x[r] W_e^T) * svh[e] * row_scale[r] for the rows of experts first .. first + experts - 1 of all_experts
+// behind `offsets`: x [rows x k] and W [experts][n][k] binary16 (k a multiple of 8, n of 128), svh binary16
+// [all_experts][n], y bf16 or fp16 with row stride ldy; rows of no expert are zeroed with zero_rest (when first is 0).
 int rows_product_rotated(const uint16_t* x, const uint16_t* w, const int64_t* offsets, int64_t rows, int64_t k, int64_t n,
-                         int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
+                         int64_t all_experts, int64_t first, int64_t experts, const uint16_t* svh, int64_t svh_stride, const float* row_scale, void* y, int64_t ldy,
                          bool bf16_out, bool zero_rest, int* err, cudaStream_t s);
 
 }  // namespace kq

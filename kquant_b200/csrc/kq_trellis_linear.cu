@@ -296,7 +296,11 @@ Way way_of(const kq_trellis_product& p) {
 
 int64_t align128(int64_t v) { return (v + 127) & ~(int64_t)127; }
 
-struct Plan { Way way; bool wide; int parts; int64_t scale, rest, bytes; };
+// The decode-once way holds at most this much of What, some experts at a time: all of 384 experts of 7168 x 4096 would be
+// 22 GB.  (16 such experts a round; what one expert needs if that is more.)
+constexpr int64_t kDecodedBytes = (int64_t)1 << 30;
+
+struct Plan { Way way; bool wide; int parts, together; int64_t scale, rest, bytes; };    // together: experts decoded at a time
 
 int few_ctas(const kq_trellis_product& p, int sms) { return sms * (p.codebook == KQ_CB_LABELS ? 1 : 2); }   // a table of 128 KB leaves room for one
 
@@ -312,7 +316,9 @@ Plan plan(const kq_trellis_product& p) {
     l.parts = (int)(most < fit ? most : fit < 2 ? 2 : fit);
     l.scale = align128(p.rows * p.k * 2);
     l.rest = l.scale + align128(p.rows * 4);
-    l.bytes = l.rest + (l.way == FEW ? (int64_t)l.parts * one : l.way == FUSED ? 0 : p.experts * p.k * p.n * 2);
+    const int64_t expert = p.k * p.n * 2, fill = kDecodedBytes / expert;
+    l.together = (int)(fill < 1 ? 1 : fill < p.experts ? fill : p.experts);
+    l.bytes = l.rest + (l.way == FEW ? (int64_t)l.parts * one : l.way == FUSED ? 0 : l.together * expert);
     return l;
 }
 
@@ -335,37 +341,44 @@ int check_trellis(const kq_trellis_product& p, const char* what) {
 }
 
 template <int K, int DEC>
-int launch_decode(const kq_trellis_product& p, __half* out, cudaStream_t s) {
+int launch_decode(const kq_trellis_product& p, int64_t first, int64_t experts, __half* out, cudaStream_t s) {
     constexpr int smem = table_bytes(DEC) + DN * DPAD * 2;
     cudaError_t e = cudaFuncSetAttribute(decode_kernel<K, DEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return KQ_ERR_CUDA; }
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    const int64_t items = (p.n / DN) * (p.k / DK) * p.experts;
+    const int64_t items = (p.n / DN) * (p.k / DK) * experts;
     const int per_sm = DEC == DEC_F16 ? 1 : DEC == DEC_E4M3 ? 2 : 8;
     const int grid = (int)(items < (int64_t)sms * per_sm ? items : (int64_t)sms * per_sm);
-    return launch_next(decode_kernel<K, DEC>, dim3((unsigned)grid), 256, smem, s, "decode_kernel",
-                       reinterpret_cast<const uint32_t*>(p.trellis), p.table, p.offsets, (int)p.rows, (int)p.experts, (int)p.k, (int)p.n,
-                       out);
+    const uint32_t* trellis = reinterpret_cast<const uint32_t*>(p.trellis) + first * (p.k / 16) * (p.n / 16) * 8 * K;
+    const int64_t* offsets = p.offsets ? p.offsets + first : nullptr;
+    // The first range is decoded beside the rotation of x.  A later one takes the memory of the one before it, whose products
+    // have to be done: an ordinary launch.
+    if (!first)
+        return launch_next(decode_kernel<K, DEC>, dim3((unsigned)grid), 256, smem, s, "decode_kernel", trellis, p.table, offsets,
+                           (int)p.rows, (int)experts, (int)p.k, (int)p.n, out);
+    decode_kernel<K, DEC><<<grid, 256, smem, s>>>(trellis, p.table, offsets, (int)p.rows, (int)experts, (int)p.k, (int)p.n, out);
+    return check_launch("decode_kernel");
 }
 
 template <int K>
-int launch_decode_k(const kq_trellis_product& p, __half* out, cudaStream_t s) {
-    if (p.codebook == KQ_CB_MCG) return launch_decode<K, DEC_MCG>(p, out, s);
-    if (p.codebook == KQ_CB_SQG) return launch_decode<K, DEC_E4M3>(p, out, s);
-    return launch_decode<K, DEC_F16>(p, out, s);
+int launch_decode_k(const kq_trellis_product& p, int64_t first, int64_t experts, __half* out, cudaStream_t s) {
+    if (p.codebook == KQ_CB_MCG) return launch_decode<K, DEC_MCG>(p, first, experts, out, s);
+    if (p.codebook == KQ_CB_SQG) return launch_decode<K, DEC_E4M3>(p, first, experts, out, s);
+    return launch_decode<K, DEC_F16>(p, first, experts, out, s);
 }
 
-int decode_all(const kq_trellis_product& p, __half* out, cudaStream_t s) {
+// What of experts first .. first + experts - 1.
+int decode_range(const kq_trellis_product& p, int64_t first, int64_t experts, __half* out, cudaStream_t s) {
     switch (p.bits) {
-        case 1: return launch_decode_k<1>(p, out, s);
-        case 2: return launch_decode_k<2>(p, out, s);
-        case 3: return launch_decode_k<3>(p, out, s);
-        case 4: return launch_decode_k<4>(p, out, s);
-        case 5: return launch_decode_k<5>(p, out, s);
-        case 6: return launch_decode_k<6>(p, out, s);
-        case 7: return launch_decode_k<7>(p, out, s);
-        default: return launch_decode_k<8>(p, out, s);
+        case 1: return launch_decode_k<1>(p, first, experts, out, s);
+        case 2: return launch_decode_k<2>(p, first, experts, out, s);
+        case 3: return launch_decode_k<3>(p, first, experts, out, s);
+        case 4: return launch_decode_k<4>(p, first, experts, out, s);
+        case 5: return launch_decode_k<5>(p, first, experts, out, s);
+        case 6: return launch_decode_k<6>(p, first, experts, out, s);
+        case 7: return launch_decode_k<7>(p, first, experts, out, s);
+        default: return launch_decode_k<8>(p, first, experts, out, s);
     }
 }
 
@@ -444,7 +457,13 @@ extern "C" int kq_trellis_linear(const kq_trellis_product* pp, void* workspace, 
              : p.bits <= 6 ? rows_trellis_k56(r, p.bits, dec, s) : rows_trellis_k78(r, p.bits, dec, s);
     }
     __half* w = reinterpret_cast<__half*>(ws + l.rest);
-    if (int rc = decode_all(p, w, s)) return rc;
-    return rows_product_rotated(reinterpret_cast<const uint16_t*>(xr), reinterpret_cast<const uint16_t*>(w), p.offsets, p.rows, p.k, p.n,
-                                p.experts, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16, p.zero_rest != 0, err, s);
+    for (int64_t e = 0; e < p.experts; e += l.together) {
+        const int64_t some = p.experts - e < l.together ? p.experts - e : l.together;
+        if (int rc = decode_range(p, e, some, w, s)) return rc;
+        if (int rc = rows_product_rotated(reinterpret_cast<const uint16_t*>(xr), reinterpret_cast<const uint16_t*>(w), p.offsets, p.rows,
+                                          p.k, p.n, p.experts, e, some, p.svh, p.svh_stride_e, scale, p.y, p.ldy, bf16,
+                                          p.zero_rest != 0, err, s))
+            return rc;
+    }
+    return KQ_OK;
 }

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from kquant_b200 import _native, experts
-from tests.expert_cases import check
+from tests.expert_cases import check, groups, offsets_of
 from tests.test_trellis_linear_gpu import expect, make, tables
 
 pytestmark = pytest.mark.gpu
@@ -37,4 +37,35 @@ def test_result_over_its_own_rows(cuda_device, counts, n):
     rows = x.clone()
     assert experts.trellis_linear(rows, t, suh, svh, off, out=rows) is rows
     assert torch.equal(rows[: sum(counts)], want[: sum(counts)]) and torch.equal(rows[sum(counts):], x[sum(counts):])
+    _native.check_wait_errors(cuda_device)
+
+
+@pytest.mark.parametrize("book", ["mcg", "labels"])
+def test_more_experts_than_are_decoded_at_a_time(cuda_device, book):
+    """Two experts of this size fit the decoded matrices' memory: three rounds, and what each expert gives alone."""
+    g = torch.Generator(device=cuda_device).manual_seed(43)
+    counts, k, n = [300, 0, 250, 200, 260], 16384, 16384
+    rows, E = sum(counts), len(counts)
+    x = torch.randn((rows + 5, k), generator=g, device=cuda_device).bfloat16()
+    t = torch.randint(-32768, 32768, (E, k // 16, n // 16, 16), generator=g, device=cuda_device, dtype=torch.int16)
+    suh, svh = (torch.rand((E, k), generator=g, device=cuda_device) + 0.5).half(), (torch.rand((E, n), generator=g, device=cuda_device) + 0.5).half()
+    cb, off = tables(cuda_device)[book], offsets_of(counts, cuda_device, first=3)
+    run = lambda: experts.trellis_linear(x, t, suh, svh, off, codebook=cb)  # noqa: E731
+    y = run()
+    assert not y[:3].any() and not y[rows + 3:].any()
+    for e, r in enumerate(groups(off)):
+        if r.stop > r.start:
+            alone = experts.trellis_linear(x[r], t[e], suh[e], svh[e], codebook=cb)
+            assert alone.abs().max() > 0 and torch.equal(y[r], alone), e
+    keep = torch.full_like(y, 7.0)
+    experts.trellis_linear(x, t, suh, svh, off, codebook=cb, out=keep)
+    assert torch.equal(keep[3: rows + 3], y[3: rows + 3]) and (keep[:3] == 7).all() and (keep[rows + 3:] == 7).all()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for new in (counts, [0, 0, 0, 0, rows], [rows, 0, 0, 0, 0], [1, 2, 3, 4, 5]):
+        off.copy_(offsets_of(new, cuda_device))
+        graph.replay()
+        assert torch.equal(got, run())
     _native.check_wait_errors(cuda_device)
