@@ -58,6 +58,8 @@ def accumulate_expert_hessians(rows: torch.Tensor, offsets: torch.Tensor, *, ind
     sums of the weights), both on the GPU: nothing waits for the device.  A fresh H whose d is not a multiple of 32 is a
     view with rows padded to one.  With ``out`` the sums are added to it,
     which is how samples stream in (it overlaps no operand); the denominators are this call's alone.  fp32 accuracy for every type.
+    Infinity or NaN in a row that counts makes infinity or NaN of that row's share of H (NaN also where the products alone would be
+    infinite, with weights or fp32 rows).
     """
     if not isinstance(rows, torch.Tensor) or rows.dtype not in _ROW_DTYPES:
         raise TypeError("rows must be a torch.bfloat16, torch.float16 or torch.float32 tensor")

@@ -16,8 +16,9 @@
 // need, where row tiles of 128 or 256 on the M axis would waste 11% or 31% of
 // the products of an unevenly routed prompt (8192 rows, 16 experts).  A CTA
 // moves 48 KB a stage for 1024 tensor cycles; one CTA with a 128 x 256 tile
-// moved the same for 512 and stood at 0.55 of the tensor peak, a pair with 256
-// x 256 at 0.63 (bytes into and out of shared memory, and TMA issue).
+// would move the same for 512.  8192 rows without an epilogue, in a run of
+// calls under the power limit: 1030 TFLOP/s at k = 1536, 1158 at 7168 (0.81
+// and 0.90 of cuBLAS; 0.72 and 0.83 for single calls).
 //
 // Warp 0 of each CTA issues TMA into a ring of 64-deep stages; warp 1 of the
 // leader issues tcgen05.mma for the pair; warps 2..17 drain.  The accumulators
@@ -910,7 +911,8 @@ extern "C" int kq_expert_weight_grad(const kq_expert_product* pp, const void* dz
     q.experts = (int)p.experts;
     q.n_tiles = (int)((n_out + TILE - 1) / TILE);
     // Few rows are few products to drain under: one accumulator then, so that the two halves of the tensor memory alternate
-    // (8 experts of 7168 x 4096, one / two accumulators: 249 / 272 us at 512 rows each, 434 / 407 at 1024).
+    // (8 experts of 7168 x 4096, one / two accumulators, back to back: 263 / 298 us at 512 rows each, 305 / 326 at 640, 353 / 364
+    // at 768, 442 / 435 at 1024, 822 / 744 at 2048).
     q.span = TILE;
     if (p.rows > 640 * (p.experts < p.rows ? p.experts : p.rows))
         if (int rc = span_for(m_out, (int64_t)q.n_tiles * p.experts, p.rows, false, false, &q.span)) return rc;

@@ -512,7 +512,8 @@ void terms_of(int dtype, bool weighted, int& na, int& nb) {
     else { na = 2; nb = 3; }
 }
 
-// fp32 rows without weights share one set of terms for both sides.
+// One set of terms for both sides where they are the 16-bit values themselves, else one for each (fp32 rows without weights too,
+// whose two sets are alike).
 int term_count(int dtype, bool weighted) {
     int na, nb;
     terms_of(dtype, weighted, na, nb);

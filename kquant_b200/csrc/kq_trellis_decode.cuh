@@ -8,7 +8,8 @@
 // neighbouring rows: a packed pair along the contraction axis.
 // Labels: MCG is computed (a multiply, a logic op, half an add); E4M3 and
 // binary16 tables are looked up in shared memory, where 32 random lookups
-// meet about 3.5-fold bank conflicts.
+// take 3.5 cycles (13.1 million for the 3.76 million load instructions of 8
+// experts of 7168 x 2048 at 3 bits, one row each).
 #pragma once
 #include "kq_expert.cuh"
 

@@ -5,7 +5,9 @@
 // of the tile), so a decoded tile goes from registers into the products of up
 // to 64 rows without touching memory.  Decoding is what bounds this (the
 // products of 64 rows take half of its time even on mma.sync), at three bits:
-// label lookups in shared memory for the tables, integer arithmetic for MCG.
+// label lookups in shared memory for the tables (E4M3: 83% of its cycles),
+// integer arithmetic for MCG (8 experts of 7168 x 4096 at 4 bits, one row
+// each: 104 us, ALU pipe 71%, issue slots 62%, DRAM idle for the most part).
 //
 // The work is dealt to a persistent grid of two CTAs an SM in equal shares of
 // k tiles, wherever strips of columns end: with whole strips the last round
